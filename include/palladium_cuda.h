@@ -64,7 +64,14 @@ typedef enum pd_family {
                                     handing the handler MSL source + entry-point name, native/ffi/palladium_ffi.cpp:136-148 */
     PD_FAMILY_SOURCE = 9,        /* a complete caller-written kernel: source text + entry-point name, the
                                     attributes of the reference handler itself, native/ffi/palladium_ffi.cpp:110-117 */
-    PD_FAMILY_COUNT = 10
+    /* driven linear ensembles (state-space layers); no counterpart in the reference */
+    PD_FAMILY_CAUSAL_CONV = 10,
+    PD_FAMILY_CAUSAL_CONV_STEP = 11,
+    PD_FAMILY_CAUSAL_CONV_GRAD = 12,
+    PD_FAMILY_SELECTIVE_SCAN = 13,
+    PD_FAMILY_SELECTIVE_SCAN_STEP = 14,
+    PD_FAMILY_SELECTIVE_SCAN_GRAD = 15,
+    PD_FAMILY_COUNT = 16
 } pd_family;
 
 /* ---- per-family parameter blocks (passed by pointer + sizeof) ------------ */
@@ -199,6 +206,54 @@ typedef struct pd_source_kernel_params {
     const char* cuda_source;     /* NUL-terminated; must stay valid for the call only */
     const char* function_name;   /* at most 63 bytes */
 } pd_source_kernel_params;
+
+/* ---- state-space families ---------------------------------------------------
+ * grid = (sequences S, channels D).  Token arrays hold elements of `type`
+ * (PD_TYPE_*), row-major: (S, length, D) for a dense call; for a packed one
+ * (length, D), `length` rows in all, sequence s in rows [offsets[s],
+ * offsets[s + 1]) with int32 offsets (S + 1).  Offsets are clamped to
+ * [0, length] and a decreasing pair is an empty sequence; output rows of no
+ * sequence are zero.  Parameters and recurrent states are float32.  Arithmetic
+ * is float32, rounded once at the store.  Zero values in a flag leave the
+ * operands and results in [ ] out.  Scratch for the gradients' partial sums
+ * comes from `workspace`, or from the library's pool, which a stream that is
+ * being captured into a graph cannot use. */
+#define PD_TYPE_F32 0
+#define PD_TYPE_F16 1
+#define PD_TYPE_BF16 2
+
+/* y_t = act(bias + sum_{j < width} weight[:, width-1-j] x_{t-j}), act = v / (1 + e^-v) with `silu`.
+ * Inputs before a sequence's first token come from `initial`, else are zero;
+ * `final` receives a sequence's last width-1 inputs.  width 2..4.
+ *   CAUSAL_CONV       in: x, weight (D, width) f32 [, bias (D) f32] [, initial (S, width-1, D)] [, offsets]
+ *                     out: y [, final (S, width-1, D)]
+ *   CAUSAL_CONV_STEP  in: x (S, D), state (S, width-1, D), weight [, bias]   out: y, state (may be the input's memory)
+ *   CAUSAL_CONV_GRAD  in: dy, x, weight [, bias] [, initial] [, dfinal] [, offsets]
+ *                     out: dx, dweight f32 [, dbias f32] [, dinitial] */
+typedef struct pd_causal_conv_params {
+    int64_t length, width, type;
+    int64_t silu, bias, initial, final, packed;
+} pd_causal_conv_params;
+
+/* d = softplus(delta + bias), h_t = exp(d A) h_{t-1} + d x_t B_t, y_t = (C_t h_t + skip x_t) * z / (1 + e^-z):
+ * the ensemble h' = A h + B(t) x(t) integrated exactly over steps of length d with B, x held constant.
+ * N = `state` (1..64) states per channel; channel c reads group c / (D / groups) of B and C.
+ *   SELECTIVE_SCAN       in: x, delta, A (D, N) f32, B (S, length, groups, N), C [, bias (D) f32] [, skip (D) f32]
+ *                            [, z] [, initial (S, D, N) f32] [, offsets]
+ *                        out: y [, final (S, D, N) f32] [, carries (chunks, D, N) f32]
+ *   SELECTIVE_SCAN_STEP  in: state (S, D, N) f32, x (S, D), delta, A, B (S, groups, N), C [, bias] [, skip] [, z]
+ *                        out: y, state (may be the input's memory)
+ *   SELECTIVE_SCAN_GRAD  in: dy, x, delta, A, B, C [, bias] [, skip] [, z], carries [, dfinal f32] [, offsets]
+ *                        out: dx, ddelta, dA f32, dB, dC [, dbias f32] [, dskip f32] [, dz] [, dinitial f32]
+ * carries: the state entering every PD_SCAN_CHUNK-th token of a sequence, what the gradient recomputes from;
+ * chunks = S * ceil(length / PD_SCAN_CHUNK), packed: length / PD_SCAN_CHUNK + S, sequence s from entry
+ * offsets[s] / PD_SCAN_CHUNK + s on (entries of no chunk are not written). */
+#define PD_SCAN_CHUNK 64
+#define PD_SCAN_MAX_STATE 64
+typedef struct pd_selective_scan_params {
+    int64_t length, state, groups, type;
+    int64_t softplus, bias, skip, gate, initial, final, carries, packed;
+} pd_selective_scan_params;
 
 /* ---- launch geometry report (the `.explain()` payload) -------------------- */
 typedef struct pd_launch_info {

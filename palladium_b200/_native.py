@@ -77,6 +77,12 @@ FAMILY_IDS = {
     "gbm_pcg": 7,
     "custom_ode": 8,
     "source": 9,
+    "causal_conv": 10,
+    "causal_conv_step": 11,
+    "causal_conv_grad": 12,
+    "selective_scan": 13,
+    "selective_scan_step": 14,
+    "selective_scan_grad": 15,
 }
 
 _i64 = ctypes.c_int64
@@ -124,6 +130,15 @@ class CustomOdeParams(ctypes.Structure):
 
 class SourceKernelParams(ctypes.Structure):
     _fields_ = [("cuda_source", ctypes.c_char_p), ("function_name", ctypes.c_char_p)]
+
+
+class CausalConvParams(ctypes.Structure):
+    _fields_ = [(name, _i64) for name in ("length", "width", "type", "silu", "bias", "initial", "final", "packed")]
+
+
+class SelectiveScanParams(ctypes.Structure):
+    _fields_ = [(name, _i64) for name in ("length", "state", "groups", "type", "softplus", "bias", "skip", "gate",
+                                          "initial", "final", "carries", "packed")]
 
 
 class GsNeighbours(ctypes.Structure):

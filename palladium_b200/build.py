@@ -1,6 +1,6 @@
 """Build recipe for libpalladium_cuda.so (sm_100a only).
 
-The kernel translation unit is compiled three times, once per math mode, each
+The kernel translation units (pd_kernels.cu, pd_scan.cu) are compiled three times, once per math mode, each
 with the nvcc flag set that *is* that mode's definition (the reference selects
 the mode when it compiles MSL: `mr.Kernel(msl, name, math_mode=...)`,
 src/palladium/dispatch.py:290; here the three variants are built ahead of time):
@@ -79,10 +79,14 @@ def build(verbose: bool = False, force: bool = False) -> Path:
     for mode, flags in MODE_FLAGS.items():
         obj = BUILD_DIR / f"pd_kernels_{mode}.o"
         jobs.append(([nvcc, *ARCH, *COMMON, *flags, *extra, "-c", str(CSRC / "pd_kernels.cu"), "-o", str(obj)], obj))
+        scan_obj = BUILD_DIR / f"pd_scan_{mode}.o"
+        jobs.append(([nvcc, *ARCH, *COMMON, *flags, *extra, "-c", str(CSRC / "pd_scan.cu"), "-o", str(scan_obj)], scan_obj))
     api_obj = BUILD_DIR / "pd_api.o"
     jobs.append(([nvcc, *ARCH, *COMMON, "-c", str(CSRC / "pd_api.cu"), "-o", str(api_obj)], api_obj))
     noalloc_obj = BUILD_DIR / "pd_noalloc.o"
     jobs.append(([nvcc, *ARCH, *COMMON, "-c", str(CSRC / "pd_noalloc.cu"), "-o", str(noalloc_obj)], noalloc_obj))
+    scan_api_obj = BUILD_DIR / "pd_scan_api.o"
+    jobs.append(([nvcc, *ARCH, *COMMON, "-c", str(CSRC / "pd_scan_api.cu"), "-o", str(scan_api_obj)], scan_api_obj))
     rtc_obj = BUILD_DIR / "pd_rtc.o"
     jobs.append(([nvcc, *ARCH, *COMMON, f"-I{BUILD_DIR}", "-c", str(CSRC / "pd_rtc.cu"), "-o", str(rtc_obj)], rtc_obj))
     with ThreadPoolExecutor(max_workers=len(jobs)) as pool:

@@ -20,35 +20,39 @@ from typing import Any
 
 import numpy as np
 
-from .diagnostics import KernelDiagnostics, explain_spec, log_compile
+from .diagnostics import KernelDiagnostics, explain_spec, log_compile, source_name
 from .dispatch import BoundKernel, PendingResult, bind
 from .errors import DispatchError, UnsupportedPrimitiveError
-from .families import Family, trace
+from .families import STATE_SPACE, Family, trace
 from .interpret import interpret_callable
 from .math_mode import MathMode, math_mode_ordinal
+from .pl import as_dtype, dtype_name
 
 # Element types the kernels take (the reference's table is emit.core.CTYPES).
 SUPPORTED_DTYPES = ("float32", "uint32", "int32")
+# ... and what the tokens of the state-space families may be besides
+SHORT_DTYPES = ("float16", "bfloat16")
 
 Signature = tuple[tuple[tuple[int, ...], str], ...]
 
 
-def require_supported_dtypes(operands) -> None:
+def require_supported_dtypes(operands, family: Family | None = None) -> None:
     """Refuse element types no kernel takes, before anything is traced, and say
     what to do about the usual culprit (the wording users of the reference know,
     src/palladium/__init__.py:58-80)."""
+    supported = SUPPORTED_DTYPES + (SHORT_DTYPES if family is not None and family.name in STATE_SPACE else ())
     names = []
     for operand in operands:
         dtype = getattr(operand, "dtype", None)
-        names.append(np.dtype(np.asarray(operand).dtype if dtype is None else dtype).name)
+        names.append(dtype_name(as_dtype(np.asarray(operand).dtype if dtype is None else dtype)))
     for position, name in enumerate(names):
-        if name in SUPPORTED_DTYPES:
+        if name in supported:
             continue
         advice = ""
         if name == "float64":
             advice = "; float64 usually means jax_enable_x64 is on, disable it or cast to float32"
         raise DispatchError(f"argument {position} has dtype {name}, which palladium cannot lower "
-                            f"(supported: {', '.join(SUPPORTED_DTYPES)}){advice}")
+                            f"(supported: {', '.join(supported)}){advice}")
 
 
 def signature_of(arrays) -> Signature:
@@ -105,7 +109,7 @@ class CudaCallable:
 
     # -- binding ----------------------------------------------------------------------
     def _bind_for(self, arrays: list[np.ndarray]) -> BoundKernel:
-        require_supported_dtypes(arrays)
+        require_supported_dtypes(arrays, self._family)
         spec = trace(self._family, self._pallas_kwargs, *arrays)
         log_compile(spec, self._threadgroup, self._math_mode)
         return bind(spec, math_mode=self._math_mode, threadgroup=self._threadgroup)
@@ -134,7 +138,7 @@ class CudaCallable:
     def explain(self, *args) -> KernelDiagnostics:
         """The launch these inputs would get.  `args` may be arrays or
         ShapeDtypeStructs; no data is read and nothing is launched."""
-        require_supported_dtypes(args)
+        require_supported_dtypes(args, self._family)
         return explain_spec(trace(self._family, self._pallas_kwargs, *args), self._threadgroup, self._math_mode)
 
 
@@ -174,4 +178,4 @@ def debug_msl(kernel: Family, *example_args, **pallas_kwargs) -> str:
     if kernel.name == "source":
         return header + kernel.constants["source"]
     return (header + f"// family: {kernel.name}\n// constants: {kernel.constants}\n"
-            "// source: palladium_b200/csrc/pd_kernels.cu\n")
+            f"// source: {source_name(spec)}\n")

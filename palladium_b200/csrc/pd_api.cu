@@ -6,6 +6,7 @@
 #include "../../include/palladium_cuda.h"
 #include "pd_kernels.h"
 #include "pd_rtc.h"
+#include "pd_scan.h"
 
 #include <cuda_runtime.h>
 #include <math.h>
@@ -225,6 +226,7 @@ struct Plan {
     int64_t dynamic_smem = 0;      // bytes of dynamic shared memory per block (the tiled stencil kernels)
     const void* kernel = nullptr;
     PdRtcKernel rtc;               // run-time compiled families only
+    PdScanPlan scan;               // state-space families only
 };
 
 int requested_block(const int64_t block[3]) {
@@ -294,6 +296,18 @@ int build_plan(int family, const void* params, size_t params_bytes, int math_mod
     if (!grid) return fail(PD_ERR_INVALID_ARGUMENT, err, err_cap, "grid must not be NULL");
     for (int i = 0; i < 3; ++i)
         if (grid[i] < 0) return fail(PD_ERR_INVALID_ARGUMENT, err, err_cap, "grid[%d] is negative", i);
+    if (pd_is_scan_family(family)) {
+        int rc = pd_scan_plan(family, params, params_bytes, grid, block, dev.sms, &plan->scan, err, err_cap);
+        if (rc) return rc;
+        plan->kernel_name = plan->scan.kernel_name;
+        plan->grid[0] = plan->scan.grid;
+        plan->block[0] = plan->scan.block;
+        plan->items = plan->scan.items;
+        plan->launches = plan->scan.launches;
+        plan->scratch_bytes = plan->scan.scratch_bytes;
+        plan->dynamic_smem = plan->scan.dynamic_smem;
+        return PD_OK;
+    }
     const PdModeTable* mt = mode_table(math_mode);
     const int req_block = requested_block(block);
     if (req_block && family != PD_FAMILY_SOURCE) {
@@ -690,8 +704,13 @@ int launch_impl(int family, const void* params, size_t params_bytes, int math_mo
     if (rc) return rc;
     if (family != PD_FAMILY_SOURCE) {   // a caller-written kernel defines its own buffer sizes
         std::vector<size_t> want_in, want_out;
-        rc = expected_sizes(family, params, grid, &want_in, &want_out, n_in, n_out, err, err_cap);
-        if (rc) return rc;
+        if (pd_is_scan_family(family)) {
+            want_in.swap(plan.scan.in_bytes);
+            want_out.swap(plan.scan.out_bytes);
+        } else {
+            rc = expected_sizes(family, params, grid, &want_in, &want_out, n_in, n_out, err, err_cap);
+            if (rc) return rc;
+        }
         rc = check_buffers("input", n_in, (int)want_in.size(), in_bytes, want_in.data(), in, err, err_cap);
         if (rc) return rc;
         rc = check_buffers("output", n_out, (int)want_out.size(), out_bytes, want_out.data(),
@@ -716,6 +735,15 @@ int launch_impl(int family, const void* params, size_t params_bytes, int math_mo
                 return fail(PD_ERR_INVALID_ARGUMENT, err, err_cap, "workspace must be 256-byte aligned");
             scratch = workspace;
         } else {
+            if (pd_is_scan_family(family)) {
+                // a captured graph would keep pointing into the pool, which may free its buffer later
+                cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+                PD_CUDA_TRY(cudaStreamIsCapturing(st, &capturing));
+                if (capturing != cudaStreamCaptureStatusNone)
+                    return fail(PD_ERR_INVALID_ARGUMENT, err, err_cap,
+                                "a call with %lld bytes of scratch needs a workspace of its own on a stream that is being captured",
+                                (long long)plan.scratch_bytes);
+            }
             PD_CUDA_TRY(scratch_get(dev.device, (void*)st, (size_t)plan.scratch_bytes, &scratch));
         }
     }
@@ -978,6 +1006,11 @@ int launch_impl(int family, const void* params, size_t params_bytes, int math_mo
             break;
         }
         default:
+            if (pd_is_scan_family(family)) {
+                rc = pd_scan_launch(family, params, math_mode, grid, plan.scan, in, out, scratch, st, err, err_cap);
+                if (rc) return rc;
+                break;
+            }
             return fail(PD_ERR_INVALID_ARGUMENT, err, err_cap, "unknown kernel family %d", family);
     }
 

@@ -1,0 +1,799 @@
+// pd_scan.cu -- the CUDA kernels of the state-space families: a short causal
+// convolution over a sequence's tokens and the selective scan, the exact
+// integration of an ensemble of driven linear systems
+//     h' = A h + B(t) x(t),   y = C(t) h + D x
+// over steps of input-dependent length, one trajectory per (sequence, channel).
+// Compiled once per math mode like pd_kernels.cu: SAFE and RELAXED use the
+// library's expf / log1pf and IEEE division, FAST the approximate ones.
+//
+// Everything is computed in float32 whatever the element type; a result is
+// rounded once, where it is stored.
+#include "pd_scan.h"
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "../../include/palladium_cuda.h"
+
+#ifndef PD_MODE
+#error "PD_MODE must be 0 (SAFE), 1 (RELAXED) or 2 (FAST)"
+#endif
+#if PD_MODE == 0
+#define PD_SCAN_TABLE pd_scan_table_safe
+#elif PD_MODE == 1
+#define PD_SCAN_TABLE pd_scan_table_relaxed
+#else
+#define PD_SCAN_TABLE pd_scan_table_fast
+#endif
+
+namespace {
+
+constexpr unsigned kFull = 0xFFFFFFFFu;
+constexpr int kStates = 4;     // states per thread
+
+// ---------------------------------------------------------------------------
+// elements
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float load1(const float* p) { return *p; }
+__device__ __forceinline__ float load1(const __half* p) { return __half2float(*p); }
+__device__ __forceinline__ float load1(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void store1(float* p, float v) { *p = v; }
+__device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+
+// V consecutive elements; V > 1 means one 16-byte access
+template <int V, class T>
+__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
+    if constexpr (V == 1) {
+        v[0] = load1(p);
+    } else {
+        static_assert(V * sizeof(T) == 16, "a vector is 16 bytes");
+        union { uint4 raw; T e[V]; } u;
+        u.raw = *reinterpret_cast<const uint4*>(p);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = load1(&u.e[i]);
+    }
+}
+template <int V, class T>
+__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+    if constexpr (V == 1) {
+        store1(p, v[0]);
+    } else {
+        union { uint4 raw; T e[V]; } u;
+#pragma unroll
+        for (int i = 0; i < V; ++i) store1(&u.e[i], v[i]);
+        *reinterpret_cast<uint4*>(p) = u.raw;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// functions
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ float exp_(float v) {
+#if PD_MODE == 2
+    return __expf(v);
+#else
+    return expf(v);
+#endif
+}
+__device__ __forceinline__ float sigmoid_(float v) {
+#if PD_MODE == 2
+    return __fdividef(1.0f, 1.0f + __expf(-v));
+#else
+    return 1.0f / (1.0f + expf(-v));
+#endif
+}
+// log(1 + e^v) without cancellation: a step size of 1e-3 is as exact as one of 10
+__device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.0f) + log1pf(exp_(-fabsf(v))); }
+
+// ---------------------------------------------------------------------------
+// sequences
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t rows) { return v < 0 ? 0 : (v > rows ? rows : v); }
+__device__ __forceinline__ void bounds_of(const PdTokens& t, int64_t s, int64_t& begin, int64_t& end) {
+    if (!t.offsets) {
+        begin = s * t.length;
+        end = begin + t.length;
+        return;
+    }
+    begin = clamp_row(t.offsets[s], t.rows);
+    end = clamp_row(t.offsets[s + 1], t.rows);
+    if (end < begin) end = begin;
+}
+// The sequence that has `row`: true with its bounds, or false (rows before the first or behind the last one).
+__device__ __forceinline__ bool sequence_of(const PdTokens& t, int64_t row, int64_t& s, int64_t& begin, int64_t& end) {
+    if (!t.offsets) {
+        s = row / t.length;
+        begin = s * t.length;
+        end = begin + t.length;
+        return true;
+    }
+    int64_t lo = 0, hi = t.seqs;   // the last s with offsets[s] <= row
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if ((int64_t)t.offsets[mid] <= row) lo = mid + 1; else hi = mid;
+    }
+    s = lo - 1;
+    if (s < 0) return false;
+    bounds_of(t, s, begin, end);
+    return begin <= row && row < end;
+}
+// f(row) for the rows before the first and behind the last sequence of a packed call
+template <class F>
+__device__ __forceinline__ void for_free_rows(const PdTokens& t, F f) {
+    const int64_t head = clamp_row(t.offsets[0], t.rows), tail = clamp_row(t.offsets[t.seqs], t.rows);
+    for (int64_t r = 0; r < head; ++r) f(r);
+    for (int64_t r = tail < head ? head : tail; r < t.rows; ++r) f(r);
+}
+// where the state entering each chunk of a sequence is kept
+__device__ __forceinline__ int64_t first_chunk(const PdTokens& t, int64_t s, int64_t begin) {
+    return t.offsets ? begin / PD_SCAN_CHUNK + s : s * ((t.length + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK);
+}
+
+// ===========================================================================
+// causal convolution:  y_t = act(bias + sum_j w[W-1-j] x_{t-j})
+// One thread owns V channels and a run of consecutive rows; the last W - 1
+// inputs stay in registers, so a row is read once apart from the run's halo.
+// ===========================================================================
+template <class T, int W, int V>
+__device__ __forceinline__ void conv_window(const PdConvArgs& a, const T* x, int64_t s, int64_t begin, int64_t row,
+                                            int64_t c, float (&win)[W - 1][V]) {
+    // the W - 1 inputs before `row`, oldest first
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        const int64_t r = row - (W - 1) + i;
+        if (r >= begin) {
+            load<V>(x + r * a.channels + c, win[i]);
+        } else if (a.initial) {
+            load<V>((const T*)a.initial + (s * (W - 1) + (W - 1) + (r - begin)) * a.channels + c, win[i]);
+        } else {
+#pragma unroll
+            for (int v = 0; v < V; ++v) win[i][v] = 0.0f;
+        }
+    }
+}
+
+template <class T, int W, int V>
+__global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
+    const int64_t lanes = (a.channels + V - 1) / V;
+    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t c = id % lanes * V;
+    int64_t row = id / lanes * a.run;
+    const int64_t runs = (a.tok.rows + a.run - 1) / a.run;
+    const T* x = (const T*)a.x;
+    if (id / lanes >= runs) {
+        // one more job per sequence: an empty one hands its carried-in inputs on
+        const int64_t s = id / lanes - runs;
+        if (!a.final_state || s >= a.tok.seqs) return;
+        int64_t begin, end;
+        bounds_of(a.tok, s, begin, end);
+        if (begin < end) return;
+        float v[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = 0.0f;
+        for (int i = 0; i < W - 1; ++i) {
+            const int64_t at = (s * (W - 1) + i) * a.channels + c;
+            if (a.initial) load<V>((const T*)a.initial + at, v);
+            store<V>((T*)a.final_state + at, v);
+        }
+        return;
+    }
+    float w[W][V], b[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) w[k][v] = a.weight[(c + v) * W + k];
+        b[v] = a.bias ? a.bias[c + v] : 0.0f;
+    }
+    const int64_t stop = row + a.run < a.tok.rows ? row + a.run : a.tok.rows;
+    int64_t s = 0, begin = 0, end = 0;
+    float win[W - 1][V];
+    while (row < stop) {
+        if (!sequence_of(a.tok, row, s, begin, end)) {
+            float zero[V];
+#pragma unroll
+            for (int v = 0; v < V; ++v) zero[v] = 0.0f;
+            store<V>((T*)a.y + row * a.channels + c, zero);
+            ++row;
+            continue;
+        }
+        conv_window<T, W, V>(a, x, s, begin, row, c, win);
+        const int64_t upto = end < stop ? end : stop;
+        for (; row < upto; ++row) {
+            float now[V], out[V];
+            load<V>(x + row * a.channels + c, now);
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float acc = b[v];
+#pragma unroll
+                for (int i = 0; i < W - 1; ++i) acc += w[i][v] * win[i][v];
+                acc += w[W - 1][v] * now[v];
+                out[v] = a.silu ? acc * sigmoid_(acc) : acc;
+#pragma unroll
+                for (int i = 0; i + 1 < W - 1; ++i) win[i][v] = win[i + 1][v];
+                win[W - 2][v] = now[v];
+            }
+            store<V>((T*)a.y + row * a.channels + c, out);
+        }
+        if (row == end && a.final_state)
+#pragma unroll
+            for (int i = 0; i < W - 1; ++i)
+                store<V>((T*)a.final_state + (s * (W - 1) + i) * a.channels + c, win[i]);
+    }
+}
+
+// one token per sequence: the window comes from and goes to the state (which may be the same memory)
+template <class T, int W, int V>
+__global__ void __launch_bounds__(256) pd_causal_conv_step_kernel(PdConvArgs a) {
+    const int64_t lanes = (a.channels + V - 1) / V;
+    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t s = id / lanes, c = id % lanes * V;
+    if (s >= a.tok.seqs) return;
+    float win[W][V], out[V];
+    const int64_t at = s * (W - 1) * a.channels + c;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) load<V>((const T*)a.initial + at + i * a.channels, win[i]);
+    load<V>((const T*)a.x + s * a.channels + c, win[W - 1]);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        float acc = a.bias ? a.bias[c + v] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) acc += a.weight[(c + v) * W + k] * win[k][v];
+        out[v] = a.silu ? acc * sigmoid_(acc) : acc;
+    }
+    store<V>((T*)a.y + s * a.channels + c, out);
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) store<V>((T*)a.final_state + at + i * a.channels, win[i + 1]);
+}
+
+// Gradients.  With g_t = dy_t act'(pre_t):
+//   dx_t = sum_j w[W-1-j] g_{t+j},   dw[W-1-j] = sum_t x_{t-j} g_t,   dbias = sum_t g_t
+// A thread walks its run and W - 1 rows beyond it, and keeps the W gradients of dx still open; sums of
+// dw and dbias stay in registers, then go to one partial per block, which a second launch adds up in order.
+template <class T, int W, int V>
+__global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) {
+    const int64_t lanes = (a.channels + V - 1) / V;
+    // blockDim.x threads across channels, blockDim.y across runs; blockIdx.x channel blocks, blockIdx.y row blocks
+    const int64_t lane = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t c = lane * V;
+    const bool active = lane < lanes;
+    const T* x = (const T*)a.x;
+    const T* dy = (const T*)a.dy;
+    float w[W][V], b[V], dw[W][V], db[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) {
+            w[k][v] = active ? a.weight[(c + v) * W + k] : 0.0f;
+            dw[k][v] = 0.0f;
+        }
+        b[v] = active && a.bias ? a.bias[c + v] : 0.0f;
+        db[v] = 0.0f;
+    }
+    const int64_t runs = (a.tok.rows + a.run - 1) / a.run;
+    const int64_t jobs = runs + (a.dinitial ? a.tok.seqs : 0);
+    for (int64_t job = (int64_t)blockIdx.y * blockDim.y + threadIdx.y; active && job < jobs;
+         job += (int64_t)gridDim.y * blockDim.y) {
+        if (job >= runs) {
+            // an empty sequence hands the gradient of its carried-out inputs back
+            const int64_t s = job - runs;
+            int64_t begin, end;
+            bounds_of(a.tok, s, begin, end);
+            if (begin < end) continue;
+            float v[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = 0.0f;
+            for (int i = 0; i < W - 1; ++i) {
+                const int64_t at = (s * (W - 1) + i) * a.channels + c;
+                if (a.dfinal) load<V>((const T*)a.dfinal + at, v);
+                store<V>((T*)a.dinitial + at, v);
+            }
+            continue;
+        }
+        int64_t row = job * a.run;
+        const int64_t stop = row + a.run < a.tok.rows ? row + a.run : a.tok.rows;
+        while (row < stop) {
+            int64_t s, begin, end;
+            if (!sequence_of(a.tok, row, s, begin, end)) {
+                float zero[V];
+#pragma unroll
+                for (int v = 0; v < V; ++v) zero[v] = 0.0f;
+                store<V>((T*)a.dx + row * a.channels + c, zero);
+                ++row;
+                continue;
+            }
+            float win[W - 1][V], open[W][V];   // open[j]: gradient of the input j rows back from the current one
+            conv_window<T, W, V>(a, x, s, begin, row, c, win);
+#pragma unroll
+            for (int j = 0; j < W; ++j)
+#pragma unroll
+                for (int v = 0; v < V; ++v) open[j][v] = 0.0f;
+            const int64_t mine = end < stop ? end : stop;                        // rows whose sums belong here
+            const int64_t upto = mine + (W - 1) < end ? mine + (W - 1) : end;    // rows whose g they need
+            const int64_t from = row;
+            for (; row < upto; ++row) {
+                float now[V], g[V];
+                load<V>(x + row * a.channels + c, now);
+                load<V>(dy + row * a.channels + c, g);
+#pragma unroll
+                for (int v = 0; v < V; ++v) {
+                    if (a.silu) {
+                        float pre = b[v];
+#pragma unroll
+                        for (int i = 0; i < W - 1; ++i) pre += w[i][v] * win[i][v];
+                        pre += w[W - 1][v] * now[v];
+                        const float sig = sigmoid_(pre);
+                        g[v] *= sig * (1.0f + pre * (1.0f - sig));
+                    }
+#pragma unroll
+                    for (int j = W - 1; j > 0; --j) open[j][v] = open[j - 1][v] + w[W - 1 - j][v] * g[v];
+                    open[0][v] = w[W - 1][v] * g[v];
+                    if (row < mine) {
+                        db[v] += g[v];
+#pragma unroll
+                        for (int i = 0; i < W - 1; ++i) dw[i][v] += win[i][v] * g[v];
+                        dw[W - 1][v] += now[v] * g[v];
+                    }
+#pragma unroll
+                    for (int i = 0; i + 1 < W - 1; ++i) win[i][v] = win[i + 1][v];
+                    win[W - 2][v] = now[v];
+                }
+                // the input W - 1 rows back is complete
+                const int64_t done = row - (W - 1);
+                if (done >= from) store<V>((T*)a.dx + done * a.channels + c, open[W - 1]);
+                else if (done < begin && from == begin && a.dinitial) {
+                    // (a carried-in input that is carried out again is still open at the end, below)
+                    store<V>((T*)a.dinitial + (s * (W - 1) + (done - begin) + (W - 1)) * a.channels + c, open[W - 1]);
+                }
+            }
+            if (row == end) {
+                // the sequence ends here: the inputs still open are complete, and were carried out
+#pragma unroll
+                for (int j = W - 2; j >= 0; --j) {
+                    const int64_t r = end - 1 - j;
+                    float v[V];
+#pragma unroll
+                    for (int u = 0; u < V; ++u) v[u] = open[j][u];
+                    if (a.dfinal) {
+                        float f[V];
+                        load<V>((const T*)a.dfinal + (s * (W - 1) + (W - 2 - j)) * a.channels + c, f);
+#pragma unroll
+                        for (int u = 0; u < V; ++u) v[u] += f[u];
+                    }
+                    if (r >= from && r < mine) store<V>((T*)a.dx + r * a.channels + c, v);
+                    else if (r < begin && from == begin && a.dinitial)
+                        store<V>((T*)a.dinitial + (s * (W - 1) + (r - begin) + (W - 1)) * a.channels + c, v);
+                }
+            }
+            row = mine;
+        }
+    }
+    // block sums, in the order of the runs
+    extern __shared__ float sums[];   // (blockDim.y, blockDim.x, V)
+    for (int k = 0; k <= W; ++k) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            float mine = db[v];
+#pragma unroll
+            for (int q = 0; q < W; ++q) if (q == k) mine = dw[q][v];
+            sums[(threadIdx.y * blockDim.x + threadIdx.x) * V + v] = mine;
+        }
+        __syncthreads();
+        if (threadIdx.y == 0 && active)
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                float total = 0.0f;
+                for (int y = 0; y < (int)blockDim.y; ++y) total += sums[(y * blockDim.x + threadIdx.x) * V + v];
+                a.partial[((int64_t)blockIdx.y * a.channels + c + v) * (W + 1) + k] = total;
+            }
+        __syncthreads();
+    }
+}
+
+template <int W>
+__global__ void __launch_bounds__(128) pd_causal_conv_sum_kernel(PdConvArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= a.channels * (W + 1)) return;
+    float total = 0.0f;
+    for (int64_t b = 0; b < a.row_blocks; ++b) total += a.partial[b * a.channels * (W + 1) + i];
+    const int64_t c = i / (W + 1), k = i % (W + 1);
+    if (k < W) a.dweight[c * W + k] = total;
+    else if (a.dbias) a.dbias[c] = total;
+}
+
+// ===========================================================================
+// selective scan:  d = softplus(delta + bias),  h = exp(d A) h + d x B,  y = (C h + skip x) silu(z)
+// LN neighbouring lanes share a channel, four states each.
+// ===========================================================================
+template <class T>
+__device__ __forceinline__ void load_states(const T* p, int first, int n, float (&v)[kStates]) {
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) v[i] = first + i < n ? load1(p + first + i) : 0.0f;
+}
+
+template <int LN>
+__device__ __forceinline__ float sum_lanes(float v) {
+#pragma unroll
+    for (int m = 1; m < LN; m *= 2) v += __shfl_xor_sync(kFull, v, m);
+    return v;
+}
+
+// a warp's tile: 32 / LN channels of one group
+struct ScanTile { int64_t channel; int group; bool active; };
+template <int LN>
+__device__ __forceinline__ ScanTile scan_tile(const PdScanArgs& a, int64_t tile) {
+    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch;
+    ScanTile t;
+    t.group = (int)(tile / tiles);
+    const int64_t within = tile % tiles * ch + (threadIdx.x & 31) / LN;
+    t.active = within < per;
+    t.channel = t.group * per + (t.active ? within : per - 1);   // an idle lane repeats the last channel, stores nothing
+    return t;
+}
+
+template <class T, int LN>
+__global__ void __launch_bounds__(128) pd_selective_scan_kernel(PdScanArgs a) {
+    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch * a.groups;
+    const int64_t job = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int64_t s = job / tiles;
+    const int lane = threadIdx.x & 31, sub = lane % LN, first = sub * kStates;
+    if (s > a.tok.seqs || (s == a.tok.seqs && !a.tok.offsets)) return;
+    const ScanTile tile = scan_tile<LN>(a, job % tiles);
+    const int64_t c = tile.channel;
+    if (s == a.tok.seqs) {
+        for_free_rows(a.tok, [&](int64_t r) {
+            if (tile.active && sub == 0) store1((T*)a.y + r * a.channels + c, 0.0f);
+        });
+        return;
+    }
+    int64_t begin, end;
+    bounds_of(a.tok, s, begin, end);
+    float A[kStates], h[kStates];
+    load_states(a.A + c * a.state, first, a.state, A);
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) h[i] = 0.0f;
+    const int64_t state_at = (s * a.channels + c) * a.state;
+    if (a.initial) load_states(a.initial + state_at, first, a.state, h);
+    const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
+    int64_t chunk = first_chunk(a.tok, s, begin);
+    for (int64_t r = begin; r < end; ++r) {
+        if (a.carries && (r - begin) % PD_SCAN_CHUNK == 0) {
+            if (tile.active)
+                for (int i = 0; i < kStates; ++i)
+                    if (first + i < a.state) a.carries[(chunk * a.channels + c) * a.state + first + i] = h[i];
+            ++chunk;
+        }
+        const float x = load1((const T*)a.x + r * a.channels + c);
+        float d = load1((const T*)a.delta + r * a.channels + c) + bias;
+        if (a.softplus) d = softplus_(d);
+        const float u = d * x;
+        float B[kStates], C[kStates], y = 0.0f;
+        const int64_t bc = (r * a.groups + tile.group) * a.state;
+        load_states((const T*)a.B + bc, first, a.state, B);
+        load_states((const T*)a.C + bc, first, a.state, C);
+#pragma unroll
+        for (int i = 0; i < kStates; ++i) {
+            h[i] = exp_(d * A[i]) * h[i] + (first + i < a.state ? u * B[i] : 0.0f);
+            y += first + i < a.state ? C[i] * h[i] : 0.0f;
+        }
+        y = sum_lanes<LN>(y);
+        if (a.skip) y += skip * x;
+        if (a.z) {
+            const float z = load1((const T*)a.z + r * a.channels + c);
+            y *= z * sigmoid_(z);
+        }
+        if (tile.active && sub == 0) store1((T*)a.y + r * a.channels + c, y);
+    }
+    if (a.final_state && tile.active)
+        for (int i = 0; i < kStates; ++i)
+            if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
+}
+
+// one token per sequence; state in and out may be the same memory
+template <class T, int LN>
+__global__ void __launch_bounds__(128) pd_selective_scan_step_kernel(PdScanArgs a) {
+    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch * a.groups;
+    const int64_t job = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int64_t s = job / tiles;
+    if (s >= a.tok.seqs) return;
+    const int lane = threadIdx.x & 31, sub = lane % LN, first = sub * kStates;
+    const ScanTile tile = scan_tile<LN>(a, job % tiles);
+    const int64_t c = tile.channel, state_at = (s * a.channels + c) * a.state;
+    float A[kStates], B[kStates], C[kStates], h[kStates];
+    load_states(a.A + c * a.state, first, a.state, A);
+    load_states(a.initial + state_at, first, a.state, h);
+    const int64_t bc = (s * a.groups + tile.group) * a.state;
+    load_states((const T*)a.B + bc, first, a.state, B);
+    load_states((const T*)a.C + bc, first, a.state, C);
+    const float x = load1((const T*)a.x + s * a.channels + c);
+    float d = load1((const T*)a.delta + s * a.channels + c) + (a.bias ? a.bias[c] : 0.0f);
+    if (a.softplus) d = softplus_(d);
+    const float u = d * x;
+    float y = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) {
+        h[i] = exp_(d * A[i]) * h[i] + (first + i < a.state ? u * B[i] : 0.0f);
+        y += first + i < a.state ? C[i] * h[i] : 0.0f;
+    }
+    y = sum_lanes<LN>(y);
+    if (a.skip) y += a.skip[c] * x;
+    if (a.z) {
+        const float z = load1((const T*)a.z + s * a.channels + c);
+        y *= z * sigmoid_(z);
+    }
+    if (!tile.active) return;
+    if (sub == 0) store1((T*)a.y + s * a.channels + c, y);
+    for (int i = 0; i < kStates; ++i)
+        if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
+}
+
+// Gradients, chunk by chunk from the end: the states of a chunk are recomputed from the one kept at its
+// start, then  g_t = C_t dy_t + a_{t+1} g_{t+1}  runs backwards through it.
+template <class T, int LN>
+__global__ void __launch_bounds__(128) pd_selective_scan_grad_kernel(PdScanArgs a) {
+    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch * a.groups;
+    const int64_t job = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
+    const int64_t s = job / tiles;
+    const int lane = threadIdx.x & 31, sub = lane % LN, first = sub * kStates;
+    if (s > a.tok.seqs || (s == a.tok.seqs && !a.tok.offsets)) return;
+    const ScanTile tile = scan_tile<LN>(a, job % tiles);
+    const int64_t c = tile.channel;
+    float* bc_out = a.partial_bc + (job % tiles) * a.tok.rows * 2 * (kStates * LN);
+    if (s == a.tok.seqs) {
+        for_free_rows(a.tok, [&](int64_t r) {
+            if (tile.active && sub == 0) {
+                store1((T*)a.dx + r * a.channels + c, 0.0f);
+                store1((T*)a.ddelta + r * a.channels + c, 0.0f);
+                if (a.dz) store1((T*)a.dz + r * a.channels + c, 0.0f);
+            }
+            for (int i = lane; i < 2 * kStates * LN; i += 32) bc_out[r * 2 * kStates * LN + i] = 0.0f;
+        });
+        return;
+    }
+    int64_t begin, end;
+    bounds_of(a.tok, s, begin, end);
+    float A[kStates], g[kStates], dA[kStates], h[PD_SCAN_CHUNK + 1][kStates];
+    load_states(a.A + c * a.state, first, a.state, A);
+    const int64_t state_at = (s * a.channels + c) * a.state;
+#pragma unroll
+    for (int i = 0; i < kStates; ++i) g[i] = dA[i] = 0.0f;
+    if (a.dfinal) load_states(a.dfinal + state_at, first, a.state, g);
+    const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
+    float dbias = 0.0f, dskip = 0.0f;
+    const int64_t chunks = (end - begin + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK;
+    for (int64_t k = chunks - 1; k >= 0; --k) {
+        const int64_t from = begin + k * PD_SCAN_CHUNK;
+        const int count = (int)(end - from < PD_SCAN_CHUNK ? end - from : PD_SCAN_CHUNK);
+        load_states(a.carries_in + ((first_chunk(a.tok, s, begin) + k) * a.channels + c) * a.state, first, a.state, h[0]);
+        for (int t = 0; t < count; ++t) {
+            const int64_t r = from + t;
+            const float x = load1((const T*)a.x + r * a.channels + c);
+            float d = load1((const T*)a.delta + r * a.channels + c) + bias;
+            if (a.softplus) d = softplus_(d);
+            float B[kStates];
+            load_states((const T*)a.B + (r * a.groups + tile.group) * a.state, first, a.state, B);
+#pragma unroll
+            for (int i = 0; i < kStates; ++i) h[t + 1][i] = exp_(d * A[i]) * h[t][i] + (first + i < a.state ? d * x * B[i] : 0.0f);
+        }
+        for (int t = count - 1; t >= 0; --t) {
+            const int64_t r = from + t, at = r * a.channels + c;
+            const float x = load1((const T*)a.x + at);
+            const float raw = load1((const T*)a.delta + at) + bias;
+            const float d = a.softplus ? softplus_(raw) : raw;
+            float B[kStates], C[kStates], y = 0.0f;
+            const int64_t bc = (r * a.groups + tile.group) * a.state;
+            load_states((const T*)a.B + bc, first, a.state, B);
+            load_states((const T*)a.C + bc, first, a.state, C);
+            float dy = load1((const T*)a.dy + at);
+            if (a.z) {
+#pragma unroll
+                for (int i = 0; i < kStates; ++i) y += first + i < a.state ? C[i] * h[t + 1][i] : 0.0f;
+                y = sum_lanes<LN>(y);
+                if (a.skip) y += skip * x;
+                const float z = load1((const T*)a.z + at), sig = sigmoid_(z);
+                if (tile.active && sub == 0) store1((T*)a.dz + at, dy * y * sig * (1.0f + z * (1.0f - sig)));
+                dy *= z * sig;
+            }
+            float du = 0.0f, dd = 0.0f;
+#pragma unroll
+            for (int i = 0; i < kStates; ++i) {
+                const bool in = first + i < a.state;
+                g[i] += in ? C[i] * dy : 0.0f;
+                float db = in ? g[i] * (d * x) : 0.0f, dc = in ? h[t + 1][i] * dy : 0.0f;
+                du += in ? g[i] * B[i] : 0.0f;
+                g[i] *= exp_(d * A[i]);               // the gradient of the state before the token
+                const float moved = in ? g[i] * h[t][i] : 0.0f;
+                dd += A[i] * moved;
+                dA[i] += moved * d;
+                if (!tile.active) db = dc = 0.0f;
+#pragma unroll
+                for (int m = LN; m < 32; m *= 2) {
+                    db += __shfl_xor_sync(kFull, db, m);
+                    dc += __shfl_xor_sync(kFull, dc, m);
+                }
+                if (lane < LN) {
+                    bc_out[r * 2 * kStates * LN + first + i] = db;
+                    bc_out[r * 2 * kStates * LN + kStates * LN + first + i] = dc;
+                }
+            }
+            du = sum_lanes<LN>(du);
+            dd = sum_lanes<LN>(dd) + du * x;
+            if (a.softplus) dd *= sigmoid_(raw);
+            if (tile.active && sub == 0) {
+                store1((T*)a.dx + at, du * d + (a.skip ? dy * skip : 0.0f));
+                store1((T*)a.ddelta + at, dd);
+            }
+            dbias += dd;
+            dskip += dy * x;
+        }
+    }
+    if (!tile.active) return;
+    float* sums = a.partial_params + (s * a.channels + c) * (a.state + 2);
+    for (int i = 0; i < kStates; ++i)
+        if (first + i < a.state) {
+            sums[first + i] = dA[i];
+            if (a.dinitial) a.dinitial[state_at + first + i] = g[i];
+        }
+    if (sub == 0) {
+        sums[a.state] = dbias;
+        sums[a.state + 1] = dskip;
+    }
+}
+
+// dB and dC: the tiles of a group added up in order
+template <class T>
+__global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArgs a, int lanes, int64_t tiles) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= a.tok.rows * a.groups * a.state) return;
+    const int n = (int)(i % a.state);
+    const int64_t g = i / a.state % a.groups, r = i / a.state / a.groups;
+    const int wide = kStates * lanes;
+    float b = 0.0f, c = 0.0f;
+    for (int64_t t = g * tiles; t < (g + 1) * tiles; ++t) {
+        const float* p = a.partial_bc + (t * a.tok.rows + r) * 2 * wide + n;
+        b += p[0];
+        c += p[wide];
+    }
+    store1((T*)a.dB + i, b);
+    store1((T*)a.dC + i, c);
+}
+
+__global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdScanArgs a) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int64_t wide = a.channels * (a.state + 2);
+    if (i >= wide) return;
+    float total = 0.0f;
+    for (int64_t s = 0; s < a.tok.seqs; ++s) total += a.partial_params[s * wide + i];
+    const int64_t c = i / (a.state + 2);
+    const int k = (int)(i % (a.state + 2));
+    if (k < a.state) a.dA[c * a.state + k] = total;
+    else if (k == a.state) { if (a.dbias) a.dbias[c] = total; }
+    else if (a.dskip) a.dskip[c] = total;
+}
+
+// ---------------------------------------------------------------------------
+// launchers
+// ---------------------------------------------------------------------------
+int64_t blocks_for(int64_t threads, int block) { return (threads + block - 1) / block; }
+
+template <class F>
+cudaError_t by_type(int type, F f) {
+    if (type == PD_TYPE_F32) return f(float());
+    if (type == PD_TYPE_F16) return f(__half());
+    return f(__nv_bfloat16());
+}
+template <int V> struct Int { static constexpr int value = V; };
+template <class F>
+cudaError_t by_width(int width, F f) {
+    return width == 2 ? f(Int<2>()) : width == 3 ? f(Int<3>()) : f(Int<4>());
+}
+template <class F>
+cudaError_t by_lanes(int state, F f) {
+    switch (pd_scan_lanes(state)) {
+        case 1: return f(Int<1>());
+        case 2: return f(Int<2>());
+        case 4: return f(Int<4>());
+        case 8: return f(Int<8>());
+        default: return f(Int<16>());
+    }
+}
+// f(element, width, vector) for the call's type, width and alignment
+template <class F>
+cudaError_t by_conv(const PdConvArgs& a, F f) {
+    return by_type(a.type, [&](auto e) {
+        using T = decltype(e);
+        return by_width(a.width, [&](auto w) {
+            return a.vec > 1 ? f(e, w, Int<(int)(16 / sizeof(T))>()) : f(e, w, Int<1>());
+        });
+    });
+}
+
+cudaError_t launch_conv(const PdConvArgs& a, cudaStream_t st) {
+    return by_conv(a, [&](auto e, auto w, auto v) {
+        using T = decltype(e);
+        const int64_t lanes = (a.channels + v.value - 1) / v.value;
+        const int64_t jobs = (a.tok.rows + a.run - 1) / a.run + (a.final_state ? a.tok.seqs : 0);
+        if (lanes * jobs == 0) return cudaSuccess;
+        pd_causal_conv_kernel<T, decltype(w)::value, decltype(v)::value><<<(unsigned)blocks_for(lanes * jobs, 256), 256, 0, st>>>(a);
+        return cudaGetLastError();
+    });
+}
+cudaError_t launch_conv_step(const PdConvArgs& a, cudaStream_t st) {
+    return by_conv(a, [&](auto e, auto w, auto v) {
+        using T = decltype(e);
+        const int64_t lanes = (a.channels + v.value - 1) / v.value;
+        if (lanes * a.tok.seqs == 0) return cudaSuccess;
+        pd_causal_conv_step_kernel<T, decltype(w)::value, decltype(v)::value><<<(unsigned)blocks_for(lanes * a.tok.seqs, 128), 128, 0, st>>>(a);
+        return cudaGetLastError();
+    });
+}
+cudaError_t launch_conv_grad(const PdConvArgs& a, cudaStream_t st) {
+    return by_conv(a, [&](auto e, auto w, auto v) {
+        using T = decltype(e);
+        constexpr int W = decltype(w)::value, V = decltype(v)::value;
+        const int64_t lanes = (a.channels + V - 1) / V;
+        if (a.channels == 0) return cudaSuccess;
+        const dim3 block(32, 8), grid((unsigned)blocks_for(lanes, 32), (unsigned)a.row_blocks);
+        pd_causal_conv_grad_kernel<T, W, V><<<grid, block, 256 * V * sizeof(float), st>>>(a);
+        cudaError_t err = cudaGetLastError();
+        if (err != cudaSuccess) return err;
+        pd_causal_conv_sum_kernel<W><<<(unsigned)blocks_for(a.channels * (W + 1), 128), 128, 0, st>>>(a);
+        return cudaGetLastError();
+    });
+}
+
+int64_t scan_tiles(const PdScanArgs& a) {
+    const int64_t per = a.channels / a.groups, ch = 32 / pd_scan_lanes(a.state);
+    return (per + ch - 1) / ch;
+}
+cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
+    return by_type(a.type, [&](auto e) {
+        using T = decltype(e);
+        return by_lanes(a.state, [&](auto ln) {
+            const int64_t jobs = scan_tiles(a) * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
+            if (jobs == 0) return cudaSuccess;
+            pd_selective_scan_kernel<T, decltype(ln)::value><<<(unsigned)blocks_for(jobs, 4), 128, 0, st>>>(a);
+            return cudaGetLastError();
+        });
+    });
+}
+cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {
+    return by_type(a.type, [&](auto e) {
+        using T = decltype(e);
+        return by_lanes(a.state, [&](auto ln) {
+            const int64_t jobs = scan_tiles(a) * a.groups * a.tok.seqs;
+            if (jobs == 0) return cudaSuccess;
+            pd_selective_scan_step_kernel<T, decltype(ln)::value><<<(unsigned)blocks_for(jobs, 4), 128, 0, st>>>(a);
+            return cudaGetLastError();
+        });
+    });
+}
+cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
+    return by_type(a.type, [&](auto e) {
+        using T = decltype(e);
+        return by_lanes(a.state, [&](auto ln) {
+            if (a.channels == 0) return cudaSuccess;
+            const int64_t jobs = scan_tiles(a) * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
+            if (jobs > 0) {
+                pd_selective_scan_grad_kernel<T, decltype(ln)::value><<<(unsigned)blocks_for(jobs, 4), 128, 0, st>>>(a);
+                cudaError_t err = cudaGetLastError();
+                if (err != cudaSuccess) return err;
+            }
+            const int64_t cells = a.tok.rows * a.groups * a.state;
+            if (cells > 0) {
+                pd_selective_scan_sum_bc_kernel<T><<<(unsigned)blocks_for(cells, 256), 256, 0, st>>>(a, decltype(ln)::value, scan_tiles(a));
+                cudaError_t err = cudaGetLastError();
+                if (err != cudaSuccess) return err;
+            }
+            pd_selective_scan_sum_params_kernel<<<(unsigned)blocks_for(a.channels * (a.state + 2), 128), 128, 0, st>>>(a);
+            return cudaGetLastError();
+        });
+    });
+}
+
+}  // namespace
+
+const PdScanTable* PD_SCAN_TABLE() {
+    static const PdScanTable table = {launch_conv, launch_conv_step, launch_conv_grad, launch_scan, launch_scan_step, launch_scan_grad};
+    return &table;
+}

@@ -1,0 +1,78 @@
+// pd_scan.h -- argument blocks, geometry and launcher tables of the state-space
+// families (causal convolution and selective scan: prompts, gradients, single
+// tokens), shared by the C-ABI side (pd_scan_api.cu) and the kernels
+// (pd_scan.cu, compiled once per math mode like pd_kernels.cu).
+#ifndef PD_SCAN_H_
+#define PD_SCAN_H_
+
+#include <cuda_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include <vector>
+
+// A sequence's tokens are rows of `x`.  Dense calls: sequence s has rows [s * length, (s + 1) * length).
+// Packed calls: rows [offsets[s], offsets[s + 1]), every value clamped to [0, rows], a decreasing pair an
+// empty sequence; whatever the offsets hold, no kernel leaves its arrays.
+struct PdTokens {
+    const int32_t* offsets;   // null: dense
+    int64_t rows;             // rows of the token arrays
+    int64_t length;           // dense: tokens per sequence
+    int64_t seqs;
+};
+
+struct PdConvArgs {
+    PdTokens tok;
+    int type, width, silu;
+    int64_t channels;
+    const void *x, *dy, *initial, *dfinal;
+    const float *weight, *bias;
+    void *y, *final_state, *dx, *dinitial;
+    float *dweight, *dbias;
+    float* partial;           // gradient: (row_blocks, channels, width + 1) sums of dweight and dbias
+    int64_t row_blocks;
+    int vec;                  // channels per thread (16-byte vectors), or 1
+    int run;                  // consecutive rows per thread
+};
+
+struct PdScanArgs {
+    PdTokens tok;
+    int type, state, groups, softplus;
+    int64_t channels;
+    const void *x, *delta, *B, *C, *z, *dy;
+    const float *A, *bias, *skip, *initial, *carries_in, *dfinal;
+    void *y, *dx, *ddelta, *dB, *dC, *dz;
+    float *final_state, *carries, *dA, *dbias, *dskip, *dinitial;
+    // gradient: sums over the channels of one tile, (tiles, rows, 2, 4 * lanes), and over the tokens of one
+    // sequence, (seqs, channels, state + 2)
+    float *partial_bc, *partial_params;
+};
+
+// Lanes that share one channel: each holds four states.
+inline int pd_scan_lanes(int state) { return state <= 4 ? 1 : state <= 8 ? 2 : state <= 16 ? 4 : state <= 32 ? 8 : 16; }
+
+struct PdScanTable {
+    cudaError_t (*conv)(const PdConvArgs&, cudaStream_t);
+    cudaError_t (*conv_step)(const PdConvArgs&, cudaStream_t);
+    cudaError_t (*conv_grad)(const PdConvArgs&, cudaStream_t);
+    cudaError_t (*scan)(const PdScanArgs&, cudaStream_t);
+    cudaError_t (*scan_step)(const PdScanArgs&, cudaStream_t);
+    cudaError_t (*scan_grad)(const PdScanArgs&, cudaStream_t);
+};
+const PdScanTable* pd_scan_table_safe();
+const PdScanTable* pd_scan_table_relaxed();
+const PdScanTable* pd_scan_table_fast();
+
+// What the C ABI needs of a call: its buffers' sizes, its launches and its scratch.
+struct PdScanPlan {
+    const char* kernel_name = "";
+    int64_t grid = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
+    std::vector<size_t> in_bytes, out_bytes;
+};
+bool pd_is_scan_family(int family);
+int pd_scan_plan(int family, const void* params, size_t params_bytes, const int64_t grid[3], const int64_t block[3],
+                 int sms, PdScanPlan* plan, char* err, size_t err_cap);
+int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
+                   const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap);
+
+#endif  // PD_SCAN_H_

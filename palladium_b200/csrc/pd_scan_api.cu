@@ -1,0 +1,310 @@
+// pd_scan_api.cu -- the C-ABI side of the state-space families: parameter
+// checks, buffer sizes, launch geometry and scratch of a call (pd_scan_plan) and
+// its launch (pd_scan_launch).  Called by pd_api.cu, which owns streams and pools.
+#include "../../include/palladium_cuda.h"
+#include "pd_scan.h"
+
+#include <stdarg.h>
+#include <stdio.h>
+#include <string.h>
+
+namespace {
+
+int fail(char* err, size_t cap, const char* fmt, ...) {
+    if (err && cap) {
+        va_list ap;
+        va_start(ap, fmt);
+        vsnprintf(err, cap, fmt, ap);
+        va_end(ap);
+    }
+    return PD_ERR_INVALID_ARGUMENT;
+}
+
+bool is_conv(int family) { return family >= PD_FAMILY_CAUSAL_CONV && family <= PD_FAMILY_CAUSAL_CONV_GRAD; }
+size_t element(int64_t type) { return type == PD_TYPE_F32 ? 4 : 2; }
+int64_t align256(int64_t v) { return (v + 255) / 256 * 256; }
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+bool flag(int64_t v) { return v == 0 || v == 1; }
+
+struct Dims {
+    int64_t seqs, channels, rows;   // rows of the token arrays
+    size_t cells;                   // rows * channels
+};
+
+// `what`: the family's name in messages
+int dims_of(const char* what, const int64_t grid[3], int64_t length, int64_t packed, bool step, int64_t type, Dims* d,
+            char* err, size_t cap) {
+    const int64_t kMost = INT32_MAX;
+    if (type < PD_TYPE_F32 || type > PD_TYPE_BF16) return fail(err, cap, "%s: type must be 0, 1 or 2", what);
+    if (!flag(packed)) return fail(err, cap, "%s: flags must be 0 or 1", what);
+    if (grid[2] > 1) return fail(err, cap, "%s: grid must be (sequences, channels)", what);
+    if (grid[0] > kMost || grid[1] < 1 || grid[1] > (1 << 20))
+        return fail(err, cap, "%s: grid (%lld, %lld) must hold at most 2^31 - 1 sequences and 1 to 2^20 channels", what,
+                    (long long)grid[0], (long long)grid[1]);
+    if (!step && (length < 0 || length > kMost)) return fail(err, cap, "%s: length must lie in [0, 2^31)", what);
+    d->seqs = grid[0];
+    d->channels = grid[1];
+    d->rows = step ? d->seqs : packed ? length : d->seqs * length;
+    if (d->rows > ((int64_t)1 << 40) / d->channels || d->seqs > ((int64_t)1 << 40) / (d->channels * 64))
+        return fail(err, cap, "%s: more than 2^40 elements per call", what);
+    d->cells = (size_t)d->rows * (size_t)d->channels;
+    return PD_OK;
+}
+
+// Rows per thread of the convolution.  A run re-reads width - 1 rows of its predecessor (from L2), so long
+// runs move less and short ones fill the GPU sooner.
+int conv_run(int64_t rows, int64_t lanes, int sms) {
+    int run = 32;
+    while (run > 4 && rows / run * lanes < (int64_t)sms * 1024) run /= 2;
+    return run;
+}
+int64_t conv_row_blocks(int64_t jobs, int64_t lanes, int sms) {
+    // eight runs per block side by side; about two blocks per SM, each of which writes one partial sum
+    const int64_t columns = (lanes + 31) / 32;
+    int64_t blocks = ((int64_t)sms * 2 + columns - 1) / columns;
+    if (blocks > (jobs + 7) / 8) blocks = (jobs + 7) / 8;
+    return blocks < 1 ? 1 : blocks > 65535 ? 65535 : blocks;
+}
+int conv_vector(const pd_causal_conv_params* p, int64_t channels) {
+    const int v = (int)(16 / element(p->type));
+    return channels % v == 0 ? v : 1;
+}
+int64_t conv_partial(const Dims& d, int64_t width, int64_t row_blocks) { return row_blocks * d.channels * (width + 1) * 4; }
+
+int64_t scan_chunks(const pd_selective_scan_params* p, const Dims& d) {
+    return p->packed ? p->length / PD_SCAN_CHUNK + d.seqs : d.seqs * ((p->length + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK);
+}
+int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d) {
+    const int64_t per = d.channels / p->groups, ch = 32 / pd_scan_lanes((int)p->state);
+    return (per + ch - 1) / ch * p->groups;
+}
+int64_t scan_partial_bc(const pd_selective_scan_params* p, const Dims& d) {
+    return align256(scan_tiles(p, d) * d.rows * 8 * pd_scan_lanes((int)p->state) * 4);
+}
+
+int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3], int sms, PdScanPlan* plan, char* err,
+              size_t cap) {
+    const bool step = family == PD_FAMILY_CAUSAL_CONV_STEP, grad = family == PD_FAMILY_CAUSAL_CONV_GRAD;
+    const char* what = step ? "causal_conv_step" : grad ? "causal_conv_grad" : "causal_conv";
+    Dims d;
+    int rc = dims_of(what, grid, p->length, p->packed, step, p->type, &d, err, cap);
+    if (rc) return rc;
+    if (p->width < 2 || p->width > 4) return fail(err, cap, "%s: width must lie in [2, 4], got %lld", what, (long long)p->width);
+    if (!flag(p->silu) || !flag(p->bias) || !flag(p->initial) || !flag(p->final))
+        return fail(err, cap, "%s: flags must be 0 or 1", what);
+    const size_t e = element(p->type), D = (size_t)d.channels, tokens = d.cells * e;
+    const size_t edge = (size_t)d.seqs * (size_t)(p->width - 1) * D * e, weight = D * (size_t)p->width * 4, vec = D * 4;
+    const size_t offsets = ((size_t)d.seqs + 1) * 4;
+    std::vector<size_t>&in = plan->in_bytes, &out = plan->out_bytes;
+    const int64_t lanes = (d.channels + conv_vector(p, d.channels) - 1) / conv_vector(p, d.channels);
+    if (step) {
+        in = {tokens, edge, weight};
+        if (p->bias) in.push_back(vec);
+        out = {tokens, edge};
+        plan->kernel_name = "pd_causal_conv_step_kernel";
+        plan->block = 128;
+        plan->grid = (d.seqs * lanes + 127) / 128;
+        return PD_OK;
+    }
+    in = {tokens, weight};
+    if (grad) in.insert(in.begin(), tokens);
+    if (p->bias) in.push_back(vec);
+    if (p->initial) in.push_back(edge);
+    if (grad && p->final) in.push_back(edge);
+    if (p->packed) in.push_back(offsets);
+    const int run = conv_run(d.rows, lanes, sms);
+    const int64_t runs = (d.rows + run - 1) / run;
+    plan->items = run;
+    plan->block = 256;
+    if (!grad) {
+        out = {tokens};
+        if (p->final) out.push_back(edge);
+        plan->kernel_name = "pd_causal_conv_kernel";
+        plan->grid = ((runs + (p->final ? d.seqs : 0)) * lanes + 255) / 256;
+        return PD_OK;
+    }
+    out = {tokens, weight};
+    if (p->bias) out.push_back(vec);
+    if (p->initial) out.push_back(edge);
+    plan->kernel_name = "pd_causal_conv_grad_kernel";
+    // the scalar form has more columns and so fewer row blocks; size the scratch for the larger count
+    const int64_t jobs = runs + (p->initial ? d.seqs : 0);
+    const int64_t row_blocks = conv_row_blocks(jobs, lanes, sms);
+    plan->grid = (lanes + 31) / 32 * row_blocks;
+    plan->launches = 2;
+    plan->scratch_bytes = conv_partial(d, p->width, row_blocks);
+    return PD_OK;
+}
+
+int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[3], int sms, PdScanPlan* plan, char* err,
+              size_t cap) {
+    (void)sms;
+    const bool step = family == PD_FAMILY_SELECTIVE_SCAN_STEP, grad = family == PD_FAMILY_SELECTIVE_SCAN_GRAD;
+    const char* what = step ? "selective_scan_step" : grad ? "selective_scan_grad" : "selective_scan";
+    Dims d;
+    int rc = dims_of(what, grid, p->length, p->packed, step, p->type, &d, err, cap);
+    if (rc) return rc;
+    if (p->state < 1 || p->state > PD_SCAN_MAX_STATE)
+        return fail(err, cap, "%s: state must lie in [1, %d], got %lld", what, PD_SCAN_MAX_STATE, (long long)p->state);
+    if (p->groups < 1 || d.channels % p->groups != 0)
+        return fail(err, cap, "%s: %lld channels do not divide into %lld groups", what, (long long)d.channels, (long long)p->groups);
+    if (!flag(p->softplus) || !flag(p->bias) || !flag(p->skip) || !flag(p->gate) || !flag(p->initial) || !flag(p->final) ||
+        !flag(p->carries))
+        return fail(err, cap, "%s: flags must be 0 or 1", what);
+    const size_t e = element(p->type), D = (size_t)d.channels, N = (size_t)p->state, tokens = d.cells * e;
+    const size_t coupling = (size_t)d.rows * (size_t)p->groups * N * e, rates = D * N * 4, vec = D * 4;
+    const size_t edge = (size_t)d.seqs * D * N * 4, offsets = ((size_t)d.seqs + 1) * 4;
+    const size_t carries = (size_t)scan_chunks(p, d) * D * N * 4;
+    std::vector<size_t>&in = plan->in_bytes, &out = plan->out_bytes;
+    in = {tokens, tokens, rates, coupling, coupling};
+    if (step) in.insert(in.begin(), edge);
+    if (grad) in.insert(in.begin(), tokens);
+    if (p->bias) in.push_back(vec);
+    if (p->skip) in.push_back(vec);
+    if (p->gate) in.push_back(tokens);
+    plan->block = 128;
+    const int64_t tiles = scan_tiles(p, d), free_rows = p->packed ? 1 : 0;
+    if (step) {
+        out = {tokens, edge};
+        plan->kernel_name = "pd_selective_scan_step_kernel";
+        plan->grid = (tiles * d.seqs + 3) / 4;
+        return PD_OK;
+    }
+    plan->grid = (tiles * (d.seqs + free_rows) + 3) / 4;
+    if (grad) {
+        in.push_back(carries);
+        if (p->final) in.push_back(edge);
+        out = {tokens, tokens, rates, coupling, coupling};
+        if (p->bias) out.push_back(vec);
+        if (p->skip) out.push_back(vec);
+        if (p->gate) out.push_back(tokens);
+        if (p->initial) out.push_back(edge);
+        plan->kernel_name = "pd_selective_scan_grad_kernel";
+        plan->launches = 3;
+        plan->scratch_bytes = scan_partial_bc(p, d) + d.seqs * d.channels * (p->state + 2) * 4;
+    } else {
+        if (p->initial) in.push_back(edge);
+        out = {tokens};
+        if (p->final) out.push_back(edge);
+        if (p->carries) out.push_back(carries);
+        plan->kernel_name = "pd_selective_scan_kernel";
+    }
+    if (p->packed) in.push_back(offsets);
+    return PD_OK;
+}
+
+}  // namespace
+
+bool pd_is_scan_family(int family) { return family >= PD_FAMILY_CAUSAL_CONV && family <= PD_FAMILY_SELECTIVE_SCAN_GRAD; }
+
+int pd_scan_plan(int family, const void* params, size_t params_bytes, const int64_t grid[3], const int64_t block[3],
+                 int sms, PdScanPlan* plan, char* err, size_t err_cap) {
+    const size_t want = is_conv(family) ? sizeof(pd_causal_conv_params) : sizeof(pd_selective_scan_params);
+    if (!params || params_bytes != want)
+        return fail(err, err_cap, "state-space family: params block must be %zu bytes, got %zu", want, params ? params_bytes : (size_t)0);
+    if (block && (block[0] > 0 || block[1] > 0 || block[2] > 0))
+        return fail(err, err_cap, "state-space family: the library chooses the threadgroup; leave it unset");
+    int rc = is_conv(family) ? plan_conv(family, static_cast<const pd_causal_conv_params*>(params), grid, sms, plan, err, err_cap)
+                             : plan_scan(family, static_cast<const pd_selective_scan_params*>(params), grid, sms, plan, err, err_cap);
+    if (rc == PD_OK && plan->grid > INT32_MAX) rc = fail(err, err_cap, "state-space family: the call needs more than 2^31 - 1 blocks");
+    return rc;
+}
+
+int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
+                   const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap) {
+    const PdScanTable* table = math_mode == PD_MATH_SAFE ? pd_scan_table_safe()
+                               : math_mode == PD_MATH_RELAXED ? pd_scan_table_relaxed() : pd_scan_table_fast();
+    cudaError_t e;
+    int i = 0, o = 0;
+    if (is_conv(family)) {
+        const pd_causal_conv_params* p = static_cast<const pd_causal_conv_params*>(params);
+        PdConvArgs a;
+        memset(&a, 0, sizeof(a));
+        const bool step = family == PD_FAMILY_CAUSAL_CONV_STEP, grad = family == PD_FAMILY_CAUSAL_CONV_GRAD;
+        a.type = (int)p->type;
+        a.width = (int)p->width;
+        a.silu = (int)p->silu;
+        a.channels = grid[1];
+        a.tok.seqs = grid[0];
+        a.tok.length = p->length;
+        a.tok.rows = step ? grid[0] : p->packed ? p->length : grid[0] * p->length;
+        a.run = (int)plan.items;
+        if (grad) a.dy = in[i++];
+        a.x = in[i++];
+        if (step) a.initial = in[i++];
+        a.weight = (const float*)in[i++];
+        if (p->bias) a.bias = (const float*)in[i++];
+        if (!step && p->initial) a.initial = in[i++];
+        if (grad && p->final) a.dfinal = in[i++];
+        if (!step && p->packed) a.tok.offsets = (const int32_t*)in[i++];
+        if (grad) {
+            a.dx = out[o++];
+            a.dweight = (float*)out[o++];
+            if (p->bias) a.dbias = (float*)out[o++];
+            if (p->initial) a.dinitial = out[o++];
+        } else {
+            a.y = out[o++];
+            if (step || p->final) a.final_state = out[o++];
+        }
+        a.vec = conv_vector(p, a.channels);
+        const void* tokens[] = {a.x, a.dy, a.initial, a.dfinal, a.y, a.final_state, a.dx, a.dinitial};
+        for (const void* t : tokens) if (!aligned16(t)) a.vec = 1;
+        if (grad) {
+            const int64_t lanes = a.channels / conv_vector(p, a.channels);
+            a.row_blocks = plan.grid / ((lanes + 31) / 32);
+            a.partial = (float*)scratch;
+        }
+        e = step ? table->conv_step(a, st) : grad ? table->conv_grad(a, st) : table->conv(a, st);
+    } else {
+        const pd_selective_scan_params* p = static_cast<const pd_selective_scan_params*>(params);
+        PdScanArgs a;
+        memset(&a, 0, sizeof(a));
+        const bool step = family == PD_FAMILY_SELECTIVE_SCAN_STEP, grad = family == PD_FAMILY_SELECTIVE_SCAN_GRAD;
+        a.type = (int)p->type;
+        a.state = (int)p->state;
+        a.groups = (int)p->groups;
+        a.softplus = (int)p->softplus;
+        a.channels = grid[1];
+        a.tok.seqs = grid[0];
+        a.tok.length = p->length;
+        a.tok.rows = step ? grid[0] : p->packed ? p->length : grid[0] * p->length;
+        if (step) a.initial = (const float*)in[i++];
+        if (grad) a.dy = in[i++];
+        a.x = in[i++];
+        a.delta = in[i++];
+        a.A = (const float*)in[i++];
+        a.B = in[i++];
+        a.C = in[i++];
+        if (p->bias) a.bias = (const float*)in[i++];
+        if (p->skip) a.skip = (const float*)in[i++];
+        if (p->gate) a.z = in[i++];
+        if (grad) {
+            a.carries_in = (const float*)in[i++];
+            if (p->final) a.dfinal = (const float*)in[i++];
+            a.dx = out[o++];
+            a.ddelta = out[o++];
+            a.dA = (float*)out[o++];
+            a.dB = out[o++];
+            a.dC = out[o++];
+            if (p->bias) a.dbias = (float*)out[o++];
+            if (p->skip) a.dskip = (float*)out[o++];
+            if (p->gate) a.dz = out[o++];
+            if (p->initial) a.dinitial = (float*)out[o++];
+            Dims d = {grid[0], grid[1], a.tok.rows, 0};
+            a.partial_bc = (float*)scratch;
+            a.partial_params = (float*)((char*)scratch + scan_partial_bc(p, d));
+        } else {
+            if (!step && p->initial) a.initial = (const float*)in[i++];
+            a.y = out[o++];
+            if (step || p->final) a.final_state = (float*)out[o++];
+            if (!step && p->carries) a.carries = (float*)out[o++];
+        }
+        if (!step && p->packed) a.tok.offsets = (const int32_t*)in[i++];
+        e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
+    }
+    if (e != cudaSuccess) {
+        fail(err, err_cap, "%s: launch failed: %s", plan.kernel_name, cudaGetErrorString(e));
+        return PD_ERR_CUDA;
+    }
+    return PD_OK;
+}

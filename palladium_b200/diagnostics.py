@@ -17,10 +17,10 @@ from functools import lru_cache
 from pathlib import Path
 
 from . import _native
-from .families import KernelSpec
+from .families import STATE_SPACE, KernelSpec
 from .math_mode import math_mode_ordinal
 
-__all__ = ["KernelDiagnostics", "explain_spec", "log_compile"]
+__all__ = ["KernelDiagnostics", "explain_spec", "log_compile", "source_name"]
 
 
 @dataclasses.dataclass(frozen=True)
@@ -60,9 +60,14 @@ class KernelDiagnostics:
         return " ".join(parts)
 
 
-@lru_cache(maxsize=1)
-def _source_lines() -> int:
-    src = Path(__file__).resolve().parent / "csrc" / "pd_kernels.cu"
+def source_name(spec: KernelSpec) -> str:
+    """The CUDA file a precompiled family is built from."""
+    return "palladium_b200/csrc/" + ("pd_scan.cu" if spec.family.name in STATE_SPACE else "pd_kernels.cu")
+
+
+@lru_cache(maxsize=2)
+def _source_lines(name: str) -> int:
+    src = Path(__file__).resolve().parent.parent / name
     try:
         return len(src.read_text().splitlines())
     except OSError:
@@ -87,7 +92,7 @@ def explain_spec(spec: KernelSpec, threadgroup=None, math_mode="fast") -> Kernel
     elif spec.family.name == "source":
         lines = len(spec.family.constants["source"].splitlines())
     else:
-        lines = _source_lines()
+        lines = _source_lines(source_name(spec))
     info = _native.explain(spec.family.family_id, spec.params, math_mode_ordinal(math_mode), spec.grid, tg)
     return KernelDiagnostics(
         name=spec.name,

@@ -26,8 +26,9 @@ import numpy as np
 
 from . import _native
 from .errors import DispatchError, PalladiumError
-from .families import KernelSpec
+from .families import STATE_SPACE, KernelSpec
 from .math_mode import MathMode, math_mode_ordinal
+from .pl import as_dtype, dtype_name
 
 __all__ = ["BoundKernel", "PendingResult", "bind"]
 
@@ -58,9 +59,9 @@ def _dump_source(spec: KernelSpec, math_mode) -> None:
     dump = os.environ.get("PALLADIUM_DUMP_MSL")
     if not dump:
         return
-    from .diagnostics import explain_spec
+    from .diagnostics import explain_spec, source_name
 
-    src = Path(__file__).resolve().parent / "csrc" / "pd_kernels.cu"
+    src = Path(__file__).resolve().parent.parent / source_name(spec)
     text = (f"// palladium kernel: {spec.name}\n// source: {src}\n// constants: {spec.family.constants}\n"
             f"// {explain_spec(spec, None, math_mode)}\n")
     if dump == "1" or dump.lower() == "stdout":
@@ -127,6 +128,7 @@ class BoundKernel:
     msl_source: str = "palladium_b200/csrc/pd_kernels.cu"
     _in_sizes: list | None = dataclasses.field(default=None, compare=False, repr=False)
     _out_sizes: list | None = dataclasses.field(default=None, compare=False, repr=False)
+    _scratch: int | None = dataclasses.field(default=None, compare=False, repr=False)
     # Launches go through the library's slot pool (a stream and an event per call in flight), which
     # serialises what it must itself: no lock is held here, neither to launch nor to wait
     # (src/palladium/dispatch.py:121-127 holds one per kernel for launching).
@@ -139,10 +141,9 @@ class BoundKernel:
         out = []
         for i, (a, info) in enumerate(zip(arrays, spec.inputs)):
             arr = np.asarray(a)
-            if arr.dtype != info.dtype:
-                raise DispatchError(
-                    f"argument {i}: dtype {arr.dtype} does not match the traced {info.dtype}; cast explicitly"
-                )
+            if as_dtype(arr.dtype) != info.dtype:
+                raise DispatchError(f"argument {i}: dtype {dtype_name(as_dtype(arr.dtype))} does not match the traced "
+                                    f"{dtype_name(info.dtype)}; cast explicitly")
             if arr.shape != info.array_shape:
                 raise DispatchError(f"argument {i}: expected shape {info.array_shape}, got {arr.shape}")
             out.append(np.ascontiguousarray(arr))
@@ -195,6 +196,14 @@ class BoundKernel:
 
         return call
 
+    def _scratch_bytes(self) -> int:
+        """Scratch of a state-space call; 0 for the families that use the library's pool."""
+        if self._scratch is None:
+            spec = self.spec
+            self._scratch = 0 if spec.family.name not in STATE_SPACE else int(_native.explain(
+                spec.family.family_id, spec.params, self.math_mode, spec.grid, self.threadgroup).scratch_bytes)
+        return self._scratch
+
     # ------------------------------------------------------------------ device-resident path
     def launch_device(self, inputs, outputs=None, stream=None, workspace=None):
         """Launch on torch CUDA tensors, stream-ordered, without any host
@@ -204,7 +213,9 @@ class BoundKernel:
         `workspace`: a uint8 CUDA tensor of at least `scratch_bytes` (see
         `pd_explain`) for the kernels' scratch, in place of the library's own
         per-stream pool -- a caller that records launches into a CUDA graph owns
-        the memory the graph keeps pointing at this way."""
+        the memory the graph keeps pointing at this way.  A state-space call that
+        is given none takes it from torch's allocator, where a captured call gets
+        memory that belongs to its graph."""
         torch = _require_cuda()
         spec = self.spec
         if len(inputs) != len(spec.inputs):
@@ -230,6 +241,9 @@ class BoundKernel:
             # The kernel writes `out_bytes[i]` bytes from each pointer whatever the tensor's own
             # size or strides: a short, strided, host or other-device tensor must stop here.
             check_device_tensors("output", outputs, out_bytes, current)
+        if workspace is None and self._scratch_bytes():
+            with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream()):
+                workspace = torch.empty(self._scratch, dtype=torch.uint8, device="cuda")
         _native.launch(
             spec.family.family_id, spec.params, self.math_mode, spec.grid, self.threadgroup,
             [(t.data_ptr(), b) for t, b in zip(inputs, in_bytes)],
@@ -266,6 +280,8 @@ def bind(spec: KernelSpec, msl_source: str | None = None, *, math_mode=MathMode.
     (src/palladium/dispatch.py:258-314); `msl_source` is accepted for signature
     compatibility and ignored, because the kernels are precompiled.  Loading the
     library here makes a missing build fail at bind time, not at first launch."""
+    from .diagnostics import source_name
+
     _native.library()
     _dump_source(spec, math_mode)
-    return BoundKernel(spec=spec, math_mode=math_mode_ordinal(math_mode), threadgroup=threadgroup)
+    return BoundKernel(spec=spec, msl_source=source_name(spec), math_mode=math_mode_ordinal(math_mode), threadgroup=threadgroup)

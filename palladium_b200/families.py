@@ -15,6 +15,10 @@ the MSL it emits: `custom_ode` (a right-hand side of the caller's inside the
 library's RK4 or adaptive loop) and `source_kernel` (a complete CUDA kernel of
 the caller's).
 
+The state-space families (`causal_conv`, `selective_scan` and their `_step` and
+`_grad` forms) integrate ensembles of driven linear systems over sequences of
+tokens; they are not in the reference.
+
 `trace(family, call_kwargs, *args)` produces the `KernelSpec` analogue: name,
 grid, and one `BlockInfo` per operand.
 """
@@ -30,11 +34,17 @@ import numpy as np
 
 from . import _native
 from .errors import DispatchError, TraceError, UnsupportedPrimitiveError
+from .pl import ShapeDtypeStruct, as_dtype, bfloat16, dtype_name
 
 __all__ = [
     "BlockInfo",
     "Family",
     "KernelSpec",
+    "SCAN_CHUNK",
+    "STATE_SPACE",
+    "causal_conv",
+    "causal_conv_grad",
+    "causal_conv_step",
     "custom_ode",
     "gbm_pcg",
     "gbm_threefry",
@@ -42,6 +52,10 @@ __all__ = [
     "kepler_rk4_df32",
     "lv_rk4",
     "lv_rk4_df32",
+    "out_shapes",
+    "selective_scan",
+    "selective_scan_grad",
+    "selective_scan_step",
     "source_kernel",
     "threefry_bits",
     "trace",
@@ -318,6 +332,225 @@ def threefry_bits(op: str = "bits", count: int = 1) -> Family:
     return Family("threefry_bits", dict(op=op, op_code=ops[op], count=int(count)))
 
 
+# ----------------------------------------------------------------------------- state-space families
+SCAN_CHUNK = 64       # tokens between two states that `selective_scan(carries=True)` keeps
+
+_TYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2}
+
+
+def _element_type(what: str, dtype) -> str:
+    try:
+        name = dtype_name(as_dtype(dtype))
+    except TypeError:
+        name = str(dtype)
+    if name not in _TYPE_CODES:
+        raise TraceError(f"{what}: dtype must be one of {', '.join(_TYPE_CODES)}, got {name}")
+    return name
+
+
+def _whole(what: str, name: str, value, low: int, high: int) -> int:
+    if isinstance(value, bool) or int(value) != value or not low <= value <= high:
+        raise TraceError(f"{what}: {name} must be a whole number in [{low}, {high}], got {value!r}")
+    return int(value)
+
+
+def _conv_family(name: str, length, width, silu, bias, initial, final, packed, dtype) -> Family:
+    return Family(name, dict(length=_whole(name, "length", length, 0, 2**31 - 1), width=_whole(name, "width", width, 2, 4),
+                             silu=bool(silu), bias=bool(bias), initial=bool(initial), final=bool(final),
+                             packed=bool(packed), dtype=_element_type(name, dtype)))
+
+
+def causal_conv(length: int, width: int = 4, *, silu: bool = True, bias: bool = True, initial: bool = False,
+                final: bool = False, packed: bool = False, dtype="float32") -> Family:
+    """A short causal convolution over the tokens of S sequences, channel by channel:
+    `y_t = act(bias + sum_j weight[:, width - 1 - j] * x_{t-j})`, j = 0 .. width - 1,
+    with act(v) = v / (1 + e^-v) or, with `silu=False`, v itself.  Not in the reference.
+
+    grid=(S, D).  Inputs: x (S, length, D), weight (D, width) float32, bias (D,)
+    float32 with `bias`, initial (S, width - 1, D) with `initial` (the inputs before
+    each sequence's first token, else zeros), offsets with `packed`.  Outputs:
+    y like x, and with `final` the last width - 1 inputs of each sequence, what the
+    next call's `initial` or `causal_conv_step`'s state is.  `width` is 2, 3 or 4.
+
+    `packed=True`: sequences of different lengths behind one another.  Token arrays
+    are (length, D) with `length` rows in all; the last operand, offsets (S + 1,)
+    int32, gives sequence s the rows offsets[s] .. offsets[s + 1] - 1.  It is read on
+    the device: values are clamped to [0, length], a decreasing pair is an empty
+    sequence, rows of no sequence come out as zeros.  Sequences that overlap
+    (offsets out of order) have undefined results.
+
+    `dtype`: float32, float16 or bfloat16 (`pl.bfloat16`, torch.bfloat16), the type
+    of x, y, initial and final.  Sums are float32, rounded once."""
+    return _conv_family("causal_conv", length, width, silu, bias, initial, final, packed, dtype)
+
+
+def causal_conv_step(width: int = 4, *, silu: bool = True, bias: bool = True, dtype="float32") -> Family:
+    """`causal_conv` for one token of each of S sequences.  grid=(S, D); inputs x (S, D),
+    state (S, width - 1, D), weight, bias; outputs y (S, D) and the state one token on.
+    On device tensors `call.on_device(..., out=(y, state))` updates a state in place."""
+    return _conv_family("causal_conv_step", 1, width, silu, bias, True, True, False, dtype)
+
+
+def causal_conv_grad(length: int, width: int = 4, *, silu: bool = True, bias: bool = True, initial: bool = False,
+                     final: bool = False, packed: bool = False, dtype="float32") -> Family:
+    """Gradients of `causal_conv` with the same constants.  Inputs: dy like y, then x,
+    weight, bias, initial as there, dfinal (the gradient of final) with `final`, offsets
+    with `packed`.  Outputs: dx, dweight float32, dbias float32 with `bias`, dinitial with
+    `initial`.  Sums run in a fixed order: equal calls on one device give equal bits."""
+    return _conv_family("causal_conv_grad", length, width, silu, bias, initial, final, packed, dtype)
+
+
+def _scan_family(name: str, length, state, groups, softplus, bias, skip, gate, initial, final, carries, packed,
+                 dtype) -> Family:
+    return Family(name, dict(length=_whole(name, "length", length, 0, 2**31 - 1), state=_whole(name, "state", state, 1, 64),
+                             groups=_whole(name, "groups", groups, 1, 2**20), softplus=bool(softplus), bias=bool(bias),
+                             skip=bool(skip), gate=bool(gate), initial=bool(initial), final=bool(final),
+                             carries=bool(carries), packed=bool(packed), dtype=_element_type(name, dtype)))
+
+
+def selective_scan(length: int, state: int = 16, *, groups: int = 1, softplus: bool = True, bias: bool = True,
+                   skip: bool = True, gate: bool = False, initial: bool = False, final: bool = False,
+                   carries: bool = False, packed: bool = False, dtype="float32") -> Family:
+    """An ensemble of driven linear systems h' = A h + B(t) x(t), y = C(t) h + skip x with
+    `state` states each, one trajectory per (sequence, channel), integrated over steps of
+    input-dependent length d with B and x held constant in each (the selective state-space
+    scan).  Not in the reference, whose ensembles have parameters fixed in time.
+
+        d = softplus(delta + bias)         (softplus=False: delta + bias)
+        h_t = exp(d A) h_{t-1} + d x_t B_t
+        y_t = (C_t . h_t + skip x_t) * z_t / (1 + e^-z_t)      (the last factor with `gate`)
+
+    grid=(S, D).  Inputs: x (S, length, D), delta like x, A (D, state) float32,
+    B (S, length, groups, state), C like B, bias (D,) float32 with `bias`, skip (D,) float32
+    with `skip`, z like x with `gate`, initial (S, D, state) float32 with `initial` (else
+    zeros), offsets with `packed` (see `causal_conv`; B and C are then (length, groups, state)).
+    Channel c reads group c // (D // groups).  Outputs: y like x; final (S, D, state) float32
+    with `final`; with `carries` the states a later `selective_scan_grad` recomputes from, one
+    per SCAN_CHUNK tokens: (S, ceil(length / SCAN_CHUNK), D, state) float32, packed
+    (length // SCAN_CHUNK + S, D, state) with entries that no token owns left unwritten.
+
+    `state` is 1 .. 64.  `dtype` (float32, float16, bfloat16) is the type of x, delta, B, C, z
+    and y; states are float32 throughout and y is rounded once."""
+    return _scan_family("selective_scan", length, state, groups, softplus, bias, skip, gate, initial, final, carries,
+                        packed, dtype)
+
+
+def selective_scan_step(state: int = 16, *, groups: int = 1, softplus: bool = True, bias: bool = True,
+                        skip: bool = True, gate: bool = False, dtype="float32") -> Family:
+    """`selective_scan` for one token of each of S sequences.  grid=(S, D); inputs
+    state (S, D, state) float32, x (S, D), delta, A, B (S, groups, state), C, bias, skip, z;
+    outputs y (S, D) and the state one token on.  On device tensors
+    `call.on_device(..., out=(y, state))` updates a state in place."""
+    return _scan_family("selective_scan_step", 1, state, groups, softplus, bias, skip, gate, True, True, False, False,
+                        dtype)
+
+
+def selective_scan_grad(length: int, state: int = 16, *, groups: int = 1, softplus: bool = True, bias: bool = True,
+                        skip: bool = True, gate: bool = False, initial: bool = False, final: bool = False,
+                        packed: bool = False, dtype="float32") -> Family:
+    """Gradients of `selective_scan` with the same constants.  Inputs: dy like y, then x,
+    delta, A, B, C, bias, skip, z as there, the carries of a forward call with
+    `carries=True`, dfinal (the gradient of final) with `final`, offsets with `packed`.
+    Outputs: dx, ddelta, dA float32, dB, dC, then dbias and dskip float32, dz and
+    dinitial float32 where the constants have them.  B and C are shared by the channels of
+    a group and the parameters by all tokens: their sums are float32 in a fixed order, so
+    equal calls on one device give equal bits."""
+    return _scan_family("selective_scan_grad", length, state, groups, softplus, bias, skip, gate, initial, final, False,
+                        packed, dtype)
+
+
+STATE_SPACE = ("causal_conv", "causal_conv_step", "causal_conv_grad", "selective_scan", "selective_scan_step",
+                  "selective_scan_grad")
+
+
+def _scan_operands(family: Family, grid) -> tuple[list, list]:
+    """(inputs, outputs) of a state-space call as (name, BlockInfo, index map): one program per
+    (sequence, channel), whose blocks are that channel's column of the sequence's tokens."""
+    c, name = family.constants, family.name
+    if len(grid) != 2:
+        raise TraceError(f"{name}: grid must be (sequences, channels), got {grid}")
+    s, d = grid
+    if s < 0 or d < 1:
+        raise TraceError(f"{name}: grid must hold at least one channel, got {grid}")
+    kind = bfloat16 if c["dtype"] == "bfloat16" else np.dtype(c["dtype"])
+    step, n, packed = name.endswith("step"), c["length"], c["packed"]
+
+    def tokens(label, dtype=kind):
+        if step:
+            return label, BlockInfo((1, 1), (s, d), dtype), lambda i, j: (i, j)
+        if packed:
+            return label, BlockInfo((n, 1), (n, d), dtype), lambda i, j: (0, j)
+        return label, BlockInfo((1, n, 1), (s, n, d), dtype), lambda i, j: (i, 0, j)
+
+    def parameter(label, *shape):
+        return label, BlockInfo((1,) + shape, (d,) + shape, F32), lambda i, j: (j,) + (0,) * len(shape)
+
+    offsets = [("offsets", BlockInfo((s + 1,), (s + 1,), I32), lambda i, j: (0,))] if packed else []
+    if name.startswith("causal_conv"):
+        w = c["width"]
+
+        def edge(label):
+            return label, BlockInfo((1, w - 1, 1), (s, w - 1, d), kind), lambda i, j: (i, 0, j)
+
+        weights = [parameter("weight", w)] + [parameter("bias")] * c["bias"]
+        if step:
+            return [tokens("x"), edge("state")] + weights, [tokens("y"), edge("state")]
+        before = [edge("initial")] * c["initial"]
+        if name == "causal_conv":
+            return [tokens("x")] + weights + before + offsets, [tokens("y")] + [edge("final")] * c["final"]
+        return ([tokens("dy"), tokens("x")] + weights + before + [edge("dfinal")] * c["final"] + offsets,
+                [tokens("dx"), parameter("dweight", w)] + [parameter("dbias")] * c["bias"] + [edge("dinitial")] * c["initial"])
+    k, g = c["state"], c["groups"]
+    if d % g:
+        raise TraceError(f"{name}: {d} channels do not divide into {g} groups")
+    per = d // g
+
+    def coupling(label):
+        if step:
+            return label, BlockInfo((1, 1, k), (s, g, k), kind), lambda i, j: (i, j // per, 0)
+        if packed:
+            return label, BlockInfo((n, 1, k), (n, g, k), kind), lambda i, j: (0, j // per, 0)
+        return label, BlockInfo((1, n, 1, k), (s, n, g, k), kind), lambda i, j: (i, 0, j // per, 0)
+
+    def edge(label):
+        return label, BlockInfo((1, 1, k), (s, d, k), F32), lambda i, j: (i, j, 0)
+
+    def kept(label):
+        if packed:
+            chunks = n // SCAN_CHUNK + s
+            return label, BlockInfo((chunks, 1, k), (chunks, d, k), F32), lambda i, j: (0, j, 0)
+        chunks = -(-n // SCAN_CHUNK)
+        return label, BlockInfo((1, chunks, 1, k), (s, chunks, d, k), F32), lambda i, j: (i, 0, j, 0)
+
+    operands = ([tokens("x"), tokens("delta"), parameter("A", k), coupling("B"), coupling("C")]
+                + [parameter("bias")] * c["bias"] + [parameter("skip")] * c["skip"] + [tokens("z")] * c["gate"])
+    if step:
+        return [edge("state")] + operands, [tokens("y"), edge("state")]
+    if name == "selective_scan":
+        return (operands + [edge("initial")] * c["initial"] + offsets,
+                [tokens("y")] + [edge("final")] * c["final"] + [kept("carries")] * c["carries"])
+    return ([tokens("dy")] + operands + [kept("carries")] + [edge("dfinal")] * c["final"] + offsets,
+            [tokens("dx"), tokens("ddelta"), parameter("dA", k), coupling("dB"), coupling("dC")]
+            + [parameter("dbias")] * c["bias"] + [parameter("dskip")] * c["skip"] + [tokens("dz")] * c["gate"]
+            + [edge("dinitial")] * c["initial"])
+
+
+def _scan_params(family: Family):
+    c = dict(family.constants, type=_TYPE_CODES[family.constants["dtype"]])
+    kind = _native.CausalConvParams if family.name.startswith("causal_conv") else _native.SelectiveScanParams
+    return kind(*[int(c[field]) for field, _ in kind._fields_])
+
+
+def out_shapes(family: Family, grid):
+    """The `out_shape` of a state-space call, for families whose outputs follow from their
+    constants: a ShapeDtypeStruct, or a tuple of them in output order."""
+    if not isinstance(family, Family) or family.name not in STATE_SPACE:
+        raise TraceError(f"out_shapes knows the state-space families ({', '.join(STATE_SPACE)}), not {family!r}")
+    grid = tuple(int(g) for g in grid)
+    shapes = tuple(ShapeDtypeStruct(info.array_shape, info.dtype) for _, info, _ in _scan_operands(family, grid)[1])
+    return shapes[0] if len(shapes) == 1 else shapes
+
+
 # ----------------------------------------------------------------------------- tracing
 def _shape_dtype(x) -> tuple[tuple[int, ...], np.dtype]:
     shape = getattr(x, "shape", None)
@@ -325,11 +558,7 @@ def _shape_dtype(x) -> tuple[tuple[int, ...], np.dtype]:
     if shape is None or dtype is None:
         arr = np.asarray(x)
         shape, dtype = arr.shape, arr.dtype
-    try:
-        dtype = np.dtype(dtype)
-    except TypeError:
-        # a torch dtype: "torch.float32" -> float32
-        dtype = np.dtype(str(dtype).rsplit(".", 1)[-1])
+    dtype = as_dtype(dtype)
     return tuple(int(s) for s in shape), dtype
 
 
@@ -380,7 +609,7 @@ def _check_args(args, inputs: Sequence[BlockInfo]) -> None:
             raise TraceError(f"argument {i}: shape {shape} does not match the {info.array_shape} implied by grid")
         if dtype != info.dtype:
             raise DispatchError(
-                f"argument {i}: dtype {dtype} does not match the traced {info.dtype}; cast explicitly"
+                f"argument {i}: dtype {dtype_name(dtype)} does not match the traced {dtype_name(info.dtype)}; cast explicitly"
             )
 
 
@@ -534,6 +763,12 @@ def trace(family: Family, call_kwargs: dict[str, Any], *args) -> KernelSpec:
             inputs, outputs = (key,), (BlockInfo((1, c["count"]), (n, c["count"]), F32),)
         blocks_in = blocks_out = None
         params = _native.ThreefryParams(c["op_code"], c["count"])
+    elif name in STATE_SPACE:
+        taken, given = _scan_operands(family, grid)
+        inputs, outputs = tuple(info for _, info, _ in taken), tuple(info for _, info, _ in given)
+        blocks_in = [(info.block_shape, index) for _, info, index in taken]
+        blocks_out = [(info.block_shape, index) for _, info, index in given]
+        params = _scan_params(family)
     else:
         raise UnsupportedPrimitiveError(f"no CUDA kernel family named {name!r}")
 

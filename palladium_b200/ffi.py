@@ -34,7 +34,7 @@ from .errors import DispatchError, UnsupportedPrimitiveError
 from .families import Family, KernelSpec, trace
 from .interpret import interpret_callable
 from .math_mode import MathMode, math_mode_ordinal
-from .pl import ShapeDtypeStruct
+from .pl import ShapeDtypeStruct, as_dtype, dtype_name
 
 __all__ = ["FfiCallable", "cuda_call_jit"]
 
@@ -63,8 +63,9 @@ def _torch_dtype_tables(torch):
     """(torch dtype -> NumPy dtype name, and back), built once."""
     if not _DTYPE_TABLES:
         to_np = {torch.float32: "float32", torch.int32: "int32", torch.uint32: "uint32", torch.float64: "float64",
-                 torch.uint8: "uint8"}
-        to_torch = {"float32": torch.float32, "int32": torch.int32, "uint32": torch.uint32, "float64": torch.float64}
+                 torch.uint8: "uint8", torch.float16: "float16", torch.bfloat16: "bfloat16"}
+        to_torch = {"float32": torch.float32, "int32": torch.int32, "uint32": torch.uint32, "float64": torch.float64,
+                    "float16": torch.float16, "bfloat16": torch.bfloat16}
         _DTYPE_TABLES.append((to_np, to_torch))
     return _DTYPE_TABLES[0]
 
@@ -129,7 +130,7 @@ class FfiCallable:
             with self._lock:
                 entry = self._cache.get(shapes)
                 if entry is None:
-                    structs = [ShapeDtypeStruct(s, np.dtype(d)) for s, d in shapes]
+                    structs = [ShapeDtypeStruct(s, d) for s, d in shapes]
                     spec = trace(self._family, self._pallas_kwargs, *structs)
                     log_compile(spec, self._threadgroup, self._math_mode)
                     entry = (spec, bind(spec, math_mode=self._math_mode, threadgroup=self._threadgroup))
@@ -187,7 +188,7 @@ class FfiCallable:
         if out is not None:
             outs = list(out) if isinstance(out, (list, tuple)) else [out]
         else:
-            outs = [torch.empty(info.array_shape, dtype=torch_dtype[info.dtype.name], device=device)
+            outs = [torch.empty(info.array_shape, dtype=torch_dtype[dtype_name(info.dtype)], device=device)
                     for info in spec.outputs]
         bound.launch_device(list(args), outs)
         return outs[0] if len(outs) == 1 else tuple(outs)
@@ -201,7 +202,7 @@ class FfiCallable:
     # ---- host buffers: the XLA:CPU handler contract -----------------------------
     def _call_host(self, args):
         arrays = [np.ascontiguousarray(a) for a in args]
-        shapes = tuple((a.shape, a.dtype.name) for a in arrays)
+        shapes = tuple((a.shape, dtype_name(as_dtype(a.dtype))) for a in arrays)
         spec, _ = self._entry(shapes)
         out_bytes = [int(np.prod(info.array_shape)) * info.dtype.itemsize for info in spec.outputs]
         if sum(a.nbytes for a in arrays) + sum(out_bytes) < _SMALL_HOST_CALL_BYTES:

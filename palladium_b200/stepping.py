@@ -19,6 +19,7 @@ import numpy as np
 
 from .dispatch import BoundKernel, _require_cuda
 from .errors import DispatchError
+from .pl import as_dtype, dtype_name
 
 __all__ = ["Stepper"]
 
@@ -94,7 +95,7 @@ class Stepper:
         if hasattr(call, "_bound"):            # CudaCallable
             return call._bound(arrs)
         if hasattr(call, "_entry"):            # FfiCallable
-            return call._entry(tuple((a.shape, a.dtype.name) for a in arrs))[1]
+            return call._entry(tuple((a.shape, dtype_name(as_dtype(a.dtype))) for a in arrs))[1]
         raise DispatchError("Stepper needs a call built by cuda_call or cuda_call_jit")
 
     def advance(self, launches: int = 1, graph: bool = False) -> "Stepper":

@@ -21,6 +21,7 @@ import numpy as np
 
 from . import _native
 from .errors import EmitError
+from .pl import as_dtype, bfloat16, dtype_name
 
 _TARGET_NAME = "palladium_cuda_dispatch"
 _SOURCE_TARGET_NAME = "palladium_cuda_dispatch_source"
@@ -69,12 +70,12 @@ def ffi_call(callable_, args):
     import jax
 
     _register()
-    shapes = tuple((tuple(a.shape), np.dtype(a.dtype).name) for a in args)
+    shapes = tuple((tuple(a.shape), dtype_name(as_dtype(a.dtype))) for a in args)
     spec, _ = callable_._entry(shapes)
     grid = tuple(spec.grid) + (1, 1, 1)
     tg = callable_._threadgroup
     tg = (0, 0, 0) if tg is None else (((tg,) if isinstance(tg, int) else tuple(tg)) + (1, 1))[:3]
-    out_structs = [jax.ShapeDtypeStruct(info.array_shape, info.dtype) for info in spec.outputs]
+    out_structs = [jax.ShapeDtypeStruct(info.array_shape, "bfloat16" if info.dtype == bfloat16 else info.dtype) for info in spec.outputs]
     result_shapes = out_structs[0] if len(out_structs) == 1 else out_structs
     params = np.frombuffer(bytes(spec.params), dtype=np.uint8)
     target, text = _TARGET_NAME, {}
