@@ -431,62 +431,341 @@ __device__ __forceinline__ ScanTile scan_tile(const PdScanArgs& a, int64_t tile)
     return t;
 }
 
-template <class T, int LN>
-__global__ void __launch_bounds__(128) pd_selective_scan_kernel(PdScanArgs a) {
-    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch * a.groups;
-    const int64_t job = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t s = job / tiles;
-    const int lane = threadIdx.x & 31, sub = lane % LN, first = sub * kStates;
-    if (s > a.tok.seqs || (s == a.tok.seqs && !a.tok.offsets)) return;
-    const ScanTile tile = scan_tile<LN>(a, job % tiles);
-    const int64_t c = tile.channel;
+// ---------------------------------------------------------------------------
+// The prompt kernel.  A block owns CH = 32 / LN channels of one group and walks one sequence in tiles of
+// 128 tokens: warp w takes tokens 16 w .. 16 w + 15 of the tile, a lane four states of one channel.  Every
+// warp integrates its 16 tokens from a zero state and keeps the 64 decays in registers; the warps' end
+// states and total decays meet in shared memory, where each lane composes the state entering its own tokens;
+// a second pass over the same registers then yields y.  So one exponential per (token, channel, state) is
+// all that is taken, whatever the number of sequences, and a single sequence of 2048 channels already
+// gives 256 blocks of eight warps.
+//
+// Bound: the exponentials, 16 per clock and SM (8 cycles per warp instruction and scheduler); next to each
+// stand six float32 operations, issued two by two, and 1.25 reads of shared memory.
+// ---------------------------------------------------------------------------
+typedef unsigned long long pair_t;     // two float32 in one 64-bit register
+__device__ __forceinline__ pair_t pack(float x, float y) {
+    pair_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void unpack(pair_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+    pair_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+    pair_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// a b + c: one rounding, except under SAFE, which keeps the product's own
+__device__ __forceinline__ pair_t mad2(pair_t a, pair_t b, pair_t c) {
+#if PD_MODE == 0
+    return add2(mul2(a, b), c);
+#else
+    pair_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+#endif
+}
+
+// exp(d A) for a rate as scan_rate() prepares it: FAST folds log2(e) into the rate.  An infinite rate becomes
+// the largest finite one, whose decay over any step is the same, so that a tile's tokens behind the
+// sequence's end (steps of length zero) leave the state as it is instead of multiplying zero by infinity.
+__device__ __forceinline__ float scan_rate(float A) {
+#if PD_MODE == 2
+    A *= 1.4426950408889634f;
+#endif
+    return fabsf(A) == INFINITY ? copysignf(3.4028234e38f, A) : A;
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ pair_t decay2(pair_t d, pair_t rate) {
+    float x, y;
+    unpack(mul2(d, rate), x, y);
+#if PD_MODE == 2
+    return pack(exp2_approx(x), exp2_approx(y));
+#else
+    return pack(expf(x), expf(y));
+#endif
+}
+
+// four elements as stored, fetched ahead of their use
+template <class T> struct Raw4 { T e[4]; };
+template <class T>
+__device__ __forceinline__ Raw4<T> fetch4(const T* p, bool vec, int n) {
+    Raw4<T> r;
+    if (vec && n == 4) {
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(r.e) = *reinterpret_cast<const uint4*>(p);
+        else *reinterpret_cast<uint2*>(r.e) = *reinterpret_cast<const uint2*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r.e[i] = i < n ? p[i] : T(0.0f);
+    }
+    return r;
+}
+template <class T>
+__device__ __forceinline__ void put4(T* p, bool vec, int n, const float (&v)[4]) {
+    if (vec && n == 4) {
+        Raw4<T> r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) store1(&r.e[i], v[i]);
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.e);
+        else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(r.e);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) if (i < n) store1(p + i, v[i]);
+    }
+}
+
+template <int LN, int NS> struct ScanShape {
+    static constexpr int kWarps = 8, kSteps = 16, kTile = kWarps * kSteps, kThreads = 32 * kWarps;
+    static constexpr int kChannels = 32 / LN, kPad = 4 * LN * NS;     // states, rounded up
+    static constexpr int kDu = 0, kB = kDu + 2 * kTile * kChannels, kC = kB + kTile * kPad, kY = kC + kTile * kPad,
+                         kEnd = kY + kTile * 32, kDecay = kEnd + kThreads * 4, kFloats = kDecay + kThreads * 4;
+    static constexpr int kVectors = kTile * kChannels / 4 / kThreads;  // vectors of four channels per thread
+    static constexpr int kCouplings = (kTile * kPad / 4 + kThreads - 1) / kThreads;
+};
+
+template <class T, int LN, int NS, bool FULL>
+__global__ void __launch_bounds__(256, 2) pd_selective_scan_kernel(PdScanArgs a) {
+    using G = ScanShape<LN, NS>;
+    extern __shared__ float4 smem4[];
+    float* smem = reinterpret_cast<float*>(smem4);
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, ch = lane / LN;
+    const int64_t per = a.channels / a.groups, tiles = (per + G::kChannels - 1) / G::kChannels;
+    const int64_t job = blockIdx.x, s = job / (tiles * a.groups);
+    const int64_t group = job / tiles % a.groups, within = job % tiles * G::kChannels;
+    const int64_t c0 = group * per + within;                            // the block's first channel
+    const int count = (int)(per - within < G::kChannels ? per - within : G::kChannels);
+    const T* gx = (const T*)a.x + c0;
+    const T* gdelta = (const T*)a.delta + c0;
+    const T* gz = a.z ? (const T*)a.z + c0 : nullptr;
+    T* gy = (T*)a.y + c0;
     if (s == a.tok.seqs) {
         for_free_rows(a.tok, [&](int64_t r) {
-            if (tile.active && sub == 0) store1((T*)a.y + r * a.channels + c, 0.0f);
+            for (int c = tid; c < count; c += G::kThreads) store1(gy + r * a.channels + c, 0.0f);
         });
         return;
     }
     int64_t begin, end;
     bounds_of(a.tok, s, begin, end);
-    float A[kStates], h[kStates];
-    load_states(a.A + c * a.state, first, a.state, A);
+    const bool mine = ch < count;
+    const int64_t c = c0 + (mine ? ch : 0);
+    pair_t rate[NS][2], carry[NS][2];
 #pragma unroll
-    for (int i = 0; i < kStates; ++i) h[i] = 0.0f;
-    const int64_t state_at = (s * a.channels + c) * a.state;
-    if (a.initial) load_states(a.initial + state_at, first, a.state, h);
-    const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
-    int64_t chunk = first_chunk(a.tok, s, begin);
-    for (int64_t r = begin; r < end; ++r) {
-        if (a.carries && (r - begin) % PD_SCAN_CHUNK == 0) {
-            if (tile.active)
-                for (int i = 0; i < kStates; ++i)
-                    if (first + i < a.state) a.carries[(chunk * a.channels + c) * a.state + first + i] = h[i];
-            ++chunk;
-        }
-        const float x = load1((const T*)a.x + r * a.channels + c);
-        float d = load1((const T*)a.delta + r * a.channels + c) + bias;
-        if (a.softplus) d = softplus_(d);
-        const float u = d * x;
-        float B[kStates], C[kStates], y = 0.0f;
-        const int64_t bc = (r * a.groups + tile.group) * a.state;
-        load_states((const T*)a.B + bc, first, a.state, B);
-        load_states((const T*)a.C + bc, first, a.state, C);
+    for (int q = 0; q < NS; ++q) {
+        float A[4], h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const int first = (q * LN + sub) * 4;
+        load_states(a.A + c * a.state, first, a.state, A);
+        if (a.initial) load_states(a.initial + (s * a.channels + c) * a.state, first, a.state, h);
 #pragma unroll
-        for (int i = 0; i < kStates; ++i) {
-            h[i] = exp_(d * A[i]) * h[i] + (first + i < a.state ? u * B[i] : 0.0f);
-            y += first + i < a.state ? C[i] * h[i] : 0.0f;
+        for (int p = 0; p < 2; ++p) {
+            rate[q][p] = pack(scan_rate(A[2 * p]), scan_rate(A[2 * p + 1]));
+            carry[q][p] = pack(h[2 * p], h[2 * p + 1]);
         }
-        y = sum_lanes<LN>(y);
-        if (a.skip) y += skip * x;
-        if (a.z) {
-            const float z = load1((const T*)a.z + r * a.channels + c);
-            y *= z * sigmoid_(z);
-        }
-        if (tile.active && sub == 0) store1((T*)a.y + r * a.channels + c, y);
     }
-    if (a.final_state && tile.active)
-        for (int i = 0; i < kStates; ++i)
-            if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
+    // what this thread stages: four channels of some tokens, always the same channels
+    const int c4 = tid % (G::kChannels / 4) * 4, left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
+    float bias[4], skip[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
+        skip[i] = a.skip && i < left ? a.skip[c0 + c4 + i] : 0.0f;
+    }
+    const int64_t stride = (int64_t)a.groups * a.state;
+    const T* gB = (const T*)a.B + group * a.state;
+    const T* gC = (const T*)a.C + group * a.state;
+    constexpr bool kAhead = NS == 1;     // couplings of the next tile fetched ahead (more would not fit the registers)
+    Raw4<T> rx[G::kVectors], rd[G::kVectors], rz[G::kVectors], rB[G::kCouplings], rC[G::kCouplings];
+    auto fetch = [&](int64_t from) {
+#pragma unroll
+        for (int j = 0; j < G::kVectors; ++j) {
+            const int64_t r = from + (tid + j * G::kThreads) / (G::kChannels / 4);
+            const int n = r < end ? left : 0;
+            const int64_t at = r * a.channels + c4;
+            rx[j] = fetch4(gx + at, a.vec, n);
+            rd[j] = fetch4(gdelta + at, a.vec, n);
+            if (gz) rz[j] = fetch4(gz + at, a.vec, n);
+        }
+    };
+    auto fetch_couplings = [&](int64_t from) {
+#pragma unroll
+        for (int j = 0; j < G::kCouplings; ++j) {
+            const int v = tid + j * G::kThreads, t = v / (G::kPad / 4), n4 = v % (G::kPad / 4) * 4;
+            const int64_t r = from + t;
+            int n = r < end && t < G::kTile ? a.state - n4 : 0;
+            n = n < 0 ? 0 : n > 4 ? 4 : n;
+            rB[j] = fetch4(gB + r * stride + n4, a.vec_states, n);
+            rC[j] = fetch4(gC + r * stride + n4, a.vec_states, n);
+        }
+    };
+    fetch(begin);
+    if (kAhead) fetch_couplings(begin);
+    const int64_t chunk0 = a.carries ? first_chunk(a.tok, s, begin) : 0;
+    float2* du = reinterpret_cast<float2*>(smem + G::kDu);
+    for (int64_t from = begin; from < end; from += G::kTile) {
+        // stage: step lengths and inputs in float32, the couplings as they are
+        Raw4<T> hx[G::kVectors], hz[G::kVectors];
+        if (!kAhead) fetch_couplings(from);
+#pragma unroll
+        for (int j = 0; j < G::kVectors; ++j) {
+            const int t = (tid + j * G::kThreads) / (G::kChannels / 4);
+            float2 v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float d = load1(&rd[j].e[i]) + bias[i];
+                if (a.softplus) d = softplus_(d);
+                if (i >= left || from + t >= end) d = 0.0f;
+                v[i] = make_float2(d, d * load1(&rx[j].e[i]));
+            }
+            float4* to = reinterpret_cast<float4*>(du + t * G::kChannels + c4);
+            to[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            to[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+            hx[j] = rx[j];
+            if (gz) hz[j] = rz[j];
+        }
+#pragma unroll
+        for (int j = 0; j < G::kCouplings; ++j) {
+            const int v = tid + j * G::kThreads;
+            if (v < G::kTile * G::kPad / 4) {
+                reinterpret_cast<float4*>(smem + G::kB)[v] =
+                    make_float4(load1(&rB[j].e[0]), load1(&rB[j].e[1]), load1(&rB[j].e[2]), load1(&rB[j].e[3]));
+                reinterpret_cast<float4*>(smem + G::kC)[v] =
+                    make_float4(load1(&rC[j].e[0]), load1(&rC[j].e[1]), load1(&rC[j].e[2]), load1(&rC[j].e[3]));
+            }
+        }
+        if (from + G::kTile < end) {
+            fetch(from + G::kTile);
+            if (kAhead) fetch_couplings(from + G::kTile);
+        }
+        __syncthreads();
+        float y[G::kSteps];
+#pragma unroll
+        for (int i = 0; i < G::kSteps; ++i) y[i] = 0.0f;
+        const int t0 = warp * G::kSteps;
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+            const int first = (q * LN + sub) * 4;
+            // pass 1: from a zero state
+            pair_t w[G::kSteps][2], h0 = pack(0.0f, 0.0f), h1 = h0;
+            float total = 0.0f;
+            auto driven = [&](int t, float u, pair_t& b0, pair_t& b1) {
+                const float4 B = *reinterpret_cast<const float4*>(smem + G::kB + t * G::kPad + first);
+                const pair_t uu = pack(u, u);
+                b0 = mul2(uu, pack(B.x, B.y));
+                b1 = mul2(uu, pack(B.z, B.w));
+                if (!FULL) {
+                    // states beyond the last one stay zero whatever the input is
+                    float x, y;
+                    unpack(b0, x, y);
+                    b0 = pack(first < a.state ? x : 0.0f, first + 1 < a.state ? y : 0.0f);
+                    unpack(b1, x, y);
+                    b1 = pack(first + 2 < a.state ? x : 0.0f, first + 3 < a.state ? y : 0.0f);
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < G::kSteps; ++i) {
+                const float2 v = du[(t0 + i) * G::kChannels + ch];
+                const pair_t dd = pack(v.x, v.x);
+                total += v.x;
+                w[i][0] = decay2(dd, rate[q][0]);
+                w[i][1] = decay2(dd, rate[q][1]);
+                pair_t b0, b1;
+                driven(t0 + i, v.y, b0, b1);
+                h0 = mad2(w[i][0], h0, b0);
+                h1 = mad2(w[i][1], h1, b1);
+            }
+            const pair_t tt = pack(total, total), p0 = decay2(tt, rate[q][0]), p1 = decay2(tt, rate[q][1]);
+            ulonglong2* ends = reinterpret_cast<ulonglong2*>(smem + G::kEnd);
+            ulonglong2* decays = reinterpret_cast<ulonglong2*>(smem + G::kDecay);
+            ends[tid] = make_ulonglong2(h0, h1);
+            decays[tid] = make_ulonglong2(p0, p1);
+            __syncthreads();
+            // the state entering this warp's tokens, and the one leaving the tile
+            h0 = carry[q][0];
+            h1 = carry[q][1];
+            pair_t in0 = h0, in1 = h1;
+#pragma unroll
+            for (int k = 0; k < G::kWarps; ++k) {
+                const ulonglong2 e = ends[k * 32 + lane], p = decays[k * 32 + lane];
+                if (k == warp) { in0 = h0; in1 = h1; }
+                h0 = mad2(p.x, h0, e.x);
+                h1 = mad2(p.y, h1, e.y);
+            }
+            carry[q][0] = h0;
+            carry[q][1] = h1;
+            if (NS > 1) __syncthreads();     // the next slice writes the same places
+            const int64_t at = from - begin + t0;
+            if (a.carries && at % PD_SCAN_CHUNK == 0 && from + t0 < end && mine) {
+                float v[4];
+                unpack(in0, v[0], v[1]);
+                unpack(in1, v[2], v[3]);
+                float* to = a.carries + ((chunk0 + at / PD_SCAN_CHUNK) * a.channels + c) * a.state;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) if (first + i < a.state) to[first + i] = v[i];
+            }
+            // pass 2: from the true one
+#pragma unroll
+            for (int i = 0; i < G::kSteps; ++i) {
+                pair_t b0, b1;
+                driven(t0 + i, du[(t0 + i) * G::kChannels + ch].y, b0, b1);
+                in0 = mad2(w[i][0], in0, b0);
+                in1 = mad2(w[i][1], in1, b1);
+                const float4 C = *reinterpret_cast<const float4*>(smem + G::kC + (t0 + i) * G::kPad + first);
+                float lo, hi;
+                unpack(mad2(pack(C.z, C.w), in1, mul2(pack(C.x, C.y), in0)), lo, hi);
+                if (NS == 1) smem[G::kY + (t0 + i) * 32 + lane] = lo + hi;
+                else y[i] += lo + hi;
+            }
+        }
+        if (NS > 1)
+#pragma unroll
+            for (int i = 0; i < G::kSteps; ++i) smem[G::kY + (t0 + i) * 32 + lane] = y[i];
+        __syncthreads();
+        // y of four channels of a token: its LN partial sums, the skip and the gate
+#pragma unroll
+        for (int j = 0; j < G::kVectors; ++j) {
+            const int t = (tid + j * G::kThreads) / (G::kChannels / 4);
+            float out[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float* part = smem + G::kY + t * 32 + (c4 + i) * LN;
+                float v;
+                if constexpr (LN == 4) {
+                    const float4 p = *reinterpret_cast<const float4*>(part);
+                    v = (p.x + p.y) + (p.z + p.w);
+                } else {
+                    v = part[0];
+#pragma unroll
+                    for (int k = 1; k < LN; ++k) v += part[k];
+                }
+                if (a.skip) v += skip[i] * load1(&hx[j].e[i]);
+                if (gz) {
+                    const float z = load1(&hz[j].e[i]);
+                    v *= z * sigmoid_(z);
+                }
+                out[i] = v;
+            }
+            if (from + t < end) put4(gy + (from + t) * a.channels + c4, a.vec, left, out);
+        }
+    }
+    if (a.final_state && warp == 0 && mine)
+#pragma unroll
+        for (int q = 0; q < NS; ++q) {
+            float v[4];
+            unpack(carry[q][0], v[0], v[1]);
+            unpack(carry[q][1], v[2], v[3]);
+            const int first = (q * LN + sub) * 4;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (first + i < a.state) a.final_state[(s * a.channels + c) * a.state + first + i] = v[i];
+        }
 }
 
 // one token per sequence; state in and out may be the same memory
@@ -746,13 +1025,29 @@ int64_t scan_tiles(const PdScanArgs& a) {
     const int64_t per = a.channels / a.groups, ch = 32 / pd_scan_lanes(a.state);
     return (per + ch - 1) / ch;
 }
+// f(lanes per channel, slices of states) for the prompt kernels: sixteen states at a time
+template <class F>
+cudaError_t by_slices(int state, F f) {
+    if (state <= 4) return f(Int<1>(), Int<1>());
+    if (state <= 8) return f(Int<2>(), Int<1>());
+    if (state <= 16) return f(Int<4>(), Int<1>());
+    if (state <= 32) return f(Int<4>(), Int<2>());
+    return f(Int<4>(), Int<4>());
+}
 cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
     return by_type(a.type, [&](auto e) {
         using T = decltype(e);
-        return by_lanes(a.state, [&](auto ln) {
-            const int64_t jobs = scan_tiles(a) * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
-            if (jobs == 0) return cudaSuccess;
-            pd_selective_scan_kernel<T, decltype(ln)::value><<<(unsigned)blocks_for(jobs, 4), 128, 0, st>>>(a);
+        return by_slices(a.state, [&](auto ln, auto ns) {
+            constexpr int LN = decltype(ln)::value, NS = decltype(ns)::value;
+            using G = ScanShape<LN, NS>;
+            const int64_t per = a.channels / a.groups, tiles = (per + G::kChannels - 1) / G::kChannels * a.groups;
+            const int64_t blocks = tiles * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
+            if (blocks == 0) return cudaSuccess;
+            auto kernel = a.state == G::kPad ? pd_selective_scan_kernel<T, LN, NS, true> : pd_selective_scan_kernel<T, LN, NS, false>;
+            constexpr int bytes = G::kFloats * 4;
+            cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            if (err != cudaSuccess) return err;
+            kernel<<<(unsigned)blocks, G::kThreads, bytes, st>>>(a);
             return cudaGetLastError();
         });
     });

@@ -38,6 +38,8 @@ struct PdConvArgs {
 struct PdScanArgs {
     PdTokens tok;
     int type, state, groups, softplus;
+    int vec;                  // tokens can be read four channels at a time
+    int vec_states;           // B and C four states at a time
     int64_t channels;
     const void *x, *delta, *B, *C, *z, *dy;
     const float *A, *bias, *skip, *initial, *carries_in, *dfinal;

@@ -171,6 +171,13 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         return PD_OK;
     }
     plan->grid = (tiles * (d.seqs + free_rows) + 3) / 4;
+    if (!grad) {
+        // one block per tile of channels (8, 16 or 32) and sequence
+        const int64_t per = d.channels / p->groups, ch = 32 / (p->state <= 4 ? 1 : p->state <= 8 ? 2 : 4);
+        plan->grid = (per + ch - 1) / ch * p->groups * (d.seqs + free_rows);
+        plan->block = 256;
+        plan->items = 16;
+    }
     if (grad) {
         in.push_back(carries);
         if (p->final) in.push_back(edge);
@@ -300,6 +307,11 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
             if (!step && p->carries) a.carries = (float*)out[o++];
         }
         if (!step && p->packed) a.tok.offsets = (const int32_t*)in[i++];
+        const size_t four = 4 * element(p->type);
+        a.vec = a.channels / a.groups % 4 == 0;
+        const void* tokens[] = {a.x, a.delta, a.z, a.dy, a.y, a.dx, a.ddelta, a.dz};
+        for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % four) a.vec = 0;
+        a.vec_states = a.state % 4 == 0 && reinterpret_cast<uintptr_t>(a.B) % four == 0 && reinterpret_cast<uintptr_t>(a.C) % four == 0;
         e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
     }
     if (e != cudaSuccess) {
