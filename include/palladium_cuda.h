@@ -248,7 +248,7 @@ typedef struct pd_causal_conv_params {
  * carries: the state entering every PD_SCAN_CHUNK-th token of a sequence, what the gradient recomputes from;
  * chunks = S * ceil(length / PD_SCAN_CHUNK), packed: length / PD_SCAN_CHUNK + S, sequence s from entry
  * offsets[s] / PD_SCAN_CHUNK + s on (entries of no chunk are not written). */
-#define PD_SCAN_CHUNK 64
+#define PD_SCAN_CHUNK 32
 #define PD_SCAN_MAX_STATE 64
 typedef struct pd_selective_scan_params {
     int64_t length, state, groups, type;

@@ -806,135 +806,405 @@ __global__ void __launch_bounds__(128) pd_selective_scan_step_kernel(PdScanArgs 
         if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
 }
 
-// Gradients, chunk by chunk from the end: the states of a chunk are recomputed from the one kept at its
-// start, then  g_t = C_t dy_t + a_{t+1} g_{t+1}  runs backwards through it.
+// ---------------------------------------------------------------------------
+// Gradients, chunk by chunk of 32 tokens from the end.  A block owns eight warps' channels of one group and one
+// sequence.  A warp takes its channels one after another, each over the whole chunk at once: a lane holds K
+// tokens' four states, LN lanes the states of a token group, 32 / LN lanes the token groups.  Forward from the
+// state kept at the chunk's start, then backwards,
+//     g_t = C_t dy_t + a_{t+1} g_{t+1},   dA += d a h_{t-1} g,  ddelta: A a h_{t-1} g + x B g,  dB += u g,  dC += dy h,
+// both as a pass from zero, a scan over the token groups by shuffles and a second pass from the true value.
+// Tokens stand across lanes, so the sums of dB and dC over channels, shared by the whole group, stay in registers
+// while a warp goes through its channels; only their sum over the eight warps passes through shared memory.
+// LN == K, and after the sums over a token's LN lanes each lane finishes one token.
+// ---------------------------------------------------------------------------
+constexpr int kGradWarps = 8, kGradThreads = 32 * kGradWarps;
+
+__device__ __forceinline__ pair_t shift_up(pair_t v, int by) {
+    float x, y;
+    unpack(v, x, y);
+    return pack(__shfl_up_sync(kFull, x, by), __shfl_up_sync(kFull, y, by));
+}
+__device__ __forceinline__ pair_t shift_down(pair_t v, int by) {
+    float x, y;
+    unpack(v, x, y);
+    return pack(__shfl_down_sync(kFull, x, by), __shfl_down_sync(kFull, y, by));
+}
+__device__ __forceinline__ float halves(pair_t v) {
+    float x, y;
+    unpack(v, x, y);
+    return x + y;
+}
+// v[i] summed over the K lanes of a group, lane i keeping the i-th sum
+template <int K>
+__device__ __forceinline__ float sum_to_lane(const float (&v)[K], int sub) {
+    if constexpr (K == 1) {
+        return v[0];
+    } else if constexpr (K == 2) {
+        return (sub & 1 ? v[1] : v[0]) + __shfl_xor_sync(kFull, sub & 1 ? v[0] : v[1], 1);
+    } else {
+        const float lo = (sub & 1 ? v[1] : v[0]) + __shfl_xor_sync(kFull, sub & 1 ? v[0] : v[1], 1);
+        const float hi = (sub & 1 ? v[3] : v[2]) + __shfl_xor_sync(kFull, sub & 1 ? v[2] : v[3], 1);
+        return (sub & 2 ? hi : lo) + __shfl_xor_sync(kFull, sub & 2 ? lo : hi, 2);
+    }
+}
+template <int K>
+__device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
+    if constexpr (K == 4) {
+        const float4 q = *reinterpret_cast<const float4*>(p);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else if constexpr (K == 2) {
+        const float2 q = *reinterpret_cast<const float2*>(p);
+        v[0] = q.x; v[1] = q.y;
+    } else {
+        v[0] = p[0];
+    }
+}
+
+struct GradShape {
+    int channels, pad, slices;    // channels per block, states rounded up, slices of 4 LN states
+    // float offsets in shared memory
+    int x, d, g, s, z, y, du, dd, carry, dA, red, skip, floats;
+    static constexpr int kRow = PD_SCAN_CHUNK;
+    __host__ __device__ GradShape(int ln, int state, int per_warp) {
+        const int wide = 4 * ln;
+        channels = kGradWarps * per_warp;
+        slices = (state + wide - 1) / wide;
+        pad = slices * wide;
+        const int cells = channels * kRow;
+        x = 0; d = x + cells; g = d + cells; s = g + cells; z = s + cells;
+        y = z + cells; du = y + (slices > 1 ? cells : 0); dd = du + (slices > 1 ? cells : 0);
+        carry = dd + (slices > 1 ? cells : 0);
+        dA = carry + channels * pad;
+        red = dA + channels * slices * 128;
+        skip = red + kGradWarps * kRow * (2 * wide + 4);
+        floats = skip + channels;
+    }
+};
+
 template <class T, int LN>
-__global__ void __launch_bounds__(128) pd_selective_scan_grad_kernel(PdScanArgs a) {
-    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch * a.groups;
-    const int64_t job = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t s = job / tiles;
-    const int lane = threadIdx.x & 31, sub = lane % LN, first = sub * kStates;
-    if (s > a.tok.seqs || (s == a.tok.seqs && !a.tok.offsets)) return;
-    const ScanTile tile = scan_tile<LN>(a, job % tiles);
-    const int64_t c = tile.channel;
-    float* bc_out = a.partial_bc + (job % tiles) * a.tok.rows * 2 * (kStates * LN);
+__global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel(PdScanArgs a) {
+    constexpr int K = LN, TL = 32 / LN, kRow = PD_SCAN_CHUNK, kWide = 4 * LN;
+    static_assert(K * TL == kRow, "a warp covers a chunk");
+    extern __shared__ float4 smem4[];
+    float* smem = reinterpret_cast<float*>(smem4);
+    const GradShape G(LN, a.state, a.per_warp);
+    float *sX = smem + G.x, *sD = smem + G.d, *sG = smem + G.g, *sS = smem + G.s, *sZ = smem + G.z;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, tl = lane / LN;
+    const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
+    const int64_t job = blockIdx.x, s = job / (tiles * a.groups);
+    const int64_t group = job / tiles % a.groups, within = job % tiles * G.channels;
+    const int64_t c0 = group * per + within;
+    const int count = (int)(per - within < G.channels ? per - within : G.channels);
+    float* bc_out = a.partial_bc + job % (tiles * a.groups) * a.tok.rows * 2 * G.pad;
     if (s == a.tok.seqs) {
         for_free_rows(a.tok, [&](int64_t r) {
-            if (tile.active && sub == 0) {
-                store1((T*)a.dx + r * a.channels + c, 0.0f);
-                store1((T*)a.ddelta + r * a.channels + c, 0.0f);
-                if (a.dz) store1((T*)a.dz + r * a.channels + c, 0.0f);
+            for (int c = tid; c < count; c += kGradThreads) {
+                store1((T*)a.dx + r * a.channels + c0 + c, 0.0f);
+                store1((T*)a.ddelta + r * a.channels + c0 + c, 0.0f);
+                if (a.dz) store1((T*)a.dz + r * a.channels + c0 + c, 0.0f);
             }
-            for (int i = lane; i < 2 * kStates * LN; i += 32) bc_out[r * 2 * kStates * LN + i] = 0.0f;
+            for (int i = tid; i < 2 * G.pad; i += kGradThreads) bc_out[r * 2 * G.pad + i] = 0.0f;
         });
         return;
     }
     int64_t begin, end;
     bounds_of(a.tok, s, begin, end);
-    float A[kStates], g[kStates], dA[kStates], h[PD_SCAN_CHUNK + 1][kStates];
-    load_states(a.A + c * a.state, first, a.state, A);
-    const int64_t state_at = (s * a.channels + c) * a.state;
-#pragma unroll
-    for (int i = 0; i < kStates; ++i) g[i] = dA[i] = 0.0f;
-    if (a.dfinal) load_states(a.dfinal + state_at, first, a.state, g);
-    const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
-    float dbias = 0.0f, dskip = 0.0f;
-    const int64_t chunks = (end - begin + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK;
-    for (int64_t k = chunks - 1; k >= 0; --k) {
-        const int64_t from = begin + k * PD_SCAN_CHUNK;
-        const int count = (int)(end - from < PD_SCAN_CHUNK ? end - from : PD_SCAN_CHUNK);
-        load_states(a.carries_in + ((first_chunk(a.tok, s, begin) + k) * a.channels + c) * a.state, first, a.state, h[0]);
-        for (int t = 0; t < count; ++t) {
-            const int64_t r = from + t;
-            const float x = load1((const T*)a.x + r * a.channels + c);
-            float d = load1((const T*)a.delta + r * a.channels + c) + bias;
-            if (a.softplus) d = softplus_(d);
-            float B[kStates];
-            load_states((const T*)a.B + (r * a.groups + tile.group) * a.state, first, a.state, B);
-#pragma unroll
-            for (int i = 0; i < kStates; ++i) h[t + 1][i] = exp_(d * A[i]) * h[t][i] + (first + i < a.state ? d * x * B[i] : 0.0f);
-        }
-        for (int t = count - 1; t >= 0; --t) {
-            const int64_t r = from + t, at = r * a.channels + c;
-            const float x = load1((const T*)a.x + at);
-            const float raw = load1((const T*)a.delta + at) + bias;
-            const float d = a.softplus ? softplus_(raw) : raw;
-            float B[kStates], C[kStates], y = 0.0f;
-            const int64_t bc = (r * a.groups + tile.group) * a.state;
-            load_states((const T*)a.B + bc, first, a.state, B);
-            load_states((const T*)a.C + bc, first, a.state, C);
-            float dy = load1((const T*)a.dy + at);
-            if (a.z) {
-#pragma unroll
-                for (int i = 0; i < kStates; ++i) y += first + i < a.state ? C[i] * h[t + 1][i] : 0.0f;
-                y = sum_lanes<LN>(y);
-                if (a.skip) y += skip * x;
-                const float z = load1((const T*)a.z + at), sig = sigmoid_(z);
-                if (tile.active && sub == 0) store1((T*)a.dz + at, dy * y * sig * (1.0f + z * (1.0f - sig)));
-                dy *= z * sig;
-            }
-            float du = 0.0f, dd = 0.0f;
-#pragma unroll
-            for (int i = 0; i < kStates; ++i) {
-                const bool in = first + i < a.state;
-                g[i] += in ? C[i] * dy : 0.0f;
-                float db = in ? g[i] * (d * x) : 0.0f, dc = in ? h[t + 1][i] * dy : 0.0f;
-                du += in ? g[i] * B[i] : 0.0f;
-                g[i] *= exp_(d * A[i]);               // the gradient of the state before the token
-                const float moved = in ? g[i] * h[t][i] : 0.0f;
-                dd += A[i] * moved;
-                dA[i] += moved * d;
-                if (!tile.active) db = dc = 0.0f;
-#pragma unroll
-                for (int m = LN; m < 32; m *= 2) {
-                    db += __shfl_xor_sync(kFull, db, m);
-                    dc += __shfl_xor_sync(kFull, dc, m);
-                }
-                if (lane < LN) {
-                    bc_out[r * 2 * kStates * LN + first + i] = db;
-                    bc_out[r * 2 * kStates * LN + kStates * LN + first + i] = dc;
-                }
-            }
-            du = sum_lanes<LN>(du);
-            dd = sum_lanes<LN>(dd) + du * x;
-            if (a.softplus) dd *= sigmoid_(raw);
-            if (tile.active && sub == 0) {
-                store1((T*)a.dx + at, du * d + (a.skip ? dy * skip : 0.0f));
-                store1((T*)a.ddelta + at, dd);
-            }
-            dbias += dd;
-            dskip += dy * x;
-        }
+    // swizzled places of (channel, token): four channels of a token and four tokens of a channel are both
+    // reached without bank conflicts
+    auto place = [](int c, int t) { return c * kRow + (t ^ ((c >> 2 & 7) << 2)); };
+    for (int i = tid; i < G.channels * G.pad; i += kGradThreads) {
+        const int c = i / G.pad, n = i % G.pad;
+        smem[G.carry + i] = a.dfinal && c < count && n < a.state ? a.dfinal[(s * a.channels + c0 + c) * a.state + n] : 0.0f;
     }
-    if (!tile.active) return;
-    float* sums = a.partial_params + (s * a.channels + c) * (a.state + 2);
-    for (int i = 0; i < kStates; ++i)
-        if (first + i < a.state) {
-            sums[first + i] = dA[i];
-            if (a.dinitial) a.dinitial[state_at + first + i] = g[i];
+    for (int i = tid; i < G.channels * G.slices * 128; i += kGradThreads) smem[G.dA + i] = 0.0f;
+    if (tid < G.channels) smem[G.skip + tid] = a.skip && tid < count ? a.skip[c0 + tid] : 0.0f;
+    // staging: four channels of one token per thread
+    const int quads = G.channels / 4, st = tid / quads, c4 = tid % quads * 4;
+    const bool stages = st < kRow;       // CH < 32: fewer vectors than threads
+    const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
+    float bias[4], dbias[4], dskip[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
+        dbias[i] = dskip[i] = 0.0f;
+    }
+    Raw4<T> rx, rd, rg, rz;
+    auto fetch = [&](int64_t from) {
+        const int n = stages && from + st < end ? left : 0;
+        const int64_t at = (from + st) * a.channels + c0 + c4;
+        rx = fetch4((const T*)a.x + at, a.vec, n);
+        rd = fetch4((const T*)a.delta + at, a.vec, n);
+        rg = fetch4((const T*)a.dy + at, a.vec, n);
+        if (a.z) rz = fetch4((const T*)a.z + at, a.vec, n);
+    };
+    const int64_t chunks = (end - begin + kRow - 1) / kRow, chunk0 = first_chunk(a.tok, s, begin);
+    const int64_t stride = (int64_t)a.groups * a.state;
+    if (chunks > 0) fetch(begin + (chunks - 1) * kRow);
+    for (int64_t k = chunks - 1; k >= 0; --k) {
+        const int64_t from = begin + k * kRow;
+        if (stages) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const bool in = i < left && from + st < end;
+                const float x = load1(&rx.e[i]), raw = load1(&rd.e[i]) + bias[i];
+                float d = raw, slope = 1.0f, g = load1(&rg.e[i]), gz = 0.0f;
+                if (a.softplus) { d = softplus_(raw); slope = sigmoid_(raw); }
+                if (a.z) {
+                    const float z = load1(&rz.e[i]), sig = sigmoid_(z);
+                    gz = g * (sig * (1.0f + z * (1.0f - sig)));
+                    g *= z * sig;
+                }
+                const int at = place(c4 + i, st);
+                sX[at] = in ? x : 0.0f;
+                sD[at] = in ? d : 0.0f;
+                sG[at] = in ? g : 0.0f;
+                sS[at] = slope;
+                sZ[at] = gz;
+                if (in) dskip[i] += g * x;
+            }
         }
-    if (sub == 0) {
-        sums[a.state] = dbias;
-        sums[a.state + 1] = dskip;
+        if (k > 0) fetch(from - kRow);
+        __syncthreads();
+        for (int q = 0; q < G.slices; ++q) {
+            const int first = q * kWide + sub * 4;
+            pair_t B[K][2], C[K][2], dB[K][2], dC[K][2];
+            {
+                int n = a.state - first;
+                n = n < 0 ? 0 : n > 4 ? 4 : n;
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const int64_t r = from + tl * K + i, at = r * stride + group * a.state + first;
+                    const Raw4<T> b = fetch4((const T*)a.B + at, a.vec_states, r < end ? n : 0);
+                    const Raw4<T> c = fetch4((const T*)a.C + at, a.vec_states, r < end ? n : 0);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        B[i][p] = pack(load1(&b.e[2 * p]), load1(&b.e[2 * p + 1]));
+                        C[i][p] = pack(load1(&c.e[2 * p]), load1(&c.e[2 * p + 1]));
+                        dB[i][p] = dC[i][p] = pack(0.0f, 0.0f);
+                    }
+                }
+            }
+            for (int cc = 0; cc < a.per_warp; ++cc) {
+                const int c = warp * a.per_warp + cc;
+                if (c >= count) break;
+                const int64_t channel = c0 + c;
+                float v[4];
+                pair_t rate[2], entry[2], leave[2];
+                load_states(a.A + channel * a.state, first, a.state, v);
+                rate[0] = pack(scan_rate(v[0]), scan_rate(v[1]));
+                rate[1] = pack(scan_rate(v[2]), scan_rate(v[3]));
+                load_states(a.carries_in + ((chunk0 + k) * a.channels + channel) * a.state, first, a.state, v);
+                entry[0] = pack(v[0], v[1]);
+                entry[1] = pack(v[2], v[3]);
+                float* kept = smem + G.carry + c * G.pad + first;
+                leave[0] = *reinterpret_cast<const pair_t*>(kept);
+                leave[1] = *reinterpret_cast<const pair_t*>(kept + 2);
+                float x[K], d[K], g[K], y[K], du[K], dd[K];
+                load_steps<K>(sX + place(c, tl * K), x);
+                load_steps<K>(sD + place(c, tl * K), d);
+                load_steps<K>(sG + place(c, tl * K), g);
+                // forward from zero, and the decay over this lane's tokens
+                pair_t w[K][2], span[2], h[K + 1][2], P[2], e[2];
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const pair_t step = pack(d[i], d[i]), u = pack(d[i] * x[i], d[i] * x[i]);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        w[i][p] = decay2(step, rate[p]);
+                        const pair_t b = mul2(u, B[i][p]);
+                        h[0][p] = i == 0 ? b : mad2(w[i][p], h[0][p], b);
+                        span[p] = i == 0 ? w[i][p] : mul2(span[p], w[i][p]);
+                    }
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    if (tl == 0) h[0][p] = mad2(span[p], entry[p], h[0][p]);
+                    P[p] = span[p];
+                }
+#pragma unroll
+                for (int off = 1; off < TL; off *= 2)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const pair_t before = shift_up(h[0][p], off * LN);
+                        if (tl >= off) h[0][p] = mad2(P[p], before, h[0][p]);
+                        if (2 * off < TL) {
+                            const pair_t more = shift_up(P[p], off * LN);
+                            if (tl >= off) P[p] = mul2(P[p], more);
+                        }
+                    }
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    h[0][p] = shift_up(h[0][p], LN);
+                    if (tl == 0) h[0][p] = entry[p];
+                }
+                // forward from the true state
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const pair_t u = pack(d[i] * x[i], d[i] * x[i]);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) h[i + 1][p] = mad2(w[i][p], h[i][p], mul2(u, B[i][p]));
+                    if (a.z) y[i] = halves(mad2(C[i][1], h[i + 1][1], mul2(C[i][0], h[i + 1][0])));
+                }
+                // backwards from zero
+#pragma unroll
+                for (int i = K - 1; i >= 0; --i) {
+                    const pair_t gg = pack(g[i], g[i]);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p)
+                        e[p] = mul2(w[i][p], i == K - 1 ? mul2(C[i][p], gg) : mad2(C[i][p], gg, e[p]));
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    if (tl == TL - 1) e[p] = mad2(span[p], leave[p], e[p]);
+                    P[p] = span[p];
+                }
+#pragma unroll
+                for (int off = 1; off < TL; off *= 2)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const pair_t behind = shift_down(e[p], off * LN);
+                        if (tl + off < TL) e[p] = mad2(P[p], behind, e[p]);
+                        if (2 * off < TL) {
+                            const pair_t more = shift_down(P[p], off * LN);
+                            if (tl + off < TL) P[p] = mul2(P[p], more);
+                        }
+                    }
+                __syncwarp();
+                if (tl == 0) {
+                    *reinterpret_cast<pair_t*>(kept) = e[0];
+                    *reinterpret_cast<pair_t*>(kept + 2) = e[1];
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    e[p] = shift_down(e[p], LN);
+                    if (tl == TL - 1) e[p] = leave[p];
+                }
+                // backwards from the true gradient
+                pair_t* sums = reinterpret_cast<pair_t*>(smem + G.dA + ((c * G.slices + q) * 32 + lane) * 4);
+                pair_t dA[2] = {sums[0], sums[1]};
+#pragma unroll
+                for (int i = K - 1; i >= 0; --i) {
+                    const pair_t gg = pack(g[i], g[i]), u = pack(d[i] * x[i], d[i] * x[i]), step = pack(d[i], d[i]);
+                    pair_t to_u, to_d;
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        const pair_t now = mad2(C[i][p], gg, e[p]);
+                        e[p] = mul2(w[i][p], now);
+                        dB[i][p] = mad2(now, u, dB[i][p]);
+                        dC[i][p] = mad2(h[i + 1][p], gg, dC[i][p]);
+                        to_u = p == 0 ? mul2(now, B[i][p]) : mad2(now, B[i][p], to_u);
+                        const pair_t moved = mul2(e[p], h[i][p]);
+                        to_d = p == 0 ? mul2(moved, rate[p]) : mad2(moved, rate[p], to_d);
+                        dA[p] = mad2(moved, step, dA[p]);
+                    }
+                    du[i] = halves(to_u);
+                    dd[i] = halves(to_d);
+                }
+                sums[0] = dA[0];
+                sums[1] = dA[1];
+                // this lane's token
+                float ty = a.z ? sum_to_lane<K>(y, sub) : 0.0f, tu = sum_to_lane<K>(du, sub), td = sum_to_lane<K>(dd, sub);
+                const int at = place(c, lane);
+                if (G.slices > 1) {
+                    if (q > 0) { ty += smem[G.y + at]; tu += smem[G.du + at]; td += smem[G.dd + at]; }
+                    smem[G.y + at] = ty; smem[G.du + at] = tu; smem[G.dd + at] = td;
+                }
+                if (q == G.slices - 1) {
+                    __syncwarp();     // the chunk's inputs of this channel give way to its gradients
+#if PD_MODE == 2
+                    td *= 0.6931471805599453f;     // rates are in units of log2(e)
+#endif
+                    const float tx = sX[at], tstep = sD[at], tg = sG[at], skip = smem[G.skip + c];
+                    sX[at] = tu * tstep + skip * tg;
+                    sD[at] = (td + tu * tx) * sS[at];
+                    if (a.z) sZ[at] *= ty + skip * tx;
+                }
+            }
+            // dB and dC over the block's warps, in order
+            float* red = smem + G.red;
+            constexpr int kStep = 2 * kWide + 4;
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                float* to = red + (warp * kRow + tl * K + i) * kStep + sub * 4;
+                *reinterpret_cast<ulonglong2*>(to) = make_ulonglong2(dB[i][0], dB[i][1]);
+                *reinterpret_cast<ulonglong2*>(to + kWide) = make_ulonglong2(dC[i][0], dC[i][1]);
+            }
+            __syncthreads();
+            for (int v = tid; v < kRow * 2 * LN; v += kGradThreads) {
+                const int t = v / (2 * LN), part = v % (2 * LN) * 4;
+                float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int k2 = 0; k2 < kGradWarps; ++k2) {
+                    const float4 p = *reinterpret_cast<const float4*>(red + (k2 * kRow + t) * kStep + part);
+                    total.x += p.x; total.y += p.y; total.z += p.z; total.w += p.w;
+                }
+                if (from + t < end) {
+                    const int which = part / kWide;
+                    *reinterpret_cast<float4*>(bc_out + ((from + t) * 2 + which) * G.pad + q * kWide + part % kWide) = total;
+                }
+            }
+            if (q + 1 < G.slices) __syncthreads();
+        }
+        if (stages) {
+            const int n = from + st < end ? left : 0;
+            const int64_t at = (from + st) * a.channels + c0 + c4;
+            float vx[4], vd[4], vz[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int p = place(c4 + i, st);
+                vx[i] = sX[p];
+                vd[i] = sD[p];
+                vz[i] = sZ[p];
+                if (i < n) dbias[i] += vd[i];
+            }
+            put4((T*)a.dx + at, a.vec, n, vx);
+            put4((T*)a.ddelta + at, a.vec, n, vd);
+            if (a.z) put4((T*)a.dz + at, a.vec, n, vz);
+        }
+        __syncthreads();
+    }
+    __syncthreads();
+    if (a.dinitial)
+        for (int i = tid; i < count * G.pad; i += kGradThreads)
+            if (i % G.pad < a.state) a.dinitial[(s * a.channels + c0 + i / G.pad) * a.state + i % G.pad] = smem[G.carry + i];
+    // the sequence's sums: dA over the token groups, dbias and dskip over the staging threads of a channel
+    float* out = a.partial_params + (s * a.channels + c0) * (a.state + 2);
+    for (int i = tid; i < count * a.state; i += kGradThreads) {
+        const int c = i / a.state, n = i % a.state;
+        const float* p = smem + G.dA + (c * G.slices + n / kWide) * 128 + n % kWide / 4 * 4 + n % 4;
+        float total = 0.0f;
+#pragma unroll
+        for (int j = 0; j < TL; ++j) total += p[j * LN * 4];
+        out[c * (a.state + 2) + n] = total;
+    }
+    float* part = smem + G.red;      // (token of the chunk, channel, 2)
+    if (stages)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            part[(st * G.channels + c4 + i) * 2] = dbias[i];
+            part[(st * G.channels + c4 + i) * 2 + 1] = dskip[i];
+        }
+    __syncthreads();
+    for (int i = tid; i < count * 2; i += kGradThreads) {
+        float total = 0.0f;
+        for (int t = 0; t < kRow; ++t) total += part[t * G.channels * 2 + i];
+        out[i / 2 * (a.state + 2) + a.state + i % 2] = total;
     }
 }
 
 // dB and dC: the tiles of a group added up in order
 template <class T>
-__global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArgs a, int lanes, int64_t tiles) {
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= a.tok.rows * a.groups * a.state) return;
-    const int n = (int)(i % a.state);
-    const int64_t g = i / a.state % a.groups, r = i / a.state / a.groups;
-    const int wide = kStates * lanes;
-    float b = 0.0f, c = 0.0f;
-    for (int64_t t = g * tiles; t < (g + 1) * tiles; ++t) {
-        const float* p = a.partial_bc + (t * a.tok.rows + r) * 2 * wide + n;
-        b += p[0];
-        c += p[wide];
-    }
-    store1((T*)a.dB + i, b);
-    store1((T*)a.dC + i, c);
+__global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArgs a, int pad, int64_t tiles) {
+    const int64_t wide = a.tok.rows * 2 * pad, i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= wide * a.groups) return;
+    const int64_t at = i % wide, g = i / wide, r = at / (2 * pad);
+    const int n = (int)(at % pad), which = (int)(at / pad % 2);
+    if (n >= a.state) return;
+    const float* p = a.partial_bc + g * tiles * wide + at;
+    float total = 0.0f;
+#pragma unroll 8
+    for (int64_t t = 0; t < tiles; ++t) total += p[t * wide];
+    store1((T*)(which ? a.dC : a.dB) + (r * a.groups + g) * a.state + n, total);
 }
 
 __global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdScanArgs a) {
@@ -942,6 +1212,7 @@ __global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdSca
     const int64_t wide = a.channels * (a.state + 2);
     if (i >= wide) return;
     float total = 0.0f;
+#pragma unroll 4
     for (int64_t s = 0; s < a.tok.seqs; ++s) total += a.partial_params[s * wide + i];
     const int64_t c = i / (a.state + 2);
     const int k = (int)(i % (a.state + 2));
@@ -1066,23 +1337,29 @@ cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {
 cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
     return by_type(a.type, [&](auto e) {
         using T = decltype(e);
-        return by_lanes(a.state, [&](auto ln) {
-            if (a.channels == 0) return cudaSuccess;
-            const int64_t jobs = scan_tiles(a) * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
-            if (jobs > 0) {
-                pd_selective_scan_grad_kernel<T, decltype(ln)::value><<<(unsigned)blocks_for(jobs, 4), 128, 0, st>>>(a);
-                cudaError_t err = cudaGetLastError();
+        auto run = [&](auto ln) -> cudaError_t {
+            constexpr int LN = decltype(ln)::value;
+            const GradShape G(LN, a.state, a.per_warp);
+            const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
+            const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
+            if (blocks > 0) {
+                auto kernel = pd_selective_scan_grad_kernel<T, LN>;
+                cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.floats * 4);
+                if (err != cudaSuccess) return err;
+                kernel<<<(unsigned)blocks, kGradThreads, G.floats * 4, st>>>(a);
+                err = cudaGetLastError();
                 if (err != cudaSuccess) return err;
             }
-            const int64_t cells = a.tok.rows * a.groups * a.state;
+            const int64_t cells = a.tok.rows * 2 * G.pad * a.groups;
             if (cells > 0) {
-                pd_selective_scan_sum_bc_kernel<T><<<(unsigned)blocks_for(cells, 256), 256, 0, st>>>(a, decltype(ln)::value, scan_tiles(a));
+                pd_selective_scan_sum_bc_kernel<T><<<(unsigned)blocks_for(cells, 256), 256, 0, st>>>(a, G.pad, tiles);
                 cudaError_t err = cudaGetLastError();
                 if (err != cudaSuccess) return err;
             }
             pd_selective_scan_sum_params_kernel<<<(unsigned)blocks_for(a.channels * (a.state + 2), 128), 128, 0, st>>>(a);
             return cudaGetLastError();
-        });
+        };
+        return a.state <= 4 ? run(Int<1>()) : a.state <= 8 ? run(Int<2>()) : run(Int<4>());
     });
 }
 

@@ -40,18 +40,22 @@ struct PdScanArgs {
     int type, state, groups, softplus;
     int vec;                  // tokens can be read four channels at a time
     int vec_states;           // B and C four states at a time
+    int per_warp;             // gradient: channels a warp takes one after another
     int64_t channels;
     const void *x, *delta, *B, *C, *z, *dy;
     const float *A, *bias, *skip, *initial, *carries_in, *dfinal;
     void *y, *dx, *ddelta, *dB, *dC, *dz;
     float *final_state, *carries, *dA, *dbias, *dskip, *dinitial;
-    // gradient: sums over the channels of one tile, (tiles, rows, 2, 4 * lanes), and over the tokens of one
-    // sequence, (seqs, channels, state + 2)
+    // gradient: sums over the channels of one tile, (tiles, rows, 2, states rounded up), and over the tokens of
+    // one sequence, (seqs, channels, state + 2)
     float *partial_bc, *partial_params;
 };
 
 // Lanes that share one channel: each holds four states.
 inline int pd_scan_lanes(int state) { return state <= 4 ? 1 : state <= 8 ? 2 : state <= 16 ? 4 : state <= 32 ? 8 : 16; }
+// The same for the prompt and gradient kernels, which take more than sixteen states in slices.
+inline int pd_scan_slice_lanes(int state) { return state <= 4 ? 1 : state <= 8 ? 2 : 4; }
+inline int pd_scan_pad(int state) { const int w = 4 * pd_scan_slice_lanes(state); return (state + w - 1) / w * w; }
 
 struct PdScanTable {
     cudaError_t (*conv)(const PdConvArgs&, cudaStream_t);
@@ -69,6 +73,7 @@ const PdScanTable* pd_scan_table_fast();
 struct PdScanPlan {
     const char* kernel_name = "";
     int64_t grid = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
+    int64_t params_offset = 0;    // gradient of the scan: where in the scratch the parameters' sums begin
     std::vector<size_t> in_bytes, out_bytes;
 };
 bool pd_is_scan_family(int family);

@@ -78,8 +78,17 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d) {
     const int64_t per = d.channels / p->groups, ch = 32 / pd_scan_lanes((int)p->state);
     return (per + ch - 1) / ch * p->groups;
 }
-int64_t scan_partial_bc(const pd_selective_scan_params* p, const Dims& d) {
-    return align256(scan_tiles(p, d) * d.rows * 8 * pd_scan_lanes((int)p->state) * 4);
+// Channels a warp of the gradient kernel takes one after another.  More of them share one sum over the block's
+// warps and one partial sum of dB and dC in memory; fewer give more blocks.
+int scan_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
+    int n = p->state > 16 ? 2 : 4;      // (slices of sixteen states need shared memory for as many sums)
+    const int64_t per = d.channels / p->groups;
+    while (n > 1 && (per + 8 * n - 1) / (8 * n) * p->groups * d.seqs < sms) n /= 2;
+    return n;
+}
+int64_t scan_partial_bc(const pd_selective_scan_params* p, const Dims& d, int sms) {
+    const int64_t per = d.channels / p->groups, ch = 8 * scan_per_warp(p, d, sms);
+    return align256((per + ch - 1) / ch * p->groups * d.rows * 2 * pd_scan_pad((int)p->state) * 4);
 }
 
 int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3], int sms, PdScanPlan* plan, char* err,
@@ -138,7 +147,6 @@ int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3],
 
 int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[3], int sms, PdScanPlan* plan, char* err,
               size_t cap) {
-    (void)sms;
     const bool step = family == PD_FAMILY_SELECTIVE_SCAN_STEP, grad = family == PD_FAMILY_SELECTIVE_SCAN_GRAD;
     const char* what = step ? "selective_scan_step" : grad ? "selective_scan_grad" : "selective_scan";
     Dims d;
@@ -170,14 +178,13 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         plan->grid = (tiles * d.seqs + 3) / 4;
         return PD_OK;
     }
-    plan->grid = (tiles * (d.seqs + free_rows) + 3) / 4;
-    if (!grad) {
-        // one block per tile of channels (8, 16 or 32) and sequence
-        const int64_t per = d.channels / p->groups, ch = 32 / (p->state <= 4 ? 1 : p->state <= 8 ? 2 : 4);
-        plan->grid = (per + ch - 1) / ch * p->groups * (d.seqs + free_rows);
-        plan->block = 256;
-        plan->items = 16;
-    }
+    // one block per tile of channels and sequence
+    const int64_t per = d.channels / p->groups;
+    const int per_warp = scan_per_warp(p, d, sms);
+    const int64_t ch = grad ? 8 * per_warp : 32 / pd_scan_slice_lanes((int)p->state);
+    plan->grid = (per + ch - 1) / ch * p->groups * (d.seqs + free_rows);
+    plan->block = 256;
+    plan->items = grad ? per_warp : 16;
     if (grad) {
         in.push_back(carries);
         if (p->final) in.push_back(edge);
@@ -188,7 +195,8 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         if (p->initial) out.push_back(edge);
         plan->kernel_name = "pd_selective_scan_grad_kernel";
         plan->launches = 3;
-        plan->scratch_bytes = scan_partial_bc(p, d) + d.seqs * d.channels * (p->state + 2) * 4;
+        plan->params_offset = scan_partial_bc(p, d, sms);
+        plan->scratch_bytes = plan->params_offset + d.seqs * d.channels * (p->state + 2) * 4;
     } else {
         if (p->initial) in.push_back(edge);
         out = {tokens};
@@ -297,9 +305,9 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
             if (p->skip) a.dskip = (float*)out[o++];
             if (p->gate) a.dz = out[o++];
             if (p->initial) a.dinitial = (float*)out[o++];
-            Dims d = {grid[0], grid[1], a.tok.rows, 0};
+            a.per_warp = (int)plan.items;
             a.partial_bc = (float*)scratch;
-            a.partial_params = (float*)((char*)scratch + scan_partial_bc(p, d));
+            a.partial_params = (float*)((char*)scratch + plan.params_offset);
         } else {
             if (!step && p->initial) a.initial = (const float*)in[i++];
             a.y = out[o++];

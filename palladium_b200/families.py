@@ -333,7 +333,7 @@ def threefry_bits(op: str = "bits", count: int = 1) -> Family:
 
 
 # ----------------------------------------------------------------------------- state-space families
-SCAN_CHUNK = 64       # tokens between two states that `selective_scan(carries=True)` keeps
+SCAN_CHUNK = 32       # tokens between two states that `selective_scan(carries=True)` keeps
 
 _TYPE_CODES = {"float32": 0, "float16": 1, "bfloat16": 2}
 

@@ -77,7 +77,7 @@ def test_out_shapes_and_operands():
     fam = families.selective_scan(130, 5, groups=2, gate=True, initial=True, final=True, carries=True, dtype="float16")
     y, final, carries = families.out_shapes(fam, (3, 8))
     assert y.shape == (3, 130, 8) and y.dtype == np.float16
-    assert final.shape == (3, 8, 5) and carries.shape == (3, 3, 8, 5) and carries.dtype == np.float32
+    assert final.shape == (3, 8, 5) and carries.shape == (3, -(-130 // families.SCAN_CHUNK), 8, 5) and carries.dtype == np.float32
     packed = families.selective_scan(130, 5, carries=True, packed=True)
     assert families.out_shapes(packed, (7, 8))[1].shape == (130 // families.SCAN_CHUNK + 7, 8, 5)
     grad = families.selective_scan_grad(130, 5, groups=2, gate=True, initial=True, final=True)
