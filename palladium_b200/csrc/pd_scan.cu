@@ -411,6 +411,16 @@ __device__ __forceinline__ void load_states(const T* p, int first, int n, float 
     for (int i = 0; i < kStates; ++i) v[i] = first + i < n ? load1(p + first + i) : 0.0f;
 }
 
+// the same for parameters and states, four at a time where the call's sizes and alignment allow
+__device__ __forceinline__ void load_states(const float* p, int first, int n, bool vec, float (&v)[kStates]) {
+    if (vec && first + 4 <= n) {
+        const float4 q = *reinterpret_cast<const float4*>(p + first);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+        load_states(p, first, n, v);
+    }
+}
+
 template <int LN>
 __device__ __forceinline__ float sum_lanes(float v) {
 #pragma unroll
@@ -807,17 +817,17 @@ __global__ void __launch_bounds__(128) pd_selective_scan_step_kernel(PdScanArgs 
 }
 
 // ---------------------------------------------------------------------------
-// Gradients, chunk by chunk of 32 tokens from the end.  A block owns eight warps' channels of one group and one
+// Gradients, chunk by chunk of 32 tokens from the end.  A block owns four warps' channels of one group and one
 // sequence.  A warp takes its channels one after another, each over the whole chunk at once: a lane holds K
 // tokens' four states, LN lanes the states of a token group, 32 / LN lanes the token groups.  Forward from the
 // state kept at the chunk's start, then backwards,
 //     g_t = C_t dy_t + a_{t+1} g_{t+1},   dA += d a h_{t-1} g,  ddelta: A a h_{t-1} g + x B g,  dB += u g,  dC += dy h,
 // both as a pass from zero, a scan over the token groups by shuffles and a second pass from the true value.
 // Tokens stand across lanes, so the sums of dB and dC over channels, shared by the whole group, stay in registers
-// while a warp goes through its channels; only their sum over the eight warps passes through shared memory.
+// while a warp goes through its channels; only their sum over the four warps passes through shared memory.
 // LN == K, and after the sums over a token's LN lanes each lane finishes one token.
 // ---------------------------------------------------------------------------
-constexpr int kGradWarps = 8, kGradThreads = 32 * kGradWarps;
+constexpr int kGradWarps = 4, kGradThreads = 32 * kGradWarps;
 
 __device__ __forceinline__ pair_t shift_up(pair_t v, int by) {
     float x, y;
@@ -876,13 +886,14 @@ struct GradShape {
         carry = dd + (slices > 1 ? cells : 0);
         dA = carry + channels * pad;
         red = dA + channels * slices * 128;
-        skip = red + kGradWarps * kRow * (2 * wide + 4);
+        const int warps = kGradWarps * kRow * (2 * wide + 4), staged = kGradThreads * 8;   // at different times
+        skip = red + (warps > staged ? warps : staged);
         floats = skip + channels;
     }
 };
 
-template <class T, int LN>
-__global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel(PdScanArgs a) {
+template <class T, int LN, bool GATE>
+__global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel(PdScanArgs a) {
     constexpr int K = LN, TL = 32 / LN, kRow = PD_SCAN_CHUNK, kWide = 4 * LN;
     static_assert(K * TL == kRow, "a warp covers a chunk");
     extern __shared__ float4 smem4[];
@@ -918,9 +929,9 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
     }
     for (int i = tid; i < G.channels * G.slices * 128; i += kGradThreads) smem[G.dA + i] = 0.0f;
     if (tid < G.channels) smem[G.skip + tid] = a.skip && tid < count ? a.skip[c0 + tid] : 0.0f;
-    // staging: four channels of one token per thread
-    const int quads = G.channels / 4, st = tid / quads, c4 = tid % quads * 4;
-    const bool stages = st < kRow;       // CH < 32: fewer vectors than threads
+    // staging: four channels of a token per thread, always the same channels
+    const int quads = G.channels / 4, rows = kGradThreads / quads, c4 = tid % quads * 4;
+    const int st = tid / quads < rows ? tid / quads : kRow;
     const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
     float bias[4], dbias[4], dskip[4];
 #pragma unroll
@@ -928,42 +939,36 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
         bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
         dbias[i] = dskip[i] = 0.0f;
     }
-    Raw4<T> rx, rd, rg, rz;
-    auto fetch = [&](int64_t from) {
-        const int n = stages && from + st < end ? left : 0;
-        const int64_t at = (from + st) * a.channels + c0 + c4;
-        rx = fetch4((const T*)a.x + at, a.vec, n);
-        rd = fetch4((const T*)a.delta + at, a.vec, n);
-        rg = fetch4((const T*)a.dy + at, a.vec, n);
-        if (a.z) rz = fetch4((const T*)a.z + at, a.vec, n);
-    };
     const int64_t chunks = (end - begin + kRow - 1) / kRow, chunk0 = first_chunk(a.tok, s, begin);
     const int64_t stride = (int64_t)a.groups * a.state;
-    if (chunks > 0) fetch(begin + (chunks - 1) * kRow);
     for (int64_t k = chunks - 1; k >= 0; --k) {
         const int64_t from = begin + k * kRow;
-        if (stages) {
+        for (int t = st; t < kRow; t += rows) {
+            const int n = from + t < end ? left : 0;
+            const int64_t at = (from + t) * a.channels + c0 + c4;
+            const Raw4<T> rx = fetch4((const T*)a.x + at, a.vec, n), rd = fetch4((const T*)a.delta + at, a.vec, n);
+            const Raw4<T> rg = fetch4((const T*)a.dy + at, a.vec, n);
+            Raw4<T> rz;
+            if (GATE) rz = fetch4((const T*)a.z + at, a.vec, n);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool in = i < left && from + st < end;
+                const bool in = i < n;
                 const float x = load1(&rx.e[i]), raw = load1(&rd.e[i]) + bias[i];
-                float d = raw, slope = 1.0f, g = load1(&rg.e[i]), gz = 0.0f;
+                float d = raw, slope = 1.0f, g = load1(&rg.e[i]);
                 if (a.softplus) { d = softplus_(raw); slope = sigmoid_(raw); }
-                if (a.z) {
+                const int at = place(c4 + i, t);
+                if (GATE) {
                     const float z = load1(&rz.e[i]), sig = sigmoid_(z);
-                    gz = g * (sig * (1.0f + z * (1.0f - sig)));
+                    sZ[at] = g * (sig * (1.0f + z * (1.0f - sig)));
                     g *= z * sig;
                 }
-                const int at = place(c4 + i, st);
                 sX[at] = in ? x : 0.0f;
                 sD[at] = in ? d : 0.0f;
                 sG[at] = in ? g : 0.0f;
                 sS[at] = slope;
-                sZ[at] = gz;
                 if (in) dskip[i] += g * x;
             }
         }
-        if (k > 0) fetch(from - kRow);
         __syncthreads();
         for (int q = 0; q < G.slices; ++q) {
             const int first = q * kWide + sub * 4;
@@ -990,10 +995,10 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
                 const int64_t channel = c0 + c;
                 float v[4];
                 pair_t rate[2], entry[2], leave[2];
-                load_states(a.A + channel * a.state, first, a.state, v);
+                load_states(a.A + channel * a.state, first, a.state, a.vec_params, v);
                 rate[0] = pack(scan_rate(v[0]), scan_rate(v[1]));
                 rate[1] = pack(scan_rate(v[2]), scan_rate(v[3]));
-                load_states(a.carries_in + ((chunk0 + k) * a.channels + channel) * a.state, first, a.state, v);
+                load_states(a.carries_in + ((chunk0 + k) * a.channels + channel) * a.state, first, a.state, a.vec_params, v);
                 entry[0] = pack(v[0], v[1]);
                 entry[1] = pack(v[2], v[3]);
                 float* kept = smem + G.carry + c * G.pad + first;
@@ -1003,70 +1008,46 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
                 load_steps<K>(sX + place(c, tl * K), x);
                 load_steps<K>(sD + place(c, tl * K), d);
                 load_steps<K>(sG + place(c, tl * K), g);
-                // forward from zero, and the decay over this lane's tokens
-                pair_t w[K][2], span[2], h[K + 1][2], P[2], e[2];
+                // both directions from zero: h[i + 1] after token i, e before token 0, and the decay over all
+                pair_t w[K][2], u[K], gg[K], h[K + 1][2], up[2], down[2], e[2];
 #pragma unroll
                 for (int i = 0; i < K; ++i) {
-                    const pair_t step = pack(d[i], d[i]), u = pack(d[i] * x[i], d[i] * x[i]);
+                    const pair_t step = pack(d[i], d[i]);
+                    u[i] = mul2(step, pack(x[i], x[i]));
+                    gg[i] = pack(g[i], g[i]);
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
                         w[i][p] = decay2(step, rate[p]);
-                        const pair_t b = mul2(u, B[i][p]);
-                        h[0][p] = i == 0 ? b : mad2(w[i][p], h[0][p], b);
-                        span[p] = i == 0 ? w[i][p] : mul2(span[p], w[i][p]);
+                        const pair_t b = mul2(u[i], B[i][p]);
+                        h[i + 1][p] = i == 0 ? b : mad2(w[i][p], h[i][p], b);
+                        up[p] = i == 0 ? w[i][p] : mul2(up[p], w[i][p]);
                     }
                 }
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    if (tl == 0) h[0][p] = mad2(span[p], entry[p], h[0][p]);
-                    P[p] = span[p];
-                }
-#pragma unroll
-                for (int off = 1; off < TL; off *= 2)
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        const pair_t before = shift_up(h[0][p], off * LN);
-                        if (tl >= off) h[0][p] = mad2(P[p], before, h[0][p]);
-                        if (2 * off < TL) {
-                            const pair_t more = shift_up(P[p], off * LN);
-                            if (tl >= off) P[p] = mul2(P[p], more);
-                        }
-                    }
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    h[0][p] = shift_up(h[0][p], LN);
-                    if (tl == 0) h[0][p] = entry[p];
-                }
-                // forward from the true state
-#pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    const pair_t u = pack(d[i] * x[i], d[i] * x[i]);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) h[i + 1][p] = mad2(w[i][p], h[i][p], mul2(u, B[i][p]));
-                    if (a.z) y[i] = halves(mad2(C[i][1], h[i + 1][1], mul2(C[i][0], h[i + 1][0])));
-                }
-                // backwards from zero
-#pragma unroll
-                for (int i = K - 1; i >= 0; --i) {
-                    const pair_t gg = pack(g[i], g[i]);
+                for (int i = K - 1; i >= 0; --i)
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
-                        e[p] = mul2(w[i][p], i == K - 1 ? mul2(C[i][p], gg) : mad2(C[i][p], gg, e[p]));
-                }
+                        e[p] = mul2(w[i][p], i == K - 1 ? mul2(C[i][p], gg[i]) : mad2(C[i][p], gg[i], e[p]));
+                // scans over the token groups.  The first group takes in the state kept for the chunk, the last the
+                // gradient that follows it; their decay then counts as zero, so that a group that has seen
+                // everything before it adds nothing more (a shuffle from beyond the edge returns the lane's own value).
+                pair_t in[2];
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
-                    if (tl == TL - 1) e[p] = mad2(span[p], leave[p], e[p]);
-                    P[p] = span[p];
+                    in[p] = h[K][p];
+                    down[p] = up[p];
+                    if (tl == 0) { in[p] = mad2(up[p], entry[p], in[p]); up[p] = 0; }
+                    if (tl == TL - 1) { e[p] = mad2(down[p], leave[p], e[p]); down[p] = 0; }
                 }
 #pragma unroll
                 for (int off = 1; off < TL; off *= 2)
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        const pair_t behind = shift_down(e[p], off * LN);
-                        if (tl + off < TL) e[p] = mad2(P[p], behind, e[p]);
+                        in[p] = mad2(up[p], shift_up(in[p], off * LN), in[p]);
+                        e[p] = mad2(down[p], shift_down(e[p], off * LN), e[p]);
                         if (2 * off < TL) {
-                            const pair_t more = shift_down(P[p], off * LN);
-                            if (tl + off < TL) P[p] = mul2(P[p], more);
+                            up[p] = mul2(up[p], shift_up(up[p], off * LN));
+                            down[p] = mul2(down[p], shift_down(down[p], off * LN));
                         }
                     }
                 __syncwarp();
@@ -1074,24 +1055,36 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
                     *reinterpret_cast<pair_t*>(kept) = e[0];
                     *reinterpret_cast<pair_t*>(kept + 2) = e[1];
                 }
+                // the true states
 #pragma unroll
                 for (int p = 0; p < 2; ++p) {
+                    in[p] = shift_up(in[p], LN);
                     e[p] = shift_down(e[p], LN);
+                    if (tl == 0) in[p] = entry[p];
                     if (tl == TL - 1) e[p] = leave[p];
+                    h[0][p] = in[p];
+#pragma unroll
+                    for (int i = 0; i < K; ++i) {
+                        in[p] = mul2(in[p], w[i][p]);
+                        h[i + 1][p] = add2(h[i + 1][p], in[p]);
+                    }
                 }
+                if (GATE)
+#pragma unroll
+                    for (int i = 0; i < K; ++i) y[i] = halves(mad2(C[i][1], h[i + 1][1], mul2(C[i][0], h[i + 1][0])));
                 // backwards from the true gradient
                 pair_t* sums = reinterpret_cast<pair_t*>(smem + G.dA + ((c * G.slices + q) * 32 + lane) * 4);
                 pair_t dA[2] = {sums[0], sums[1]};
 #pragma unroll
                 for (int i = K - 1; i >= 0; --i) {
-                    const pair_t gg = pack(g[i], g[i]), u = pack(d[i] * x[i], d[i] * x[i]), step = pack(d[i], d[i]);
+                    const pair_t step = pack(d[i], d[i]);
                     pair_t to_u, to_d;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        const pair_t now = mad2(C[i][p], gg, e[p]);
+                        const pair_t now = mad2(C[i][p], gg[i], e[p]);
                         e[p] = mul2(w[i][p], now);
-                        dB[i][p] = mad2(now, u, dB[i][p]);
-                        dC[i][p] = mad2(h[i + 1][p], gg, dC[i][p]);
+                        dB[i][p] = mad2(now, u[i], dB[i][p]);
+                        dC[i][p] = mad2(h[i + 1][p], gg[i], dC[i][p]);
                         to_u = p == 0 ? mul2(now, B[i][p]) : mad2(now, B[i][p], to_u);
                         const pair_t moved = mul2(e[p], h[i][p]);
                         to_d = p == 0 ? mul2(moved, rate[p]) : mad2(moved, rate[p], to_d);
@@ -1103,7 +1096,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
                 sums[0] = dA[0];
                 sums[1] = dA[1];
                 // this lane's token
-                float ty = a.z ? sum_to_lane<K>(y, sub) : 0.0f, tu = sum_to_lane<K>(du, sub), td = sum_to_lane<K>(dd, sub);
+                float ty = GATE ? sum_to_lane<K>(y, sub) : 0.0f, tu = sum_to_lane<K>(du, sub), td = sum_to_lane<K>(dd, sub);
                 const int at = place(c, lane);
                 if (G.slices > 1) {
                     if (q > 0) { ty += smem[G.y + at]; tu += smem[G.du + at]; td += smem[G.dd + at]; }
@@ -1117,7 +1110,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
                     const float tx = sX[at], tstep = sD[at], tg = sG[at], skip = smem[G.skip + c];
                     sX[at] = tu * tstep + skip * tg;
                     sD[at] = (td + tu * tx) * sS[at];
-                    if (a.z) sZ[at] *= ty + skip * tx;
+                    if (GATE) sZ[at] *= ty + skip * tx;
                 }
             }
             // dB and dC over the block's warps, in order
@@ -1145,21 +1138,21 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
             }
             if (q + 1 < G.slices) __syncthreads();
         }
-        if (stages) {
-            const int n = from + st < end ? left : 0;
-            const int64_t at = (from + st) * a.channels + c0 + c4;
+        for (int t = st; t < kRow; t += rows) {
+            const int n = from + t < end ? left : 0;
+            const int64_t at = (from + t) * a.channels + c0 + c4;
             float vx[4], vd[4], vz[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int p = place(c4 + i, st);
+                const int p = place(c4 + i, t);
                 vx[i] = sX[p];
                 vd[i] = sD[p];
-                vz[i] = sZ[p];
+                if (GATE) vz[i] = sZ[p];
                 if (i < n) dbias[i] += vd[i];
             }
             put4((T*)a.dx + at, a.vec, n, vx);
             put4((T*)a.ddelta + at, a.vec, n, vd);
-            if (a.z) put4((T*)a.dz + at, a.vec, n, vz);
+            if (GATE) put4((T*)a.dz + at, a.vec, n, vz);
         }
         __syncthreads();
     }
@@ -1177,8 +1170,8 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
         for (int j = 0; j < TL; ++j) total += p[j * LN * 4];
         out[c * (a.state + 2) + n] = total;
     }
-    float* part = smem + G.red;      // (token of the chunk, channel, 2)
-    if (stages)
+    float* part = smem + G.red;      // (staging row, channel, 2)
+    if (st < rows)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             part[(st * G.channels + c4 + i) * 2] = dbias[i];
@@ -1187,7 +1180,7 @@ __global__ void __launch_bounds__(kGradThreads, 2) pd_selective_scan_grad_kernel
     __syncthreads();
     for (int i = tid; i < count * 2; i += kGradThreads) {
         float total = 0.0f;
-        for (int t = 0; t < kRow; ++t) total += part[t * G.channels * 2 + i];
+        for (int t = 0; t < rows; ++t) total += part[t * G.channels * 2 + i];
         out[i / 2 * (a.state + 2) + a.state + i % 2] = total;
     }
 }
@@ -1343,7 +1336,7 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
             const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
             const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
             if (blocks > 0) {
-                auto kernel = pd_selective_scan_grad_kernel<T, LN>;
+                auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true> : pd_selective_scan_grad_kernel<T, LN, false>;
                 cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.floats * 4);
                 if (err != cudaSuccess) return err;
                 kernel<<<(unsigned)blocks, kGradThreads, G.floats * 4, st>>>(a);
