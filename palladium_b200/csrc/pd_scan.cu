@@ -83,8 +83,35 @@ __device__ __forceinline__ float sigmoid_(float v) {
     return 1.0f / (1.0f + expf(-v));
 #endif
 }
-// log(1 + e^v) without cancellation: a step size of 1e-3 is as exact as one of 10
-__device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.0f) + log1pf(exp_(-fabsf(v))); }
+// log(1 + e^v) = max(v, 0) + log1p(e), e = e^-|v| <= 1, without cancellation: a step size of 1e-3 is as exact
+// as one of 10.  FAST sums log1p(e) = 2 artanh(s), s = e / (2 + e) <= 1/3, as 2 s (1 + s^2/3 + .. + s^12/13):
+// the next term is below 2e-8 of the sum, and no branch is taken.
+__device__ __forceinline__ float log1p_unit(float e) {
+#if PD_MODE == 2
+    const float s = __fdividef(e, 2.0f + e), q = s * s;
+    float p = 1.0f / 13.0f;
+    p = fmaf(p, q, 1.0f / 11.0f);
+    p = fmaf(p, q, 1.0f / 9.0f);
+    p = fmaf(p, q, 1.0f / 7.0f);
+    p = fmaf(p, q, 1.0f / 5.0f);
+    p = fmaf(p, q, 1.0f / 3.0f);
+    return fmaf(2.0f * s, q * p, 2.0f * s);
+#else
+    return log1pf(e);
+#endif
+}
+__device__ __forceinline__ float softplus_(float v) { return fmaxf(v, 0.0f) + log1p_unit(exp_(-fabsf(v))); }
+// the same with its slope, 1 / (1 + e^-v)
+__device__ __forceinline__ float softplus_(float v, float& slope) {
+    const float e = exp_(-fabsf(v));
+#if PD_MODE == 2
+    const float r = __fdividef(1.0f, 1.0f + e);
+#else
+    const float r = 1.0f / (1.0f + e);
+#endif
+    slope = v >= 0.0f ? r : e * r;
+    return fmaxf(v, 0.0f) + log1p_unit(e);
+}
 
 // ---------------------------------------------------------------------------
 // sequences
@@ -533,6 +560,27 @@ __device__ __forceinline__ void put4(T* p, bool vec, int n, const float (&v)[4])
     }
 }
 
+// The same straight to shared memory: asynchronous where it is one aligned access of a whole vector.
+template <class T>
+__device__ __forceinline__ void copy4(T* to, const T* from, bool vec, int n) {
+    if (vec && n == 4) {
+        const unsigned at = (unsigned)__cvta_generic_to_shared(to);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(at), "l"(from), "n"(4 * sizeof(T)) : "memory");
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = i < n ? from[i] : T(0.0f);
+    }
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+template <class T>
+__device__ __forceinline__ Raw4<T> raw4(const T* p) {       // from shared memory, aligned to four elements
+    Raw4<T> r;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(r.e) = *reinterpret_cast<const uint4*>(p);
+    else *reinterpret_cast<uint2*>(r.e) = *reinterpret_cast<const uint2*>(p);
+    return r;
+}
+
 template <int LN, int NS> struct ScanShape {
     static constexpr int kWarps = 8, kSteps = 16, kTile = kWarps * kSteps, kThreads = 32 * kWarps;
     static constexpr int kChannels = 32 / LN, kPad = 4 * LN * NS;     // states, rounded up
@@ -872,23 +920,29 @@ __device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
 
 struct GradShape {
     int channels, pad, slices;    // channels per block, states rounded up, slices of 4 LN states
-    // float offsets in shared memory
-    int x, d, g, s, z, y, du, dd, carry, dA, red, skip, floats;
+    // offsets in shared memory: float32 arrays in floats, the chunks as stored behind them in bytes
+    int x, d, g, s, z, y, du, dd, carry, rate, entry, dA, red, skip, raw, couplings, bytes;
+    int pitch;                    // elements between two tokens' couplings
     static constexpr int kRow = PD_SCAN_CHUNK;
-    __host__ __device__ GradShape(int ln, int state, int per_warp) {
+    __host__ __device__ GradShape(int ln, int state, int per_warp, int element) {
         const int wide = 4 * ln;
         channels = kGradWarps * per_warp;
         slices = (state + wide - 1) / wide;
         pad = slices * wide;
+        pitch = pad + 4;          // (the token groups' rows then lie in different banks)
         const int cells = channels * kRow;
         x = 0; d = x + cells; g = d + cells; s = g + cells; z = s + cells;
         y = z + cells; du = y + (slices > 1 ? cells : 0); dd = du + (slices > 1 ? cells : 0);
         carry = dd + (slices > 1 ? cells : 0);
-        dA = carry + channels * pad;
+        rate = carry + channels * pad;
+        entry = rate + channels * pad;           // two buffers
+        dA = entry + 2 * channels * pad;
         red = dA + channels * slices * 128;
         const int warps = kGradWarps * kRow * (2 * wide + 4), staged = kGradThreads * 8;   // at different times
         skip = red + (warps > staged ? warps : staged);
-        floats = skip + channels;
+        raw = (skip + channels) * 4;             // x, delta, dy, z: (4, tokens, channels)
+        couplings = raw + 4 * cells * element;   // two buffers of B and C: (2, 2, tokens, pitch)
+        bytes = couplings + 4 * kRow * pitch * element;
     }
 };
 
@@ -898,7 +952,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
     static_assert(K * TL == kRow, "a warp covers a chunk");
     extern __shared__ float4 smem4[];
     float* smem = reinterpret_cast<float*>(smem4);
-    const GradShape G(LN, a.state, a.per_warp);
+    const GradShape G(LN, a.state, a.per_warp, sizeof(T));
     float *sX = smem + G.x, *sD = smem + G.d, *sG = smem + G.g, *sS = smem + G.s, *sZ = smem + G.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, tl = lane / LN;
     const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
@@ -927,6 +981,10 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
         const int c = i / G.pad, n = i % G.pad;
         smem[G.carry + i] = a.dfinal && c < count && n < a.state ? a.dfinal[(s * a.channels + c0 + c) * a.state + n] : 0.0f;
     }
+    for (int i = tid; i < G.channels * G.pad; i += kGradThreads) {
+        const int c = i / G.pad, n = i % G.pad;
+        smem[G.rate + i] = c < count && n < a.state ? scan_rate(a.A[(c0 + c) * a.state + n]) : 0.0f;
+    }
     for (int i = tid; i < G.channels * G.slices * 128; i += kGradThreads) smem[G.dA + i] = 0.0f;
     if (tid < G.channels) smem[G.skip + tid] = a.skip && tid < count ? a.skip[c0 + tid] : 0.0f;
     // staging: four channels of a token per thread, always the same channels
@@ -941,66 +999,94 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
     }
     const int64_t chunks = (end - begin + kRow - 1) / kRow, chunk0 = first_chunk(a.tok, s, begin);
     const int64_t stride = (int64_t)a.groups * a.state;
-    for (int64_t k = chunks - 1; k >= 0; --k) {
+    T* raw = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.raw);
+    T* couplings = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.couplings);
+    const int cells = kRow * G.channels;
+    // a chunk's operands on their way while the one behind it is worked on
+    auto copy_chunk = [&](int64_t k) {
         const int64_t from = begin + k * kRow;
         for (int t = st; t < kRow; t += rows) {
-            const int n = from + t < end ? left : 0;
+            const int n = from + t < end ? left : 0, to = t * G.channels + c4;
             const int64_t at = (from + t) * a.channels + c0 + c4;
-            const Raw4<T> rx = fetch4((const T*)a.x + at, a.vec, n), rd = fetch4((const T*)a.delta + at, a.vec, n);
-            const Raw4<T> rg = fetch4((const T*)a.dy + at, a.vec, n);
+            copy4(raw + to, (const T*)a.x + at, a.vec, n);
+            copy4(raw + cells + to, (const T*)a.delta + at, a.vec, n);
+            copy4(raw + 2 * cells + to, (const T*)a.dy + at, a.vec, n);
+            if (GATE) copy4(raw + 3 * cells + to, (const T*)a.z + at, a.vec, n);
+        }
+        for (int i = tid; i < kRow * (G.pad / 4); i += kGradThreads) {
+            const int t = i / (G.pad / 4), n4 = i % (G.pad / 4) * 4;
+            int n = from + t < end ? a.state - n4 : 0;
+            n = n < 0 ? 0 : n > 4 ? 4 : n;
+            const int64_t at = (from + t) * stride + group * a.state + n4;
+            T* to = couplings + ((int)(k & 1) * 2 * kRow + t) * G.pitch + n4;
+            copy4(to, (const T*)a.B + at, a.vec_states, n);
+            copy4(to + kRow * G.pitch, (const T*)a.C + at, a.vec_states, n);
+        }
+        for (int i = tid; i < G.channels * (G.pad / 4); i += kGradThreads) {
+            const int c = i / (G.pad / 4), n4 = i % (G.pad / 4) * 4;
+            int n = c < count ? a.state - n4 : 0;
+            n = n < 0 ? 0 : n > 4 ? 4 : n;
+            copy4(smem + G.entry + ((int)(k & 1) * G.channels + c) * G.pad + n4,
+                  a.carries_in + ((chunk0 + k) * a.channels + c0 + c) * a.state + n4, a.vec_params, n);
+        }
+        copies_commit();
+    };
+    if (chunks > 0) copy_chunk(chunks - 1);
+    for (int64_t k = chunks - 1; k >= 0; --k) {
+        const int64_t from = begin + k * kRow;
+        copies_wait();
+        // (each thread reads back what it has fetched itself)
+        for (int t = st; t < kRow; t += rows) {
+            const int n = from + t < end ? left : 0, to = t * G.channels + c4;
+            const Raw4<T> rx = raw4(raw + to), rd = raw4(raw + cells + to), rg = raw4(raw + 2 * cells + to);
             Raw4<T> rz;
-            if (GATE) rz = fetch4((const T*)a.z + at, a.vec, n);
+            if (GATE) rz = raw4(raw + 3 * cells + to);
+            const int row = place(c4, t);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const bool in = i < n;
-                const float x = load1(&rx.e[i]), raw = load1(&rd.e[i]) + bias[i];
-                float d = raw, slope = 1.0f, g = load1(&rg.e[i]);
-                if (a.softplus) { d = softplus_(raw); slope = sigmoid_(raw); }
-                const int at = place(c4 + i, t);
+                const int at = row + i * kRow;
+                const float x = load1(&rx.e[i]), bent = load1(&rd.e[i]) + bias[i];
+                float d = bent, slope = 1.0f, g = load1(&rg.e[i]);
+                if (a.softplus) d = softplus_(bent, slope);
                 if (GATE) {
                     const float z = load1(&rz.e[i]), sig = sigmoid_(z);
                     sZ[at] = g * (sig * (1.0f + z * (1.0f - sig)));
                     g *= z * sig;
                 }
-                sX[at] = in ? x : 0.0f;
-                sD[at] = in ? d : 0.0f;
-                sG[at] = in ? g : 0.0f;
+                // (what lies behind the sequence's end was fetched as zeros)
+                sX[at] = x;
+                sD[at] = i < n ? d : 0.0f;
+                sG[at] = g;
                 sS[at] = slope;
-                if (in) dskip[i] += g * x;
+                dskip[i] += g * x;
             }
         }
+        if (k > 0) copy_chunk(k - 1);
         __syncthreads();
         for (int q = 0; q < G.slices; ++q) {
             const int first = q * kWide + sub * 4;
             pair_t B[K][2], C[K][2], dB[K][2], dC[K][2];
-            {
-                int n = a.state - first;
-                n = n < 0 ? 0 : n > 4 ? 4 : n;
 #pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    const int64_t r = from + tl * K + i, at = r * stride + group * a.state + first;
-                    const Raw4<T> b = fetch4((const T*)a.B + at, a.vec_states, r < end ? n : 0);
-                    const Raw4<T> c = fetch4((const T*)a.C + at, a.vec_states, r < end ? n : 0);
+            for (int i = 0; i < K; ++i) {
+                const T* from_row = couplings + ((int)(k & 1) * 2 * kRow + tl * K + i) * G.pitch + first;
+                const Raw4<T> b = raw4(from_row), c = raw4(from_row + kRow * G.pitch);
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        B[i][p] = pack(load1(&b.e[2 * p]), load1(&b.e[2 * p + 1]));
-                        C[i][p] = pack(load1(&c.e[2 * p]), load1(&c.e[2 * p + 1]));
-                        dB[i][p] = dC[i][p] = pack(0.0f, 0.0f);
-                    }
+                for (int p = 0; p < 2; ++p) {
+                    B[i][p] = pack(load1(&b.e[2 * p]), load1(&b.e[2 * p + 1]));
+                    C[i][p] = pack(load1(&c.e[2 * p]), load1(&c.e[2 * p + 1]));
+                    dB[i][p] = dC[i][p] = pack(0.0f, 0.0f);
                 }
             }
             for (int cc = 0; cc < a.per_warp; ++cc) {
                 const int c = warp * a.per_warp + cc;
                 if (c >= count) break;
-                const int64_t channel = c0 + c;
-                float v[4];
                 pair_t rate[2], entry[2], leave[2];
-                load_states(a.A + channel * a.state, first, a.state, a.vec_params, v);
-                rate[0] = pack(scan_rate(v[0]), scan_rate(v[1]));
-                rate[1] = pack(scan_rate(v[2]), scan_rate(v[3]));
-                load_states(a.carries_in + ((chunk0 + k) * a.channels + channel) * a.state, first, a.state, a.vec_params, v);
-                entry[0] = pack(v[0], v[1]);
-                entry[1] = pack(v[2], v[3]);
+                const pair_t* rates = reinterpret_cast<const pair_t*>(smem + G.rate + c * G.pad + first);
+                const pair_t* entries = reinterpret_cast<const pair_t*>(smem + G.entry + ((int)(k & 1) * G.channels + c) * G.pad + first);
+                rate[0] = rates[0];
+                rate[1] = rates[1];
+                entry[0] = entries[0];
+                entry[1] = entries[1];
                 float* kept = smem + G.carry + c * G.pad + first;
                 leave[0] = *reinterpret_cast<const pair_t*>(kept);
                 leave[1] = *reinterpret_cast<const pair_t*>(kept + 2);
@@ -1141,10 +1227,11 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
         for (int t = st; t < kRow; t += rows) {
             const int n = from + t < end ? left : 0;
             const int64_t at = (from + t) * a.channels + c0 + c4;
+            const int row = place(c4, t);
             float vx[4], vd[4], vz[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int p = place(c4 + i, t);
+                const int p = row + i * kRow;
                 vx[i] = sX[p];
                 vd[i] = sD[p];
                 if (GATE) vz[i] = sZ[p];
@@ -1332,14 +1419,14 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
         using T = decltype(e);
         auto run = [&](auto ln) -> cudaError_t {
             constexpr int LN = decltype(ln)::value;
-            const GradShape G(LN, a.state, a.per_warp);
+            const GradShape G(LN, a.state, a.per_warp, sizeof(T));
             const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
             const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
             if (blocks > 0) {
                 auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true> : pd_selective_scan_grad_kernel<T, LN, false>;
-                cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.floats * 4);
+                cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.bytes);
                 if (err != cudaSuccess) return err;
-                kernel<<<(unsigned)blocks, kGradThreads, G.floats * 4, st>>>(a);
+                kernel<<<(unsigned)blocks, kGradThreads, G.bytes, st>>>(a);
                 err = cudaGetLastError();
                 if (err != cudaSuccess) return err;
             }
