@@ -468,18 +468,6 @@ __device__ __forceinline__ ScanTile scan_tile(const PdScanArgs& a, int64_t tile)
     return t;
 }
 
-// ---------------------------------------------------------------------------
-// The prompt kernel.  A block owns CH = 32 / LN channels of one group and walks one sequence in tiles of
-// 128 tokens: warp w takes tokens 16 w .. 16 w + 15 of the tile, a lane four states of one channel.  Every
-// warp integrates its 16 tokens from a zero state and keeps the 64 decays in registers; the warps' end
-// states and total decays meet in shared memory, where each lane composes the state entering its own tokens;
-// a second pass over the same registers then yields y.  So one exponential per (token, channel, state) is
-// all that is taken, whatever the number of sequences, and a single sequence of 2048 channels already
-// gives 256 blocks of eight warps.
-//
-// Bound: the exponentials, 16 per clock and SM (8 cycles per warp instruction and scheduler); next to each
-// stand six float32 operations, issued two by two, and 1.25 reads of shared memory.
-// ---------------------------------------------------------------------------
 typedef unsigned long long pair_t;     // two float32 in one 64-bit register
 __device__ __forceinline__ pair_t pack(float x, float y) {
     pair_t v;
@@ -581,251 +569,6 @@ __device__ __forceinline__ Raw4<T> raw4(const T* p) {       // from shared memor
     return r;
 }
 
-template <int LN, int NS> struct ScanShape {
-    static constexpr int kWarps = 8, kSteps = 16, kTile = kWarps * kSteps, kThreads = 32 * kWarps;
-    static constexpr int kChannels = 32 / LN, kPad = 4 * LN * NS;     // states, rounded up
-    static constexpr int kDu = 0, kB = kDu + 2 * kTile * kChannels, kC = kB + kTile * kPad, kY = kC + kTile * kPad,
-                         kEnd = kY + kTile * 32, kDecay = kEnd + kThreads * 4, kFloats = kDecay + kThreads * 4;
-    static constexpr int kVectors = kTile * kChannels / 4 / kThreads;  // vectors of four channels per thread
-    static constexpr int kCouplings = (kTile * kPad / 4 + kThreads - 1) / kThreads;
-};
-
-template <class T, int LN, int NS, bool FULL>
-__global__ void __launch_bounds__(256, 2) pd_selective_scan_kernel(PdScanArgs a) {
-    using G = ScanShape<LN, NS>;
-    extern __shared__ float4 smem4[];
-    float* smem = reinterpret_cast<float*>(smem4);
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, ch = lane / LN;
-    const int64_t per = a.channels / a.groups, tiles = (per + G::kChannels - 1) / G::kChannels;
-    const int64_t job = blockIdx.x, s = job / (tiles * a.groups);
-    const int64_t group = job / tiles % a.groups, within = job % tiles * G::kChannels;
-    const int64_t c0 = group * per + within;                            // the block's first channel
-    const int count = (int)(per - within < G::kChannels ? per - within : G::kChannels);
-    const T* gx = (const T*)a.x + c0;
-    const T* gdelta = (const T*)a.delta + c0;
-    const T* gz = a.z ? (const T*)a.z + c0 : nullptr;
-    T* gy = (T*)a.y + c0;
-    if (s == a.tok.seqs) {
-        for_free_rows(a.tok, [&](int64_t r) {
-            for (int c = tid; c < count; c += G::kThreads) store1(gy + r * a.channels + c, 0.0f);
-        });
-        return;
-    }
-    int64_t begin, end;
-    bounds_of(a.tok, s, begin, end);
-    const bool mine = ch < count;
-    const int64_t c = c0 + (mine ? ch : 0);
-    pair_t rate[NS][2], carry[NS][2];
-#pragma unroll
-    for (int q = 0; q < NS; ++q) {
-        float A[4], h[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        const int first = (q * LN + sub) * 4;
-        load_states(a.A + c * a.state, first, a.state, A);
-        if (a.initial) load_states(a.initial + (s * a.channels + c) * a.state, first, a.state, h);
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-            rate[q][p] = pack(scan_rate(A[2 * p]), scan_rate(A[2 * p + 1]));
-            carry[q][p] = pack(h[2 * p], h[2 * p + 1]);
-        }
-    }
-    // what this thread stages: four channels of some tokens, always the same channels
-    const int c4 = tid % (G::kChannels / 4) * 4, left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
-    float bias[4], skip[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
-        skip[i] = a.skip && i < left ? a.skip[c0 + c4 + i] : 0.0f;
-    }
-    const int64_t stride = (int64_t)a.groups * a.state;
-    const T* gB = (const T*)a.B + group * a.state;
-    const T* gC = (const T*)a.C + group * a.state;
-    constexpr bool kAhead = NS == 1;     // couplings of the next tile fetched ahead (more would not fit the registers)
-    Raw4<T> rx[G::kVectors], rd[G::kVectors], rz[G::kVectors], rB[G::kCouplings], rC[G::kCouplings];
-    auto fetch = [&](int64_t from) {
-#pragma unroll
-        for (int j = 0; j < G::kVectors; ++j) {
-            const int64_t r = from + (tid + j * G::kThreads) / (G::kChannels / 4);
-            const int n = r < end ? left : 0;
-            const int64_t at = r * a.channels + c4;
-            rx[j] = fetch4(gx + at, a.vec, n);
-            rd[j] = fetch4(gdelta + at, a.vec, n);
-            if (gz) rz[j] = fetch4(gz + at, a.vec, n);
-        }
-    };
-    auto fetch_couplings = [&](int64_t from) {
-#pragma unroll
-        for (int j = 0; j < G::kCouplings; ++j) {
-            const int v = tid + j * G::kThreads, t = v / (G::kPad / 4), n4 = v % (G::kPad / 4) * 4;
-            const int64_t r = from + t;
-            int n = r < end && t < G::kTile ? a.state - n4 : 0;
-            n = n < 0 ? 0 : n > 4 ? 4 : n;
-            rB[j] = fetch4(gB + r * stride + n4, a.vec_states, n);
-            rC[j] = fetch4(gC + r * stride + n4, a.vec_states, n);
-        }
-    };
-    fetch(begin);
-    if (kAhead) fetch_couplings(begin);
-    const int64_t chunk0 = a.carries ? first_chunk(a.tok, s, begin) : 0;
-    float2* du = reinterpret_cast<float2*>(smem + G::kDu);
-    for (int64_t from = begin; from < end; from += G::kTile) {
-        // stage: step lengths and inputs in float32, the couplings as they are
-        Raw4<T> hx[G::kVectors], hz[G::kVectors];
-        if (!kAhead) fetch_couplings(from);
-#pragma unroll
-        for (int j = 0; j < G::kVectors; ++j) {
-            const int t = (tid + j * G::kThreads) / (G::kChannels / 4);
-            float2 v[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float d = load1(&rd[j].e[i]) + bias[i];
-                if (a.softplus) d = softplus_(d);
-                if (i >= left || from + t >= end) d = 0.0f;
-                v[i] = make_float2(d, d * load1(&rx[j].e[i]));
-            }
-            float4* to = reinterpret_cast<float4*>(du + t * G::kChannels + c4);
-            to[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-            to[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
-            hx[j] = rx[j];
-            if (gz) hz[j] = rz[j];
-        }
-#pragma unroll
-        for (int j = 0; j < G::kCouplings; ++j) {
-            const int v = tid + j * G::kThreads;
-            if (v < G::kTile * G::kPad / 4) {
-                reinterpret_cast<float4*>(smem + G::kB)[v] =
-                    make_float4(load1(&rB[j].e[0]), load1(&rB[j].e[1]), load1(&rB[j].e[2]), load1(&rB[j].e[3]));
-                reinterpret_cast<float4*>(smem + G::kC)[v] =
-                    make_float4(load1(&rC[j].e[0]), load1(&rC[j].e[1]), load1(&rC[j].e[2]), load1(&rC[j].e[3]));
-            }
-        }
-        if (from + G::kTile < end) {
-            fetch(from + G::kTile);
-            if (kAhead) fetch_couplings(from + G::kTile);
-        }
-        __syncthreads();
-        float y[G::kSteps];
-#pragma unroll
-        for (int i = 0; i < G::kSteps; ++i) y[i] = 0.0f;
-        const int t0 = warp * G::kSteps;
-#pragma unroll
-        for (int q = 0; q < NS; ++q) {
-            const int first = (q * LN + sub) * 4;
-            // pass 1: from a zero state
-            pair_t w[G::kSteps][2], h0 = pack(0.0f, 0.0f), h1 = h0;
-            float total = 0.0f;
-            auto driven = [&](int t, float u, pair_t& b0, pair_t& b1) {
-                const float4 B = *reinterpret_cast<const float4*>(smem + G::kB + t * G::kPad + first);
-                const pair_t uu = pack(u, u);
-                b0 = mul2(uu, pack(B.x, B.y));
-                b1 = mul2(uu, pack(B.z, B.w));
-                if (!FULL) {
-                    // states beyond the last one stay zero whatever the input is
-                    float x, y;
-                    unpack(b0, x, y);
-                    b0 = pack(first < a.state ? x : 0.0f, first + 1 < a.state ? y : 0.0f);
-                    unpack(b1, x, y);
-                    b1 = pack(first + 2 < a.state ? x : 0.0f, first + 3 < a.state ? y : 0.0f);
-                }
-            };
-#pragma unroll
-            for (int i = 0; i < G::kSteps; ++i) {
-                const float2 v = du[(t0 + i) * G::kChannels + ch];
-                const pair_t dd = pack(v.x, v.x);
-                total += v.x;
-                w[i][0] = decay2(dd, rate[q][0]);
-                w[i][1] = decay2(dd, rate[q][1]);
-                pair_t b0, b1;
-                driven(t0 + i, v.y, b0, b1);
-                h0 = mad2(w[i][0], h0, b0);
-                h1 = mad2(w[i][1], h1, b1);
-            }
-            const pair_t tt = pack(total, total), p0 = decay2(tt, rate[q][0]), p1 = decay2(tt, rate[q][1]);
-            ulonglong2* ends = reinterpret_cast<ulonglong2*>(smem + G::kEnd);
-            ulonglong2* decays = reinterpret_cast<ulonglong2*>(smem + G::kDecay);
-            ends[tid] = make_ulonglong2(h0, h1);
-            decays[tid] = make_ulonglong2(p0, p1);
-            __syncthreads();
-            // the state entering this warp's tokens, and the one leaving the tile
-            h0 = carry[q][0];
-            h1 = carry[q][1];
-            pair_t in0 = h0, in1 = h1;
-#pragma unroll
-            for (int k = 0; k < G::kWarps; ++k) {
-                const ulonglong2 e = ends[k * 32 + lane], p = decays[k * 32 + lane];
-                if (k == warp) { in0 = h0; in1 = h1; }
-                h0 = mad2(p.x, h0, e.x);
-                h1 = mad2(p.y, h1, e.y);
-            }
-            carry[q][0] = h0;
-            carry[q][1] = h1;
-            if (NS > 1) __syncthreads();     // the next slice writes the same places
-            const int64_t at = from - begin + t0;
-            if (a.carries && at % PD_SCAN_CHUNK == 0 && from + t0 < end && mine) {
-                float v[4];
-                unpack(in0, v[0], v[1]);
-                unpack(in1, v[2], v[3]);
-                float* to = a.carries + ((chunk0 + at / PD_SCAN_CHUNK) * a.channels + c) * a.state;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) if (first + i < a.state) to[first + i] = v[i];
-            }
-            // pass 2: from the true one
-#pragma unroll
-            for (int i = 0; i < G::kSteps; ++i) {
-                pair_t b0, b1;
-                driven(t0 + i, du[(t0 + i) * G::kChannels + ch].y, b0, b1);
-                in0 = mad2(w[i][0], in0, b0);
-                in1 = mad2(w[i][1], in1, b1);
-                const float4 C = *reinterpret_cast<const float4*>(smem + G::kC + (t0 + i) * G::kPad + first);
-                float lo, hi;
-                unpack(mad2(pack(C.z, C.w), in1, mul2(pack(C.x, C.y), in0)), lo, hi);
-                if (NS == 1) smem[G::kY + (t0 + i) * 32 + lane] = lo + hi;
-                else y[i] += lo + hi;
-            }
-        }
-        if (NS > 1)
-#pragma unroll
-            for (int i = 0; i < G::kSteps; ++i) smem[G::kY + (t0 + i) * 32 + lane] = y[i];
-        __syncthreads();
-        // y of four channels of a token: its LN partial sums, the skip and the gate
-#pragma unroll
-        for (int j = 0; j < G::kVectors; ++j) {
-            const int t = (tid + j * G::kThreads) / (G::kChannels / 4);
-            float out[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float* part = smem + G::kY + t * 32 + (c4 + i) * LN;
-                float v;
-                if constexpr (LN == 4) {
-                    const float4 p = *reinterpret_cast<const float4*>(part);
-                    v = (p.x + p.y) + (p.z + p.w);
-                } else {
-                    v = part[0];
-#pragma unroll
-                    for (int k = 1; k < LN; ++k) v += part[k];
-                }
-                if (a.skip) v += skip[i] * load1(&hx[j].e[i]);
-                if (gz) {
-                    const float z = load1(&hz[j].e[i]);
-                    v *= z * sigmoid_(z);
-                }
-                out[i] = v;
-            }
-            if (from + t < end) put4(gy + (from + t) * a.channels + c4, a.vec, left, out);
-        }
-    }
-    if (a.final_state && warp == 0 && mine)
-#pragma unroll
-        for (int q = 0; q < NS; ++q) {
-            float v[4];
-            unpack(carry[q][0], v[0], v[1]);
-            unpack(carry[q][1], v[2], v[3]);
-            const int first = (q * LN + sub) * 4;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (first + i < a.state) a.final_state[(s * a.channels + c) * a.state + first + i] = v[i];
-        }
-}
-
 // one token per sequence; state in and out may be the same memory
 template <class T, int LN>
 __global__ void __launch_bounds__(128) pd_selective_scan_step_kernel(PdScanArgs a) {
@@ -865,18 +608,8 @@ __global__ void __launch_bounds__(128) pd_selective_scan_step_kernel(PdScanArgs 
 }
 
 // ---------------------------------------------------------------------------
-// Gradients, chunk by chunk of 32 tokens from the end.  A block owns four warps' channels of one group and one
-// sequence.  A warp takes its channels one after another, each over the whole chunk at once: a lane holds K
-// tokens' four states, LN lanes the states of a token group, 32 / LN lanes the token groups.  Forward from the
-// state kept at the chunk's start, then backwards,
-//     g_t = C_t dy_t + a_{t+1} g_{t+1},   dA += d a h_{t-1} g,  ddelta: A a h_{t-1} g + x B g,  dB += u g,  dC += dy h,
-// both as a pass from zero, a scan over the token groups by shuffles and a second pass from the true value.
-// Tokens stand across lanes, so the sums of dB and dC over channels, shared by the whole group, stay in registers
-// while a warp goes through its channels; only their sum over the four warps passes through shared memory.
-// LN == K, and after the sums over a token's LN lanes each lane finishes one token.
+// what the prompt and gradient kernels share
 // ---------------------------------------------------------------------------
-constexpr int kGradWarps = 4, kGradThreads = 32 * kGradWarps;
-
 __device__ __forceinline__ pair_t shift_up(pair_t v, int by) {
     float x, y;
     unpack(v, x, y);
@@ -905,6 +638,12 @@ __device__ __forceinline__ float sum_to_lane(const float (&v)[K], int sub) {
         return (sub & 2 ? hi : lo) + __shfl_xor_sync(kFull, sub & 2 ? lo : hi, 2);
     }
 }
+// a pair of states of which the first n exist
+__device__ __forceinline__ pair_t keep_states(pair_t v, int n) {
+    float x, y;
+    unpack(v, x, y);
+    return pack(n > 0 ? x : 0.0f, n > 1 ? y : 0.0f);
+}
 template <int K>
 __device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
     if constexpr (K == 4) {
@@ -917,6 +656,273 @@ __device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
         v[0] = p[0];
     }
 }
+
+// ---------------------------------------------------------------------------
+// The prompt kernel.  A block owns four warps' channels of one group and walks one sequence in tiles of 64
+// tokens.  A warp takes its channels one after another, each over the whole tile at once: a lane holds K tokens'
+// four states, LN lanes the states of a token group, 32 / LN lanes the token groups.  A pass from a zero state
+// keeps the decays exp(d A) in registers, a scan over the token groups by shuffles gives the state entering each,
+// and a second pass over the same registers the outputs: one exponential per (token, channel, state).  With tokens
+// across lanes a single sequence fills the GPU, and B and C, which all channels of a group share, are read from
+// shared memory once per tile and warp instead of once per channel (a layout with channels across lanes, decays
+// in registers and warps across tokens spent its time reading them: 5 words of shared memory per state).
+// ---------------------------------------------------------------------------
+#ifndef PD_SCAN_BLOCKS
+#define PD_SCAN_BLOCKS 3
+#endif
+constexpr int kScanWarps = 4, kScanThreads = 32 * kScanWarps;
+
+struct ScanShape {
+    int channels, pad, slices, pitch;
+    int x, d, z, y, carry, rate, skip, raw, couplings, bytes;
+    static constexpr int kRow = 64;
+    __host__ __device__ ScanShape(int ln, int state, int per_warp, int element) {
+        const int wide = 4 * ln;
+        channels = kScanWarps * per_warp;
+        slices = (state + wide - 1) / wide;
+        pad = slices * wide;
+        pitch = pad + 4;          // elements between two tokens' couplings: the token groups lie in different banks
+        const int cells = channels * kRow;
+        x = 0; d = x + cells; z = d + cells; y = z + cells;
+        carry = y + (slices > 1 ? cells : 0);
+        rate = carry + channels * pad;
+        skip = rate + channels * pad;
+        raw = (skip + channels) * 4;             // x, delta, z: (3, tokens, channels)
+        couplings = raw + 3 * cells * element;   // two buffers of B and C: (2, 2, tokens, pitch)
+        bytes = couplings + 4 * kRow * pitch * element;
+    }
+};
+
+template <class T, int LN, bool GATE, bool FULL>
+__global__ void __launch_bounds__(kScanThreads, PD_SCAN_BLOCKS) pd_selective_scan_kernel(PdScanArgs a) {
+    constexpr int K = 2 * LN, TL = 32 / LN, kRow = ScanShape::kRow, kWide = 4 * LN, kPart = K < 4 ? K : 4;
+    static_assert(K * TL == kRow && kRow % PD_SCAN_CHUNK == 0 && PD_SCAN_CHUNK % K == 0, "a warp covers a tile of whole chunks");
+    extern __shared__ float4 smem4[];
+    float* smem = reinterpret_cast<float*>(smem4);
+    const ScanShape G(LN, a.state, a.per_warp, sizeof(T));
+    float *sX = smem + G.x, *sD = smem + G.d, *sZ = smem + G.z;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, tl = lane / LN;
+    const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
+    const int64_t job = blockIdx.x, s = job / (tiles * a.groups);
+    const int64_t group = job / tiles % a.groups, within = job % tiles * G.channels;
+    const int64_t c0 = group * per + within;                            // the block's first channel
+    const int count = (int)(per - within < G.channels ? per - within : G.channels);
+    if (s == a.tok.seqs) {
+        for_free_rows(a.tok, [&](int64_t r) {
+            for (int c = tid; c < count; c += kScanThreads) store1((T*)a.y + r * a.channels + c0 + c, 0.0f);
+        });
+        return;
+    }
+    int64_t begin, end;
+    bounds_of(a.tok, s, begin, end);
+    // swizzled places of (channel, token), as in the gradient kernel
+    auto place = [](int c, int t) { return c * kRow + (t ^ ((c >> 2 & 7) << 2)); };
+    for (int i = tid; i < G.channels * G.pad; i += kScanThreads) {
+        const int c = i / G.pad, n = i % G.pad;
+        const bool in = c < count && n < a.state;
+        smem[G.carry + i] = a.initial && in ? a.initial[(s * a.channels + c0 + c) * a.state + n] : 0.0f;
+        smem[G.rate + i] = in ? scan_rate(a.A[(c0 + c) * a.state + n]) : 0.0f;
+    }
+    if (tid < G.channels) smem[G.skip + tid] = a.skip && tid < count ? a.skip[c0 + tid] : 0.0f;
+    // staging: four channels of a token per thread, always the same channels
+    const int quads = G.channels / 4, rows = kScanThreads / quads, c4 = tid % quads * 4;
+    const int st = tid / quads < rows ? tid / quads : kRow;
+    const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
+    float bias[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
+    const int64_t chunk0 = first_chunk(a.tok, s, begin), stride = (int64_t)a.groups * a.state;
+    T* raw = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.raw);
+    T* couplings = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.couplings);
+    const int cells = kRow * G.channels;
+    // a tile's operands on their way while the one before it is worked on
+    auto copy_tile = [&](int64_t from, int buffer) {
+        for (int t = st; t < kRow; t += rows) {
+            const int n = from + t < end ? left : 0, to = t * G.channels + c4;
+            const int64_t at = (from + t) * a.channels + c0 + c4;
+            copy4(raw + to, (const T*)a.x + at, a.vec, n);
+            copy4(raw + cells + to, (const T*)a.delta + at, a.vec, n);
+            if (GATE) copy4(raw + 2 * cells + to, (const T*)a.z + at, a.vec, n);
+        }
+        for (int i = tid; i < kRow * (G.pad / 4); i += kScanThreads) {
+            const int t = i / (G.pad / 4), n4 = i % (G.pad / 4) * 4;
+            int n = from + t < end ? a.state - n4 : 0;
+            n = n < 0 ? 0 : n > 4 ? 4 : n;
+            const int64_t at = (from + t) * stride + group * a.state + n4;
+            T* to = couplings + (buffer * 2 * kRow + t) * G.pitch + n4;
+            copy4(to, (const T*)a.B + at, a.vec_states, n);
+            copy4(to + kRow * G.pitch, (const T*)a.C + at, a.vec_states, n);
+        }
+        copies_commit();
+    };
+    if (begin < end) copy_tile(begin, 0);
+    int buffer = 0;
+    for (int64_t from = begin; from < end; from += kRow, buffer ^= 1) {
+        copies_wait();
+        // (each thread reads back what it has fetched itself)
+        for (int t = st; t < kRow; t += rows) {
+            const int n = from + t < end ? left : 0, to = t * G.channels + c4, row = place(c4, t);
+            const Raw4<T> rx = raw4(raw + to), rd = raw4(raw + cells + to);
+            Raw4<T> rz;
+            if (GATE) rz = raw4(raw + 2 * cells + to);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float d = load1(&rd.e[i]) + bias[i];
+                if (a.softplus) d = softplus_(d);
+                sX[row + i * kRow] = load1(&rx.e[i]);
+                sD[row + i * kRow] = i < n ? d : 0.0f;
+                if (GATE) {
+                    const float z = load1(&rz.e[i]);
+                    sZ[row + i * kRow] = z * sigmoid_(z);
+                }
+            }
+        }
+        if (from + kRow < end) copy_tile(from + kRow, buffer ^ 1);
+        __syncthreads();
+        for (int q = 0; q < G.slices; ++q) {
+            const int first = q * kWide + sub * 4;
+            // (FULL: all of a slice's states exist; else those beyond the last one stay zero whatever the input is)
+            pair_t B[K][2], C[K][2];
+#pragma unroll
+            for (int i = 0; i < K; ++i) {
+                const T* from_row = couplings + (buffer * 2 * kRow + tl * K + i) * G.pitch + first;
+                const Raw4<T> b = raw4(from_row), c = raw4(from_row + kRow * G.pitch);
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    B[i][p] = pack(load1(&b.e[2 * p]), load1(&b.e[2 * p + 1]));
+                    C[i][p] = pack(load1(&c.e[2 * p]), load1(&c.e[2 * p + 1]));
+                }
+            }
+            for (int cc = 0; cc < a.per_warp; ++cc) {
+                const int c = warp * a.per_warp + cc;
+                if (c >= count) break;
+                float* kept = smem + G.carry + c * G.pad + first;
+                const float* rates = smem + G.rate + c * G.pad + first;
+                pair_t entry[2], rate[2], w[K][2], h[2], span[2];
+                entry[0] = reinterpret_cast<const pair_t*>(kept)[0];
+                entry[1] = reinterpret_cast<const pair_t*>(kept)[1];
+                rate[0] = reinterpret_cast<const pair_t*>(rates)[0];
+                rate[1] = reinterpret_cast<const pair_t*>(rates)[1];
+                float u[K];
+                {
+                    float x[K], d[K];
+#pragma unroll
+                    for (int i = 0; i < K; i += kPart) {
+                        load_steps<kPart>(sX + place(c, tl * K + i), reinterpret_cast<float(&)[kPart]>(x[i]));
+                        load_steps<kPart>(sD + place(c, tl * K + i), reinterpret_cast<float(&)[kPart]>(d[i]));
+                    }
+                    // from a zero state, and the decay over this lane's tokens
+#pragma unroll
+                    for (int i = 0; i < K; ++i) {
+                        const pair_t step = pack(d[i], d[i]);
+                        u[i] = d[i] * x[i];
+                        const pair_t uu = pack(u[i], u[i]);
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            w[i][p] = decay2(step, rate[p]);
+                            const pair_t b = mul2(uu, B[i][p]);
+                            h[p] = i == 0 ? b : mad2(w[i][p], h[p], b);
+                            span[p] = i == 0 ? w[i][p] : mul2(span[p], w[i][p]);
+                        }
+                    }
+                }
+                // over the token groups.  The first one takes in the carried state; its decay then counts as zero,
+                // so that a group that has seen everything before it adds nothing more (a shuffle from beyond the
+                // edge returns the lane's own value).
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    h[p] = mad2(span[p], tl == 0 ? entry[p] : 0, h[p]);
+                    span[p] = tl == 0 ? 0 : span[p];
+                }
+#pragma unroll
+                for (int off = 1; off < TL; off *= 2)
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        h[p] = mad2(span[p], shift_up(h[p], off * LN), h[p]);
+                        if (2 * off < TL) span[p] = mul2(span[p], shift_up(span[p], off * LN));
+                    }
+                __syncwarp();
+                if (tl == TL - 1) {
+                    reinterpret_cast<pair_t*>(kept)[0] = FULL ? h[0] : keep_states(h[0], a.state - first);
+                    reinterpret_cast<pair_t*>(kept)[1] = FULL ? h[1] : keep_states(h[1], a.state - first - 2);
+                }
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    h[p] = shift_up(h[p], LN);
+                    h[p] = tl == 0 ? entry[p] : h[p];
+                }
+                if (a.carries && tl * K % PD_SCAN_CHUNK == 0 && from + tl * K < end) {
+                    float v[4];
+                    unpack(h[0], v[0], v[1]);
+                    unpack(h[1], v[2], v[3]);
+                    float* to = a.carries + ((chunk0 + (from - begin + tl * K) / PD_SCAN_CHUNK) * a.channels + c0 + c) * a.state;
+                    if (FULL && a.vec_params) {
+                        *reinterpret_cast<float4*>(to + first) = make_float4(v[0], v[1], v[2], v[3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) if (first + i < a.state) to[first + i] = v[i];
+                    }
+                }
+                // from the true state
+                float y[K];
+#pragma unroll
+                for (int i = 0; i < K; ++i) {
+                    const pair_t uu = pack(u[i], u[i]);
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) h[p] = mad2(w[i][p], h[p], mul2(uu, B[i][p]));
+                    const pair_t low = FULL ? h[0] : keep_states(h[0], a.state - first);
+                    const pair_t high = FULL ? h[1] : keep_states(h[1], a.state - first - 2);
+                    y[i] = halves(mad2(C[i][1], high, mul2(C[i][0], low)));
+                }
+                // a token's sum over its lanes; each lane finishes two tokens
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float part[LN];
+#pragma unroll
+                    for (int j = 0; j < LN; ++j) part[j] = y[i * LN + j];
+                    float v = sum_to_lane<LN>(part, sub);
+                    const int at = place(c, tl * K + i * LN + sub);
+                    if (G.slices > 1) {
+                        if (q > 0) v += smem[G.y + at];
+                        smem[G.y + at] = v;
+                    }
+                    if (q == G.slices - 1) {
+                        __syncwarp();     // the tile's inputs of this channel give way to its outputs
+                        v += smem[G.skip + c] * sX[at];
+                        sX[at] = GATE ? v * sZ[at] : v;
+                    }
+                }
+            }
+        }
+        __syncthreads();
+        for (int t = st; t < kRow; t += rows) {
+            const int n = from + t < end ? left : 0, row = place(c4, t);
+            float v[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] = sX[row + i * kRow];
+            put4((T*)a.y + (from + t) * a.channels + c0 + c4, a.vec, n, v);
+        }
+        __syncthreads();
+    }
+    if (a.final_state) {
+        __syncthreads();
+        for (int i = tid; i < count * G.pad; i += kScanThreads)
+            if (i % G.pad < a.state) a.final_state[(s * a.channels + c0 + i / G.pad) * a.state + i % G.pad] = smem[G.carry + i];
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Gradients, chunk by chunk of 32 tokens from the end.  A block owns four warps' channels of one group and one
+// sequence.  A warp takes its channels one after another, each over the whole chunk at once: a lane holds K
+// tokens' four states, LN lanes the states of a token group, 32 / LN lanes the token groups.  Forward from the
+// state kept at the chunk's start, then backwards,
+//     g_t = C_t dy_t + a_{t+1} g_{t+1},   dA += d a h_{t-1} g,  ddelta: A a h_{t-1} g + x B g,  dB += u g,  dC += dy h,
+// both as a pass from zero, a scan over the token groups by shuffles and a second pass from the true value.
+// Tokens stand across lanes, so the sums of dB and dC over channels, shared by the whole group, stay in registers
+// while a warp goes through its channels; only their sum over the four warps passes through shared memory.
+// LN == K, and after the sums over a token's LN lanes each lane finishes one token.
+// ---------------------------------------------------------------------------
+constexpr int kGradWarps = 4, kGradThreads = 32 * kGradWarps;
 
 struct GradShape {
     int channels, pad, slices;    // channels per block, states rounded up, slices of 4 LN states
@@ -1122,8 +1128,10 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                 for (int p = 0; p < 2; ++p) {
                     in[p] = h[K][p];
                     down[p] = up[p];
-                    if (tl == 0) { in[p] = mad2(up[p], entry[p], in[p]); up[p] = 0; }
-                    if (tl == TL - 1) { e[p] = mad2(down[p], leave[p], e[p]); down[p] = 0; }
+                    in[p] = mad2(up[p], tl == 0 ? entry[p] : 0, in[p]);
+                    e[p] = mad2(down[p], tl == TL - 1 ? leave[p] : 0, e[p]);
+                    up[p] = tl == 0 ? 0 : up[p];
+                    down[p] = tl == TL - 1 ? 0 : down[p];
                 }
 #pragma unroll
                 for (int off = 1; off < TL; off *= 2)
@@ -1146,8 +1154,8 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                 for (int p = 0; p < 2; ++p) {
                     in[p] = shift_up(in[p], LN);
                     e[p] = shift_down(e[p], LN);
-                    if (tl == 0) in[p] = entry[p];
-                    if (tl == TL - 1) e[p] = leave[p];
+                    in[p] = tl == 0 ? entry[p] : in[p];
+                    e[p] = tl == TL - 1 ? leave[p] : e[p];
                     h[0][p] = in[p];
 #pragma unroll
                     for (int i = 0; i < K; ++i) {
@@ -1376,31 +1384,24 @@ int64_t scan_tiles(const PdScanArgs& a) {
     const int64_t per = a.channels / a.groups, ch = 32 / pd_scan_lanes(a.state);
     return (per + ch - 1) / ch;
 }
-// f(lanes per channel, slices of states) for the prompt kernels: sixteen states at a time
-template <class F>
-cudaError_t by_slices(int state, F f) {
-    if (state <= 4) return f(Int<1>(), Int<1>());
-    if (state <= 8) return f(Int<2>(), Int<1>());
-    if (state <= 16) return f(Int<4>(), Int<1>());
-    if (state <= 32) return f(Int<4>(), Int<2>());
-    return f(Int<4>(), Int<4>());
-}
 cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
     return by_type(a.type, [&](auto e) {
         using T = decltype(e);
-        return by_slices(a.state, [&](auto ln, auto ns) {
-            constexpr int LN = decltype(ln)::value, NS = decltype(ns)::value;
-            using G = ScanShape<LN, NS>;
-            const int64_t per = a.channels / a.groups, tiles = (per + G::kChannels - 1) / G::kChannels * a.groups;
+        auto run = [&](auto ln) -> cudaError_t {
+            constexpr int LN = decltype(ln)::value;
+            const ScanShape G(LN, a.state, a.per_warp, sizeof(T));
+            const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels * a.groups;
             const int64_t blocks = tiles * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
             if (blocks == 0) return cudaSuccess;
-            auto kernel = a.state == G::kPad ? pd_selective_scan_kernel<T, LN, NS, true> : pd_selective_scan_kernel<T, LN, NS, false>;
-            constexpr int bytes = G::kFloats * 4;
-            cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+            const bool full = a.state % (4 * LN) == 0;
+            auto kernel = a.z ? (full ? pd_selective_scan_kernel<T, LN, true, true> : pd_selective_scan_kernel<T, LN, true, false>)
+                              : (full ? pd_selective_scan_kernel<T, LN, false, true> : pd_selective_scan_kernel<T, LN, false, false>);
+            cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.bytes);
             if (err != cudaSuccess) return err;
-            kernel<<<(unsigned)blocks, G::kThreads, bytes, st>>>(a);
+            kernel<<<(unsigned)blocks, kScanThreads, G.bytes, st>>>(a);
             return cudaGetLastError();
-        });
+        };
+        return a.state <= 4 ? run(Int<1>()) : a.state <= 8 ? run(Int<2>()) : run(Int<4>());
     });
 }
 cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {

@@ -41,7 +41,7 @@ struct PdScanArgs {
     int vec;                  // tokens can be read four channels at a time
     int vec_states;           // B and C four states at a time
     int vec_params;           // A and the states four at a time
-    int per_warp;             // gradient: channels a warp takes one after another
+    int per_warp;             // channels a warp takes one after another
     int64_t channels;
     const void *x, *delta, *B, *C, *z, *dy;
     const float *A, *bias, *skip, *initial, *carries_in, *dfinal;

@@ -78,23 +78,24 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d) {
     const int64_t per = d.channels / p->groups, ch = 32 / pd_scan_lanes((int)p->state);
     return (per + ch - 1) / ch * p->groups;
 }
-// Channels a warp of the gradient kernel takes one after another (a block is four warps, three blocks an SM).
-// More of them share one sum over the block's warps and one partial sum of dB and dC in memory, worth about
-// one channel's work per chunk; fewer give more blocks.  The smallest product of waves and work per wave wins.
-int scan_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
-    const int64_t per = d.channels / p->groups;
+// Channels a warp takes one after another (a block is four warps; four blocks an SM for prompts, three for
+// gradients).  More of them share the fetched B and C and, in the gradient, one sum over the block's warps and one
+// partial sum of dB and dC in memory, worth about one channel's work per tile; fewer give more blocks.  The
+// smallest product of waves and work per wave wins.
+int scan_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms, bool grad) {
+    const int64_t per = d.channels / p->groups, slots = (int64_t)sms * 3;
     const int most = p->state > 16 ? 4 : 8;    // (slices of sixteen states need shared memory for as many sums)
     int best = 1;
     int64_t least = INT64_MAX;
     for (int n = most; n >= 1; --n) {
         const int64_t blocks = (per + 4 * n - 1) / (4 * n) * p->groups * (d.seqs > 0 ? d.seqs : 1);
-        const int64_t cost = (blocks + 3 * sms - 1) / (3 * sms) * (n + 1);
+        const int64_t cost = (blocks + slots - 1) / slots * (n + 1);
         if (cost < least) { least = cost; best = n; }
     }
     return best;
 }
 int64_t scan_partial_bc(const pd_selective_scan_params* p, const Dims& d, int sms) {
-    const int64_t per = d.channels / p->groups, ch = 4 * scan_per_warp(p, d, sms);
+    const int64_t per = d.channels / p->groups, ch = 4 * scan_per_warp(p, d, sms, true);
     return align256((per + ch - 1) / ch * p->groups * d.rows * 2 * pd_scan_pad((int)p->state) * 4);
 }
 
@@ -187,11 +188,10 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
     }
     // one block per tile of channels and sequence
     const int64_t per = d.channels / p->groups;
-    const int per_warp = scan_per_warp(p, d, sms);
-    const int64_t ch = grad ? 4 * per_warp : 32 / pd_scan_slice_lanes((int)p->state);
+    const int per_warp = scan_per_warp(p, d, sms, grad);
+    const int64_t ch = 4 * per_warp;
     plan->grid = (per + ch - 1) / ch * p->groups * (d.seqs + free_rows);
-    plan->block = grad ? 128 : 256;
-    plan->items = grad ? per_warp : 16;
+    plan->items = per_warp;
     if (grad) {
         in.push_back(carries);
         if (p->final) in.push_back(edge);
@@ -312,7 +312,6 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
             if (p->skip) a.dskip = (float*)out[o++];
             if (p->gate) a.dz = out[o++];
             if (p->initial) a.dinitial = (float*)out[o++];
-            a.per_warp = (int)plan.items;
             a.partial_bc = (float*)scratch;
             a.partial_params = (float*)((char*)scratch + plan.params_offset);
         } else {
@@ -327,7 +326,8 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         const void* tokens[] = {a.x, a.delta, a.z, a.dy, a.y, a.dx, a.ddelta, a.dz};
         for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % four) a.vec = 0;
         a.vec_states = a.state % 4 == 0 && reinterpret_cast<uintptr_t>(a.B) % four == 0 && reinterpret_cast<uintptr_t>(a.C) % four == 0;
-        a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial);
+        a.per_warp = (int)plan.items;
+        a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries);
         e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
     }
     if (e != cudaSuccess) {
