@@ -290,6 +290,9 @@ def _arrays_plain(grid, block):
     return garr, barr
 
 
+grid_and_block = _arrays
+
+
 def _buffers(ptrs_and_bytes):
     n = len(ptrs_and_bytes)
     ptrs = (ctypes.c_void_p * max(n, 1))(*[p for p, _ in ptrs_and_bytes])
@@ -319,6 +322,17 @@ def launch(family: int, params: ctypes.Structure, math_mode: int, grid, block, i
     ws_ptr, ws_bytes = workspace if workspace else (None, 0)
     rc = lib.pd_launch(family, ctypes.addressof(params), ctypes.sizeof(params), math_mode, garr, barr, n_in, in_ptrs,
                        in_sizes, n_out, out_ptrs, out_sizes, ws_ptr, ws_bytes, stream or None, err, _ERR_CAP)
+    if rc:
+        _raise(rc, err.value)
+
+
+def launch_again(call, math_mode: int, inputs, outputs, workspace, stream: int) -> None:
+    """pd_launch with the sizes of a call made before (`ffi._Repeat`) on other tensors."""
+    err = _err_buffer()
+    rc = _lib.pd_launch(call.family_id, call.params, call.params_bytes, math_mode, call.grid, call.block,
+                        call.n_in, call.pointers_in(*[t.data_ptr() for t in inputs]), call.in_sizes,
+                        call.n_out, call.pointers_out(*[t.data_ptr() for t in outputs]), call.out_sizes,
+                        None if workspace is None else workspace.data_ptr(), call.scratch, stream or None, err, _ERR_CAP)
     if rc:
         _raise(rc, err.value)
 

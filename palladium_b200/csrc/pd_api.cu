@@ -108,7 +108,20 @@ inline int64_t knob(Knob k) {
 // ---------------------------------------------------------------------------
 struct DeviceFacts { int device = -1; int sms = 148; bool present = false; };
 DeviceFacts device_facts() {
+    static std::atomic<int> known[64];     // multiprocessors of a device once asked, 0 before
     DeviceFacts f;
+    int current = -1;
+    if (cudaGetDevice(&current) == cudaSuccess && current >= 0 && current < 64) {
+        const int sms = known[current].load(std::memory_order_relaxed);
+        if (sms > 0) {
+            f.device = current;
+            f.sms = sms;
+            f.present = true;
+            return f;
+        }
+    } else {
+        cudaGetLastError();
+    }
     int count = 0;
     if (cudaGetDeviceCount(&count) != cudaSuccess || count == 0) {
         cudaGetLastError();
@@ -116,8 +129,10 @@ DeviceFacts device_facts() {
     }
     if (cudaGetDevice(&f.device) != cudaSuccess) { cudaGetLastError(); return f; }
     int sms = 0;
-    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, f.device) == cudaSuccess && sms > 0)
+    if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, f.device) == cudaSuccess && sms > 0) {
         f.sms = sms;
+        if (f.device >= 0 && f.device < 64) known[f.device].store(sms, std::memory_order_relaxed);
+    }
     f.present = true;
     return f;
 }

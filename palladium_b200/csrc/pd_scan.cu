@@ -1314,6 +1314,11 @@ __global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdSca
 // ---------------------------------------------------------------------------
 int64_t blocks_for(int64_t threads, int block) { return (threads + block - 1) / block; }
 
+template <class K>
+cudaError_t allow_smem(K kernel, int bytes) {     // up to 48 KB need no leave
+    return bytes <= 48 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 template <class F>
 cudaError_t by_type(int type, F f) {
     if (type == PD_TYPE_F32) return f(float());
@@ -1396,7 +1401,7 @@ cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
             const bool full = a.state % (4 * LN) == 0;
             auto kernel = a.z ? (full ? pd_selective_scan_kernel<T, LN, true, true> : pd_selective_scan_kernel<T, LN, true, false>)
                               : (full ? pd_selective_scan_kernel<T, LN, false, true> : pd_selective_scan_kernel<T, LN, false, false>);
-            cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.bytes);
+            cudaError_t err = allow_smem(kernel, G.bytes);
             if (err != cudaSuccess) return err;
             kernel<<<(unsigned)blocks, kScanThreads, G.bytes, st>>>(a);
             return cudaGetLastError();
@@ -1425,7 +1430,7 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
             const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
             if (blocks > 0) {
                 auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true> : pd_selective_scan_grad_kernel<T, LN, false>;
-                cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, G.bytes);
+                cudaError_t err = allow_smem(kernel, G.bytes);
                 if (err != cudaSuccess) return err;
                 kernel<<<(unsigned)blocks, kGradThreads, G.bytes, st>>>(a);
                 err = cudaGetLastError();

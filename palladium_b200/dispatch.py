@@ -196,7 +196,7 @@ class BoundKernel:
 
         return call
 
-    def _scratch_bytes(self) -> int:
+    def scratch_bytes(self) -> int:
         """Scratch of a state-space call; 0 for the families that use the library's pool."""
         if self._scratch is None:
             spec = self.spec
@@ -241,7 +241,7 @@ class BoundKernel:
             # The kernel writes `out_bytes[i]` bytes from each pointer whatever the tensor's own
             # size or strides: a short, strided, host or other-device tensor must stop here.
             check_device_tensors("output", outputs, out_bytes, current)
-        if workspace is None and self._scratch_bytes():
+        if workspace is None and self.scratch_bytes():
             with torch.cuda.stream(stream if stream is not None else torch.cuda.current_stream()):
                 workspace = torch.empty(self._scratch, dtype=torch.uint8, device="cuda")
         _native.launch(

@@ -21,6 +21,7 @@ here, chosen by the argument type:
 
 from __future__ import annotations
 
+import ctypes
 import importlib.util
 import threading
 from typing import Any
@@ -86,6 +87,42 @@ def _pinned_empty(shape, dtype) -> np.ndarray:
     return np.empty(shape, dtype)
 
 
+class _Repeat:
+    """What a call on device tensors needs again and again for one signature, as the native call takes it: a
+    repeated call compares its operands with the last one's and goes straight to the library.  (Checked operand
+    by operand the long way, a call of nine operands spent 30 us here, ten times its kernel.)"""
+
+    __slots__ = ("torch", "family_id", "spec", "shapes", "dtypes", "outputs", "n_in", "n_out", "in_sizes", "out_sizes", "pointers_in",
+                 "pointers_out", "grid", "block", "params", "params_bytes", "scratch")
+
+    def __init__(self, torch, spec: KernelSpec, bound: BoundKernel, args) -> None:
+        _, torch_dtype = _torch_dtype_tables(torch)
+        self.torch, self.family_id = torch, spec.family.family_id
+        self.spec = spec              # (holds the parameter block whose address is used)
+        self.shapes = [a.shape for a in args]
+        self.dtypes = [a.dtype for a in args]
+        self.outputs = [(info.array_shape, torch_dtype[dtype_name(info.dtype)]) for info in spec.outputs]
+        self.n_in, self.n_out = len(args), len(spec.outputs)
+        sizes = [int(np.prod(i.array_shape)) * i.dtype.itemsize for i in (*spec.inputs, *spec.outputs)]
+        self.in_sizes = (ctypes.c_size_t * max(self.n_in, 1))(*sizes[:self.n_in])
+        self.out_sizes = (ctypes.c_size_t * self.n_out)(*sizes[self.n_in:])
+        self.pointers_in = ctypes.c_void_p * max(self.n_in, 1)
+        self.pointers_out = ctypes.c_void_p * self.n_out
+        self.grid, self.block = _native.grid_and_block(spec.grid, bound.threadgroup)
+        self.params, self.params_bytes = ctypes.addressof(spec.params), ctypes.sizeof(spec.params)
+        self.scratch = bound.scratch_bytes()
+
+    def takes(self, args, device: int) -> bool:
+        """Whether these operands have the recorded shapes and types, are contiguous and on the current device."""
+        if len(args) != self.n_in:
+            return False
+        for a, shape, dtype in zip(args, self.shapes, self.dtypes):
+            if (getattr(a, "dtype", None) is not dtype or a.shape != shape or a.get_device() != device
+                    or not a.is_contiguous()):
+                return False
+        return True
+
+
 class FfiCallable:
     """A kernel family callable on device tensors (stream-ordered), host
     arrays (blocking), or JAX values (through jax.ffi when available).
@@ -120,6 +157,7 @@ class FfiCallable:
         self.interpret = interpret_callable(kernel, self._pallas_kwargs)
         self._cache: dict[tuple, tuple[KernelSpec, BoundKernel]] = {}
         self._lock = threading.Lock()
+        self._repeat: _Repeat | None = None
 
     def explain(self, *args) -> KernelDiagnostics:
         return explain_spec(trace(self._family, self._pallas_kwargs, *args), self._threadgroup, self._math_mode)
@@ -138,6 +176,11 @@ class FfiCallable:
         return entry
 
     def __call__(self, *args):
+        repeat = self._repeat
+        if repeat is not None:
+            outs = self._call_again(repeat, args)
+            if outs is not None:
+                return outs
         if args and all(_is_torch_tensor(a) for a in args):
             return self._call_torch(args)
         if args and any(_is_jax_value(a) for a in args):
@@ -178,6 +221,18 @@ class FfiCallable:
         return stacked[0] if single else tuple(stacked)
 
     # ---- torch CUDA tensors: stream-ordered, no synchronisation ----------------
+    def _call_again(self, repeat: _Repeat, args):
+        """The outputs of a repeated call, or None where these are other operands than the last ones'."""
+        torch = repeat.torch
+        device = torch._C._cuda_getDevice()
+        if not repeat.takes(args, device):
+            return None
+        empty, where = torch.empty, args[0].device
+        outs = [empty(shape, dtype=dtype, device=where) for shape, dtype in repeat.outputs]
+        workspace = empty(repeat.scratch, dtype=torch.uint8, device=where) if repeat.scratch else None
+        _native.launch_again(repeat, self._math_mode, args, outs, workspace, torch._C._cuda_getCurrentRawStream(device))
+        return outs[0] if repeat.n_out == 1 else tuple(outs)
+
     def _call_torch(self, args, out=None):
         import torch
 
@@ -191,6 +246,8 @@ class FfiCallable:
             outs = [torch.empty(info.array_shape, dtype=torch_dtype[dtype_name(info.dtype)], device=device)
                     for info in spec.outputs]
         bound.launch_device(list(args), outs)
+        if out is None and args and hasattr(torch._C, "_cuda_getCurrentRawStream"):
+            self._repeat = _Repeat(torch, spec, bound, args)      # everything was checked on the way
         return outs[0] if len(outs) == 1 else tuple(outs)
 
     def on_device(self, *args, out=None):
