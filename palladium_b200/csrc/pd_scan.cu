@@ -41,29 +41,31 @@ __device__ __forceinline__ void store1(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store1(__half* p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void store1(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 
-// V consecutive elements; V > 1 means one 16-byte access
+// V consecutive elements, as stored; V > 1 means one aligned access of 8 or 16 bytes
+template <class T, int V> struct Vec { T e[V]; };
 template <int V, class T>
-__device__ __forceinline__ void load(const T* p, float (&v)[V]) {
-    if constexpr (V == 1) {
-        v[0] = load1(p);
-    } else {
-        static_assert(V * sizeof(T) == 16, "a vector is 16 bytes");
-        union { uint4 raw; T e[V]; } u;
-        u.raw = *reinterpret_cast<const uint4*>(p);
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = load1(&u.e[i]);
-    }
+__device__ __forceinline__ Vec<T, V> fetch(const T* p) {
+    Vec<T, V> r;
+    if constexpr (V == 1) r.e[0] = p[0];
+    else if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(r.e) = *reinterpret_cast<const uint4*>(p);
+    else *reinterpret_cast<uint2*>(r.e) = *reinterpret_cast<const uint2*>(p);
+    return r;
 }
 template <int V, class T>
-__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
-    if constexpr (V == 1) {
-        store1(p, v[0]);
-    } else {
-        union { uint4 raw; T e[V]; } u;
+__device__ __forceinline__ void widen(const Vec<T, V>& r, float (&v)[V]) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) store1(&u.e[i], v[i]);
-        *reinterpret_cast<uint4*>(p) = u.raw;
-    }
+    for (int i = 0; i < V; ++i) v[i] = load1(&r.e[i]);
+}
+template <int V, class T>
+__device__ __forceinline__ void load(const T* p, float (&v)[V]) { widen(fetch<V>(p), v); }
+template <int V, class T>
+__device__ __forceinline__ void store(T* p, const float (&v)[V]) {
+    Vec<T, V> r;
+#pragma unroll
+    for (int i = 0; i < V; ++i) store1(&r.e[i], v[i]);
+    if constexpr (V == 1) p[0] = r.e[0];
+    else if constexpr (V * sizeof(T) == 16) *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(r.e);
+    else *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(r.e);
 }
 
 // ---------------------------------------------------------------------------
@@ -180,7 +182,7 @@ __device__ __forceinline__ void conv_window(const PdConvArgs& a, const T* x, int
     }
 }
 
-template <class T, int W, int V>
+template <class T, int W, int V, bool SILU>
 __global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
     const int64_t lanes = (a.channels + V - 1) / V;
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -226,22 +228,31 @@ __global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
         }
         conv_window<T, W, V>(a, x, s, begin, row, c, win);
         const int64_t upto = end < stop ? end : stop;
-        for (; row < upto; ++row) {
+        auto step = [&](int64_t r, const Vec<T, V>& got) {
             float now[V], out[V];
-            load<V>(x + row * a.channels + c, now);
+            widen(got, now);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
                 float acc = b[v];
 #pragma unroll
                 for (int i = 0; i < W - 1; ++i) acc += w[i][v] * win[i][v];
                 acc += w[W - 1][v] * now[v];
-                out[v] = a.silu ? acc * sigmoid_(acc) : acc;
+                out[v] = SILU ? acc * sigmoid_(acc) : acc;
 #pragma unroll
                 for (int i = 0; i + 1 < W - 1; ++i) win[i][v] = win[i + 1][v];
                 win[W - 2][v] = now[v];
             }
-            store<V>((T*)a.y + row * a.channels + c, out);
+            store<V>((T*)a.y + r * a.channels + c, out);
+        };
+        // four rows in flight per thread
+        for (; row + 4 <= upto; row += 4) {
+            Vec<T, V> got[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) got[i] = fetch<V>(x + (row + i) * a.channels + c);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) step(row + i, got[i]);
         }
+        for (; row < upto; ++row) step(row, fetch<V>(x + row * a.channels + c));
         if (row == end && a.final_state)
 #pragma unroll
             for (int i = 0; i < W - 1; ++i)
@@ -277,7 +288,7 @@ __global__ void __launch_bounds__(256) pd_causal_conv_step_kernel(PdConvArgs a) 
 //   dx_t = sum_j w[W-1-j] g_{t+j},   dw[W-1-j] = sum_t x_{t-j} g_t,   dbias = sum_t g_t
 // A thread walks its run and W - 1 rows beyond it, and keeps the W gradients of dx still open; sums of
 // dw and dbias stay in registers, then go to one partial per block, which a second launch adds up in order.
-template <class T, int W, int V>
+template <class T, int W, int V, bool SILU>
 __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) {
     const int64_t lanes = (a.channels + V - 1) / V;
     // blockDim.x threads across channels, blockDim.y across runs; blockIdx.x channel blocks, blockIdx.y row blocks
@@ -338,13 +349,13 @@ __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) 
             const int64_t mine = end < stop ? end : stop;                        // rows whose sums belong here
             const int64_t upto = mine + (W - 1) < end ? mine + (W - 1) : end;    // rows whose g they need
             const int64_t from = row;
-            for (; row < upto; ++row) {
+            auto step = [&](int64_t r, const Vec<T, V>& got_x, const Vec<T, V>& got_g) {
                 float now[V], g[V];
-                load<V>(x + row * a.channels + c, now);
-                load<V>(dy + row * a.channels + c, g);
+                widen(got_x, now);
+                widen(got_g, g);
 #pragma unroll
                 for (int v = 0; v < V; ++v) {
-                    if (a.silu) {
+                    if (SILU) {
                         float pre = b[v];
 #pragma unroll
                         for (int i = 0; i < W - 1; ++i) pre += w[i][v] * win[i][v];
@@ -355,24 +366,34 @@ __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) 
 #pragma unroll
                     for (int j = W - 1; j > 0; --j) open[j][v] = open[j - 1][v] + w[W - 1 - j][v] * g[v];
                     open[0][v] = w[W - 1][v] * g[v];
-                    if (row < mine) {
-                        db[v] += g[v];
+                    const float h = r < mine ? g[v] : 0.0f;
+                    db[v] += h;
 #pragma unroll
-                        for (int i = 0; i < W - 1; ++i) dw[i][v] += win[i][v] * g[v];
-                        dw[W - 1][v] += now[v] * g[v];
-                    }
+                    for (int i = 0; i < W - 1; ++i) dw[i][v] += win[i][v] * h;
+                    dw[W - 1][v] += now[v] * h;
 #pragma unroll
                     for (int i = 0; i + 1 < W - 1; ++i) win[i][v] = win[i + 1][v];
                     win[W - 2][v] = now[v];
                 }
                 // the input W - 1 rows back is complete
-                const int64_t done = row - (W - 1);
+                const int64_t done = r - (W - 1);
                 if (done >= from) store<V>((T*)a.dx + done * a.channels + c, open[W - 1]);
                 else if (done < begin && from == begin && a.dinitial) {
                     // (a carried-in input that is carried out again is still open at the end, below)
                     store<V>((T*)a.dinitial + (s * (W - 1) + (done - begin) + (W - 1)) * a.channels + c, open[W - 1]);
                 }
+            };
+            for (; row + 4 <= upto; row += 4) {
+                Vec<T, V> got_x[4], got_g[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    got_x[i] = fetch<V>(x + (row + i) * a.channels + c);
+                    got_g[i] = fetch<V>(dy + (row + i) * a.channels + c);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) step(row + i, got_x[i], got_g[i]);
             }
+            for (; row < upto; ++row) step(row, fetch<V>(x + row * a.channels + c), fetch<V>(dy + row * a.channels + c));
             if (row == end) {
                 // the sequence ends here: the inputs still open are complete, and were carried out
 #pragma unroll
@@ -1357,7 +1378,9 @@ cudaError_t launch_conv(const PdConvArgs& a, cudaStream_t st) {
         const int64_t lanes = (a.channels + v.value - 1) / v.value;
         const int64_t jobs = (a.tok.rows + a.run - 1) / a.run + (a.final_state ? a.tok.seqs : 0);
         if (lanes * jobs == 0) return cudaSuccess;
-        pd_causal_conv_kernel<T, decltype(w)::value, decltype(v)::value><<<(unsigned)blocks_for(lanes * jobs, 256), 256, 0, st>>>(a);
+        constexpr int W = decltype(w)::value, V = decltype(v)::value;
+        auto kernel = a.silu ? pd_causal_conv_kernel<T, W, V, true> : pd_causal_conv_kernel<T, W, V, false>;
+        kernel<<<(unsigned)blocks_for(lanes * jobs, 256), 256, 0, st>>>(a);
         return cudaGetLastError();
     });
 }
@@ -1371,17 +1394,23 @@ cudaError_t launch_conv_step(const PdConvArgs& a, cudaStream_t st) {
     });
 }
 cudaError_t launch_conv_grad(const PdConvArgs& a, cudaStream_t st) {
-    return by_conv(a, [&](auto e, auto w, auto v) {
+    return by_type(a.type, [&](auto e) {
         using T = decltype(e);
-        constexpr int W = decltype(w)::value, V = decltype(v)::value;
-        const int64_t lanes = (a.channels + V - 1) / V;
-        if (a.channels == 0) return cudaSuccess;
-        const dim3 block(32, 8), grid((unsigned)blocks_for(lanes, 32), (unsigned)a.row_blocks);
-        pd_causal_conv_grad_kernel<T, W, V><<<grid, block, 256 * V * sizeof(float), st>>>(a);
-        cudaError_t err = cudaGetLastError();
-        if (err != cudaSuccess) return err;
-        pd_causal_conv_sum_kernel<W><<<(unsigned)blocks_for(a.channels * (W + 1), 128), 128, 0, st>>>(a);
-        return cudaGetLastError();
+        return by_width(a.width, [&](auto w) {
+            constexpr int W = decltype(w)::value;
+            auto run = [&](auto v) -> cudaError_t {
+                constexpr int V = decltype(v)::value;
+                const int64_t lanes = (a.channels + V - 1) / V;
+                const dim3 block(32, 8), grid((unsigned)blocks_for(lanes, 32), (unsigned)a.row_blocks);
+                auto kernel = a.silu ? pd_causal_conv_grad_kernel<T, W, V, true> : pd_causal_conv_grad_kernel<T, W, V, false>;
+                kernel<<<grid, block, 256 * V * sizeof(float), st>>>(a);
+                cudaError_t err = cudaGetLastError();
+                if (err != cudaSuccess) return err;
+                pd_causal_conv_sum_kernel<W><<<(unsigned)blocks_for(a.channels * (W + 1), 128), 128, 0, st>>>(a);
+                return cudaGetLastError();
+            };
+            return a.vec > 1 ? run(Int<4>()) : run(Int<1>());
+        });
     });
 }
 

@@ -31,7 +31,7 @@ struct PdConvArgs {
     float *dweight, *dbias;
     float* partial;           // gradient: (row_blocks, channels, width + 1) sums of dweight and dbias
     int64_t row_blocks;
-    int vec;                  // channels per thread (16-byte vectors), or 1
+    int vec;                  // channels per thread in one aligned access, or 1
     int run;                  // consecutive rows per thread
 };
 
@@ -74,6 +74,7 @@ const PdScanTable* pd_scan_table_fast();
 struct PdScanPlan {
     const char* kernel_name = "";
     int64_t grid = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
+    int64_t row_blocks = 0;       // gradient of the convolution: blocks along the rows
     int64_t params_offset = 0;    // gradient of the scan: where in the scratch the parameters' sums begin
     std::vector<size_t> in_bytes, out_bytes;
 };

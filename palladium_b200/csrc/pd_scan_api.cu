@@ -58,16 +58,23 @@ int conv_run(int64_t rows, int64_t lanes, int sms) {
     while (run > 4 && rows / run * lanes < (int64_t)sms * 1024) run /= 2;
     return run;
 }
-int64_t conv_row_blocks(int64_t jobs, int64_t lanes, int sms) {
-    // eight runs per block side by side; about two blocks per SM, each of which writes one partial sum
-    const int64_t columns = (lanes + 31) / 32;
-    int64_t blocks = ((int64_t)sms * 2 + columns - 1) / columns;
-    if (blocks > (jobs + 7) / 8) blocks = (jobs + 7) / 8;
-    return blocks < 1 ? 1 : blocks > 65535 ? 65535 : blocks;
-}
-int conv_vector(const pd_causal_conv_params* p, int64_t channels) {
-    const int v = (int)(16 / element(p->type));
+// Channels per thread: 16 bytes' worth, in the gradient four, whose sums of dweight take registers too.
+int conv_vector(const pd_causal_conv_params* p, int64_t channels, bool grad) {
+    const int v = grad ? 4 : (int)(16 / element(p->type));
     return channels % v == 0 ? v : 1;
+}
+// The gradient's blocks: 32 threads across channels, eight runs of rows side by side.  Enough rows of blocks for
+// about two blocks per SM, each of which writes one partial sum of dweight, and runs as long as that asks for.
+void conv_grad_blocks(int64_t rows, int64_t extra, int64_t lanes, int sms, int* run, int64_t* row_blocks) {
+    const int64_t columns = (lanes + 31) / 32;
+    int64_t blocks = (int64_t)sms * 2 / columns;
+    if (blocks < 1) blocks = 1;
+    int64_t n = (rows + 8 * blocks - 1) / (8 * blocks);
+    if (n < 8) n = 8;
+    *run = (int)(n > (1 << 20) ? 1 << 20 : n);
+    const int64_t jobs = (rows + *run - 1) / *run + extra;
+    blocks = (jobs + 7) / 8;
+    *row_blocks = blocks < 1 ? 1 : blocks > 65535 ? 65535 : blocks;
 }
 int64_t conv_partial(const Dims& d, int64_t width, int64_t row_blocks) { return row_blocks * d.channels * (width + 1) * 4; }
 
@@ -113,7 +120,7 @@ int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3],
     const size_t edge = (size_t)d.seqs * (size_t)(p->width - 1) * D * e, weight = D * (size_t)p->width * 4, vec = D * 4;
     const size_t offsets = ((size_t)d.seqs + 1) * 4;
     std::vector<size_t>&in = plan->in_bytes, &out = plan->out_bytes;
-    const int64_t lanes = (d.channels + conv_vector(p, d.channels) - 1) / conv_vector(p, d.channels);
+    const int64_t lanes = d.channels / conv_vector(p, d.channels, grad);
     if (step) {
         in = {tokens, edge, weight};
         if (p->bias) in.push_back(vec);
@@ -144,12 +151,12 @@ int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3],
     if (p->bias) out.push_back(vec);
     if (p->initial) out.push_back(edge);
     plan->kernel_name = "pd_causal_conv_grad_kernel";
-    // the scalar form has more columns and so fewer row blocks; size the scratch for the larger count
-    const int64_t jobs = runs + (p->initial ? d.seqs : 0);
-    const int64_t row_blocks = conv_row_blocks(jobs, lanes, sms);
-    plan->grid = (lanes + 31) / 32 * row_blocks;
+    int grad_run;
+    conv_grad_blocks(d.rows, p->initial ? d.seqs : 0, lanes, sms, &grad_run, &plan->row_blocks);
+    plan->items = grad_run;
+    plan->grid = (lanes + 31) / 32 * plan->row_blocks;
     plan->launches = 2;
-    plan->scratch_bytes = conv_partial(d, p->width, row_blocks);
+    plan->scratch_bytes = conv_partial(d, p->width, plan->row_blocks);
     return PD_OK;
 }
 
@@ -268,14 +275,11 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
             a.y = out[o++];
             if (step || p->final) a.final_state = out[o++];
         }
-        a.vec = conv_vector(p, a.channels);
+        a.vec = conv_vector(p, a.channels, grad);
         const void* tokens[] = {a.x, a.dy, a.initial, a.dfinal, a.y, a.final_state, a.dx, a.dinitial};
-        for (const void* t : tokens) if (!aligned16(t)) a.vec = 1;
-        if (grad) {
-            const int64_t lanes = a.channels / conv_vector(p, a.channels);
-            a.row_blocks = plan.grid / ((lanes + 31) / 32);
-            a.partial = (float*)scratch;
-        }
+        for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % (a.vec * element(p->type))) a.vec = 1;
+        a.row_blocks = plan.row_blocks;
+        a.partial = (float*)scratch;
         e = step ? table->conv_step(a, st) : grad ? table->conv_grad(a, st) : table->conv(a, st);
     } else {
         const pd_selective_scan_params* p = static_cast<const pd_selective_scan_params*>(params);
