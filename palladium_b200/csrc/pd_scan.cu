@@ -116,6 +116,60 @@ __device__ __forceinline__ float softplus_(float v, float& slope) {
 }
 
 // ---------------------------------------------------------------------------
+// pairs: one instruction, and one issue slot, for two float32 operations
+// ---------------------------------------------------------------------------
+typedef unsigned long long pair_t;     // two float32 in one 64-bit register
+__device__ __forceinline__ pair_t pack(float x, float y) {
+    pair_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+    return v;
+}
+__device__ __forceinline__ void unpack(pair_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
+__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
+    pair_t v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
+    pair_t v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+    return v;
+}
+// a b + c: one rounding, except under SAFE, which keeps the product's own
+__device__ __forceinline__ pair_t mad2(pair_t a, pair_t b, pair_t c) {
+#if PD_MODE == 0
+    return add2(mul2(a, b), c);
+#else
+    pair_t v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+    return v;
+#endif
+}
+
+__device__ __forceinline__ float halves(pair_t v) {
+    float x, y;
+    unpack(v, x, y);
+    return x + y;
+}
+// V elements as pairs (one element: its pair's other half is zero)
+template <int V> constexpr int kPairs = (V + 1) / 2;
+template <int V>
+__device__ __forceinline__ void pair_up(const float (&v)[V], pair_t (&p)[kPairs<V>]) {
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) p[i] = pack(v[2 * i], 2 * i + 1 < V ? v[2 * i + 1 < V ? 2 * i + 1 : 0] : 0.0f);
+}
+template <int V>
+__device__ __forceinline__ void part(const pair_t (&p)[kPairs<V>], float (&v)[V]) {
+#pragma unroll
+    for (int i = 0; i < kPairs<V>; ++i) {
+        float x, y;
+        unpack(p[i], x, y);
+        v[2 * i] = x;
+        if (2 * i + 1 < V) v[2 * i + 1 < V ? 2 * i + 1 : 0] = y;
+    }
+}
+
+// ---------------------------------------------------------------------------
 // sequences
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ int64_t clamp_row(int64_t v, int64_t rows) { return v < 0 ? 0 : (v > rows ? rows : v); }
@@ -163,11 +217,61 @@ __device__ __forceinline__ int64_t first_chunk(const PdTokens& t, int64_t s, int
 // causal convolution:  y_t = act(bias + sum_j w[W-1-j] x_{t-j})
 // One thread owns V channels and a run of consecutive rows; the last W - 1
 // inputs stay in registers, so a row is read once apart from the run's halo.
+// Bound: memory, 2 bytes in and 2 out per bf16 element; next to them stand two
+// special-function operations (30 us of the 41 that 2 x 134 MB take) and two
+// packed multiply-adds, so what matters is to keep rows in flight: four of them
+// are fetched while the four before are worked on.
 // ===========================================================================
+// the taps and the bias of V channels, as 16-byte vectors where the channels are
+template <int W, int V>
+__device__ __forceinline__ void conv_parameters(const PdConvArgs& a, int64_t c, pair_t (&w)[W][kPairs<V>], pair_t (&b)[kPairs<V>]) {
+    float flat[V * W], bias[V];
+    if constexpr (V >= 4) {
+#pragma unroll
+        for (int i = 0; i < V * W / 4; ++i) {
+            const float4 q = reinterpret_cast<const float4*>(a.weight + c * W)[i];
+            flat[4 * i] = q.x; flat[4 * i + 1] = q.y; flat[4 * i + 2] = q.z; flat[4 * i + 3] = q.w;
+        }
+#pragma unroll
+        for (int i = 0; i < V / 4; ++i) {
+            const float4 q = a.bias ? reinterpret_cast<const float4*>(a.bias + c)[i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            bias[4 * i] = q.x; bias[4 * i + 1] = q.y; bias[4 * i + 2] = q.z; bias[4 * i + 3] = q.w;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < V * W; ++i) flat[i] = a.weight[c * W + i];
+#pragma unroll
+        for (int v = 0; v < V; ++v) bias[v] = a.bias ? a.bias[c + v] : 0.0f;
+    }
+    pair_up<V>(bias, b);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {
+        float tap[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) tap[v] = flat[v * W + k];
+        pair_up<V>(tap, w[k]);
+    }
+}
+
+template <int V, class T>
+__device__ __forceinline__ void widen(const Vec<T, V>& r, pair_t (&p)[kPairs<V>]) {
+    float v[V];
+    widen(r, v);
+    pair_up<V>(v, p);
+}
+template <int V, class T>
+__device__ __forceinline__ void load(const T* at, pair_t (&p)[kPairs<V>]) { widen(fetch<V>(at), p); }
+template <int V, class T>
+__device__ __forceinline__ void store(T* at, const pair_t (&p)[kPairs<V>]) {
+    float v[V];
+    part<V>(p, v);
+    store<V>(at, v);
+}
+
+// the W - 1 inputs before `row`, oldest first
 template <class T, int W, int V>
 __device__ __forceinline__ void conv_window(const PdConvArgs& a, const T* x, int64_t s, int64_t begin, int64_t row,
-                                            int64_t c, float (&win)[W - 1][V]) {
-    // the W - 1 inputs before `row`, oldest first
+                                            int64_t c, pair_t (&win)[W - 1][kPairs<V>]) {
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) {
         const int64_t r = row - (W - 1) + i;
@@ -177,82 +281,108 @@ __device__ __forceinline__ void conv_window(const PdConvArgs& a, const T* x, int
             load<V>((const T*)a.initial + (s * (W - 1) + (W - 1) + (r - begin)) * a.channels + c, win[i]);
         } else {
 #pragma unroll
-            for (int v = 0; v < V; ++v) win[i][v] = 0.0f;
+            for (int p = 0; p < kPairs<V>; ++p) win[i][p] = 0;
         }
     }
+}
+template <int W, int P>
+__device__ __forceinline__ void slide(pair_t (&win)[W][P], const pair_t (&now)[P]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+        for (int i = 0; i + 1 < W; ++i) win[i][p] = win[i + 1][p];
+        win[W - 1][p] = now[p];
+    }
+}
+// bias + sum_j w[j] (window, now)[j]
+template <int W, int P>
+__device__ __forceinline__ void convolve(const pair_t (&w)[W][P], const pair_t (&b)[P], const pair_t (&win)[W - 1][P],
+                                         const pair_t (&now)[P], pair_t (&pre)[P]) {
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+        pre[p] = b[p];
+#pragma unroll
+        for (int i = 0; i < W - 1; ++i) pre[p] = mad2(w[i][p], win[i][p], pre[p]);
+        pre[p] = mad2(w[W - 1][p], now[p], pre[p]);
+    }
+}
+template <int V>
+__device__ __forceinline__ void silu(const pair_t (&pre)[kPairs<V>], float (&out)[V]) {
+    part<V>(pre, out);
+#pragma unroll
+    for (int v = 0; v < V; ++v) out[v] *= sigmoid_(out[v]);
 }
 
 template <class T, int W, int V, bool SILU>
 __global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
+    constexpr int P = kPairs<V>;
     const int64_t lanes = (a.channels + V - 1) / V;
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t c = id % lanes * V;
-    int64_t row = id / lanes * a.run;
+    const int64_t job = id / lanes, c = id % lanes * V;
     const int64_t runs = (a.tok.rows + a.run - 1) / a.run;
     const T* x = (const T*)a.x;
-    if (id / lanes >= runs) {
+    const float none[V] = {};
+    if (job >= runs) {
         // one more job per sequence: an empty one hands its carried-in inputs on
-        const int64_t s = id / lanes - runs;
+        const int64_t s = job - runs;
         if (!a.final_state || s >= a.tok.seqs) return;
         int64_t begin, end;
         bounds_of(a.tok, s, begin, end);
         if (begin < end) return;
-        float v[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = 0.0f;
         for (int i = 0; i < W - 1; ++i) {
             const int64_t at = (s * (W - 1) + i) * a.channels + c;
+            float v[V] = {};
             if (a.initial) load<V>((const T*)a.initial + at, v);
             store<V>((T*)a.final_state + at, v);
         }
         return;
     }
-    float w[W][V], b[V];
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-#pragma unroll
-        for (int k = 0; k < W; ++k) w[k][v] = a.weight[(c + v) * W + k];
-        b[v] = a.bias ? a.bias[c + v] : 0.0f;
-    }
+    pair_t w[W][P], b[P], win[W - 1][P];
+    conv_parameters<W, V>(a, c, w, b);
+    int64_t row = job * a.run;
     const int64_t stop = row + a.run < a.tok.rows ? row + a.run : a.tok.rows;
-    int64_t s = 0, begin = 0, end = 0;
-    float win[W - 1][V];
     while (row < stop) {
+        int64_t s, begin, end;
         if (!sequence_of(a.tok, row, s, begin, end)) {
-            float zero[V];
-#pragma unroll
-            for (int v = 0; v < V; ++v) zero[v] = 0.0f;
-            store<V>((T*)a.y + row * a.channels + c, zero);
+            store<V>((T*)a.y + row * a.channels + c, none);
             ++row;
             continue;
         }
         conv_window<T, W, V>(a, x, s, begin, row, c, win);
         const int64_t upto = end < stop ? end : stop;
-        auto step = [&](int64_t r, const Vec<T, V>& got) {
-            float now[V], out[V];
+        const T* from = x + row * a.channels + c;
+        T* to = (T*)a.y + row * a.channels + c;
+        auto step = [&](const Vec<T, V>& got) {
+            pair_t now[P], pre[P];
             widen(got, now);
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                float acc = b[v];
-#pragma unroll
-                for (int i = 0; i < W - 1; ++i) acc += w[i][v] * win[i][v];
-                acc += w[W - 1][v] * now[v];
-                out[v] = SILU ? acc * sigmoid_(acc) : acc;
-#pragma unroll
-                for (int i = 0; i + 1 < W - 1; ++i) win[i][v] = win[i + 1][v];
-                win[W - 2][v] = now[v];
+            convolve<W, P>(w, b, win, now, pre);
+            slide<W - 1, P>(win, now);
+            if (SILU) {
+                float out[V];
+                silu<V>(pre, out);
+                store<V>(to, out);
+            } else {
+                store<V>(to, pre);
             }
-            store<V>((T*)a.y + r * a.channels + c, out);
+            to += a.channels;
         };
-        // four rows in flight per thread
-        for (; row + 4 <= upto; row += 4) {
-            Vec<T, V> got[4];
+        constexpr int F = 4;
+        Vec<T, V> got[F], next[F];
+        const int blocks = (int)((upto - row) / F);
+        if (blocks > 0)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) got[i] = fetch<V>(x + (row + i) * a.channels + c);
+            for (int i = 0; i < F; ++i) got[i] = fetch<V>(from + i * a.channels);
+        for (int k = 0; k < blocks; ++k) {
+            from += F * a.channels;
+            if (k + 1 < blocks)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) step(row + i, got[i]);
+                for (int i = 0; i < F; ++i) next[i] = fetch<V>(from + i * a.channels);
+#pragma unroll
+            for (int i = 0; i < F; ++i) step(got[i]);
+#pragma unroll
+            for (int i = 0; i < F; ++i) got[i] = next[i];
         }
-        for (; row < upto; ++row) step(row, fetch<V>(x + row * a.channels + c));
+        for (row += (int64_t)blocks * F; row < upto; ++row, from += a.channels) step(fetch<V>(from));
         if (row == end && a.final_state)
 #pragma unroll
             for (int i = 0; i < W - 1; ++i)
@@ -262,26 +392,29 @@ __global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
 
 // one token per sequence: the window comes from and goes to the state (which may be the same memory)
 template <class T, int W, int V>
-__global__ void __launch_bounds__(256) pd_causal_conv_step_kernel(PdConvArgs a) {
+__global__ void __launch_bounds__(128) pd_causal_conv_step_kernel(PdConvArgs a) {
+    constexpr int P = kPairs<V>;
     const int64_t lanes = (a.channels + V - 1) / V;
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t s = id / lanes, c = id % lanes * V;
     if (s >= a.tok.seqs) return;
-    float win[W][V], out[V];
+    pair_t win[W - 1][P], now[P], pre[P], w[W][P], b[P];
     const int64_t at = s * (W - 1) * a.channels + c;
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) load<V>((const T*)a.initial + at + i * a.channels, win[i]);
-    load<V>((const T*)a.x + s * a.channels + c, win[W - 1]);
-#pragma unroll
-    for (int v = 0; v < V; ++v) {
-        float acc = a.bias ? a.bias[c + v] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < W; ++k) acc += a.weight[(c + v) * W + k] * win[k][v];
-        out[v] = a.silu ? acc * sigmoid_(acc) : acc;
+    load<V>((const T*)a.x + s * a.channels + c, now);
+    conv_parameters<W, V>(a, c, w, b);
+    convolve<W, P>(w, b, win, now, pre);
+    if (a.silu) {
+        float out[V];
+        silu<V>(pre, out);
+        store<V>((T*)a.y + s * a.channels + c, out);
+    } else {
+        store<V>((T*)a.y + s * a.channels + c, pre);
     }
-    store<V>((T*)a.y + s * a.channels + c, out);
+    slide<W - 1, P>(win, now);
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) store<V>((T*)a.final_state + at + i * a.channels, win[i + 1]);
+    for (int i = 0; i < W - 1; ++i) store<V>((T*)a.final_state + at + i * a.channels, win[i]);
 }
 
 // Gradients.  With g_t = dy_t act'(pre_t):
@@ -289,7 +422,8 @@ __global__ void __launch_bounds__(256) pd_causal_conv_step_kernel(PdConvArgs a) 
 // A thread walks its run and W - 1 rows beyond it, and keeps the W gradients of dx still open; sums of
 // dw and dbias stay in registers, then go to one partial per block, which a second launch adds up in order.
 template <class T, int W, int V, bool SILU>
-__global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) {
+__global__ void __launch_bounds__(256, 2) pd_causal_conv_grad_kernel(PdConvArgs a) {
+    constexpr int P = kPairs<V>;
     const int64_t lanes = (a.channels + V - 1) / V;
     // blockDim.x threads across channels, blockDim.y across runs; blockIdx.x channel blocks, blockIdx.y row blocks
     const int64_t lane = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -297,16 +431,14 @@ __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) 
     const bool active = lane < lanes;
     const T* x = (const T*)a.x;
     const T* dy = (const T*)a.dy;
-    float w[W][V], b[V], dw[W][V], db[V];
+    const float none[V] = {};
+    pair_t w[W][P], b[P], dw[W][P], db[P];
+    if (active) conv_parameters<W, V>(a, c, w, b);
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
+    for (int p = 0; p < P; ++p) {
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            w[k][v] = active ? a.weight[(c + v) * W + k] : 0.0f;
-            dw[k][v] = 0.0f;
-        }
-        b[v] = active && a.bias ? a.bias[c + v] : 0.0f;
-        db[v] = 0.0f;
+        for (int k = 0; k < W; ++k) dw[k][p] = 0;
+        db[p] = 0;
     }
     const int64_t runs = (a.tok.rows + a.run - 1) / a.run;
     const int64_t jobs = runs + (a.dinitial ? a.tok.seqs : 0);
@@ -318,11 +450,9 @@ __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) 
             int64_t begin, end;
             bounds_of(a.tok, s, begin, end);
             if (begin < end) continue;
-            float v[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) v[i] = 0.0f;
             for (int i = 0; i < W - 1; ++i) {
                 const int64_t at = (s * (W - 1) + i) * a.channels + c;
+                float v[V] = {};
                 if (a.dfinal) load<V>((const T*)a.dfinal + at, v);
                 store<V>((T*)a.dinitial + at, v);
             }
@@ -333,83 +463,105 @@ __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) 
         while (row < stop) {
             int64_t s, begin, end;
             if (!sequence_of(a.tok, row, s, begin, end)) {
-                float zero[V];
-#pragma unroll
-                for (int v = 0; v < V; ++v) zero[v] = 0.0f;
-                store<V>((T*)a.dx + row * a.channels + c, zero);
+                store<V>((T*)a.dx + row * a.channels + c, none);
                 ++row;
                 continue;
             }
-            float win[W - 1][V], open[W][V];   // open[j]: gradient of the input j rows back from the current one
+            pair_t win[W - 1][P], open[W][P];   // open[j]: gradient of the input j rows back from the current one
             conv_window<T, W, V>(a, x, s, begin, row, c, win);
 #pragma unroll
             for (int j = 0; j < W; ++j)
 #pragma unroll
-                for (int v = 0; v < V; ++v) open[j][v] = 0.0f;
+                for (int p = 0; p < P; ++p) open[j][p] = 0;
             const int64_t mine = end < stop ? end : stop;                        // rows whose sums belong here
             const int64_t upto = mine + (W - 1) < end ? mine + (W - 1) : end;    // rows whose g they need
-            const int64_t from = row;
-            auto step = [&](int64_t r, const Vec<T, V>& got_x, const Vec<T, V>& got_g) {
-                float now[V], g[V];
+            const int64_t first = row;
+            const T* from_x = x + row * a.channels + c;
+            const T* from_g = dy + row * a.channels + c;
+            T* to = (T*)a.dx + (row - (W - 1)) * a.channels + c;                 // where the input W - 1 rows back goes
+            auto step = [&](const Vec<T, V>& got_x, const Vec<T, V>& got_g, bool counts) {
+                pair_t now[P], g[P];
                 widen(got_x, now);
-                widen(got_g, g);
+                if (SILU) {
+                    pair_t pre[P];
+                    float v[V], q[V];
+                    convolve<W, P>(w, b, win, now, pre);
+                    part<V>(pre, q);
+                    widen(got_g, v);
 #pragma unroll
-                for (int v = 0; v < V; ++v) {
-                    if (SILU) {
-                        float pre = b[v];
-#pragma unroll
-                        for (int i = 0; i < W - 1; ++i) pre += w[i][v] * win[i][v];
-                        pre += w[W - 1][v] * now[v];
-                        const float sig = sigmoid_(pre);
-                        g[v] *= sig * (1.0f + pre * (1.0f - sig));
+                    for (int i = 0; i < V; ++i) {
+                        const float sig = sigmoid_(q[i]);
+                        v[i] *= sig * (1.0f + q[i] * (1.0f - sig));
                     }
-#pragma unroll
-                    for (int j = W - 1; j > 0; --j) open[j][v] = open[j - 1][v] + w[W - 1 - j][v] * g[v];
-                    open[0][v] = w[W - 1][v] * g[v];
-                    const float h = r < mine ? g[v] : 0.0f;
-                    db[v] += h;
-#pragma unroll
-                    for (int i = 0; i < W - 1; ++i) dw[i][v] += win[i][v] * h;
-                    dw[W - 1][v] += now[v] * h;
-#pragma unroll
-                    for (int i = 0; i + 1 < W - 1; ++i) win[i][v] = win[i + 1][v];
-                    win[W - 2][v] = now[v];
+                    pair_up<V>(v, g);
+                } else {
+                    widen(got_g, g);
                 }
-                // the input W - 1 rows back is complete
-                const int64_t done = r - (W - 1);
-                if (done >= from) store<V>((T*)a.dx + done * a.channels + c, open[W - 1]);
-                else if (done < begin && from == begin && a.dinitial) {
+#pragma unroll
+                for (int p = 0; p < P; ++p) {
+#pragma unroll
+                    for (int j = W - 1; j > 0; --j) open[j][p] = mad2(w[W - 1 - j][p], g[p], open[j - 1][p]);
+                    open[0][p] = mul2(w[W - 1][p], g[p]);
+                    if (counts) {
+                        db[p] = add2(db[p], g[p]);
+#pragma unroll
+                        for (int i = 0; i < W - 1; ++i) dw[i][p] = mad2(win[i][p], g[p], dw[i][p]);
+                        dw[W - 1][p] = mad2(now[p], g[p], dw[W - 1][p]);
+                    }
+                }
+                slide<W - 1, P>(win, now);
+            };
+            // the first W - 1 rows: the inputs before them are carried in, or another run's
+            auto edge = [&](bool counts) {
+                step(fetch<V>(from_x), fetch<V>(from_g), counts);
+                const int64_t done = row - (W - 1);
+                if (done >= first) store<V>(to, open[W - 1]);
+                else if (done < begin && first == begin && a.dinitial) {
                     // (a carried-in input that is carried out again is still open at the end, below)
                     store<V>((T*)a.dinitial + (s * (W - 1) + (done - begin) + (W - 1)) * a.channels + c, open[W - 1]);
                 }
+                ++row;
+                from_x += a.channels;
+                from_g += a.channels;
+                to += a.channels;
             };
-            for (; row + 4 <= upto; row += 4) {
-                Vec<T, V> got_x[4], got_g[4];
+            const int64_t head = first + (W - 1) < mine ? first + (W - 1) : mine;
+            while (row < head) edge(true);
+            constexpr int F = 4;
+            const int blocks = (int)((mine - row) / F);
+            for (int k = 0; k < blocks; ++k) {
+                Vec<T, V> got_x[F], got_g[F];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    got_x[i] = fetch<V>(x + (row + i) * a.channels + c);
-                    got_g[i] = fetch<V>(dy + (row + i) * a.channels + c);
+                for (int i = 0; i < F; ++i) {
+                    got_x[i] = fetch<V>(from_x + i * a.channels);
+                    got_g[i] = fetch<V>(from_g + i * a.channels);
                 }
+                from_x += F * a.channels;
+                from_g += F * a.channels;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) step(row + i, got_x[i], got_g[i]);
+                for (int i = 0; i < F; ++i) {
+                    step(got_x[i], got_g[i], true);
+                    store<V>(to, open[W - 1]);
+                    to += a.channels;
+                }
             }
-            for (; row < upto; ++row) step(row, fetch<V>(x + row * a.channels + c), fetch<V>(dy + row * a.channels + c));
+            row += (int64_t)blocks * F;
+            while (row < upto) edge(row < mine);
             if (row == end) {
                 // the sequence ends here: the inputs still open are complete, and were carried out
 #pragma unroll
                 for (int j = W - 2; j >= 0; --j) {
                     const int64_t r = end - 1 - j;
                     float v[V];
-#pragma unroll
-                    for (int u = 0; u < V; ++u) v[u] = open[j][u];
+                    part<V>(open[j], v);
                     if (a.dfinal) {
                         float f[V];
                         load<V>((const T*)a.dfinal + (s * (W - 1) + (W - 2 - j)) * a.channels + c, f);
 #pragma unroll
                         for (int u = 0; u < V; ++u) v[u] += f[u];
                     }
-                    if (r >= from && r < mine) store<V>((T*)a.dx + r * a.channels + c, v);
-                    else if (r < begin && from == begin && a.dinitial)
+                    if (r >= first && r < mine) store<V>((T*)a.dx + r * a.channels + c, v);
+                    else if (r < begin && first == begin && a.dinitial)
                         store<V>((T*)a.dinitial + (s * (W - 1) + (r - begin) + (W - 1)) * a.channels + c, v);
                 }
             }
@@ -418,14 +570,12 @@ __global__ void __launch_bounds__(256) pd_causal_conv_grad_kernel(PdConvArgs a) 
     }
     // block sums, in the order of the runs
     extern __shared__ float sums[];   // (blockDim.y, blockDim.x, V)
+#pragma unroll
     for (int k = 0; k <= W; ++k) {
+        float mine[V];
+        part<V>(k < W ? dw[k < W ? k : 0] : db, mine);
 #pragma unroll
-        for (int v = 0; v < V; ++v) {
-            float mine = db[v];
-#pragma unroll
-            for (int q = 0; q < W; ++q) if (q == k) mine = dw[q][v];
-            sums[(threadIdx.y * blockDim.x + threadIdx.x) * V + v] = mine;
-        }
+        for (int v = 0; v < V; ++v) sums[(threadIdx.y * blockDim.x + threadIdx.x) * V + v] = mine[v];
         __syncthreads();
         if (threadIdx.y == 0 && active)
 #pragma unroll
@@ -487,34 +637,6 @@ __device__ __forceinline__ ScanTile scan_tile(const PdScanArgs& a, int64_t tile)
     t.active = within < per;
     t.channel = t.group * per + (t.active ? within : per - 1);   // an idle lane repeats the last channel, stores nothing
     return t;
-}
-
-typedef unsigned long long pair_t;     // two float32 in one 64-bit register
-__device__ __forceinline__ pair_t pack(float x, float y) {
-    pair_t v;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
-    return v;
-}
-__device__ __forceinline__ void unpack(pair_t v, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v)); }
-__device__ __forceinline__ pair_t mul2(pair_t a, pair_t b) {
-    pair_t v;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-__device__ __forceinline__ pair_t add2(pair_t a, pair_t b) {
-    pair_t v;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
-    return v;
-}
-// a b + c: one rounding, except under SAFE, which keeps the product's own
-__device__ __forceinline__ pair_t mad2(pair_t a, pair_t b, pair_t c) {
-#if PD_MODE == 0
-    return add2(mul2(a, b), c);
-#else
-    pair_t v;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
-    return v;
-#endif
 }
 
 // exp(d A) for a rate as scan_rate() prepares it: FAST folds log2(e) into the rate.  An infinite rate becomes
@@ -640,11 +762,6 @@ __device__ __forceinline__ pair_t shift_down(pair_t v, int by) {
     float x, y;
     unpack(v, x, y);
     return pack(__shfl_down_sync(kFull, x, by), __shfl_down_sync(kFull, y, by));
-}
-__device__ __forceinline__ float halves(pair_t v) {
-    float x, y;
-    unpack(v, x, y);
-    return x + y;
 }
 // v[i] summed over the K lanes of a group, lane i keeping the i-th sum
 template <int K>
@@ -1365,9 +1482,8 @@ cudaError_t by_lanes(int state, F f) {
 template <class F>
 cudaError_t by_conv(const PdConvArgs& a, F f) {
     return by_type(a.type, [&](auto e) {
-        using T = decltype(e);
         return by_width(a.width, [&](auto w) {
-            return a.vec > 1 ? f(e, w, Int<(int)(16 / sizeof(T))>()) : f(e, w, Int<1>());
+            return a.vec > 1 ? f(e, w, Int<4>()) : f(e, w, Int<1>());
         });
     });
 }
@@ -1394,23 +1510,17 @@ cudaError_t launch_conv_step(const PdConvArgs& a, cudaStream_t st) {
     });
 }
 cudaError_t launch_conv_grad(const PdConvArgs& a, cudaStream_t st) {
-    return by_type(a.type, [&](auto e) {
+    return by_conv(a, [&](auto e, auto w, auto v) {
         using T = decltype(e);
-        return by_width(a.width, [&](auto w) {
-            constexpr int W = decltype(w)::value;
-            auto run = [&](auto v) -> cudaError_t {
-                constexpr int V = decltype(v)::value;
-                const int64_t lanes = (a.channels + V - 1) / V;
-                const dim3 block(32, 8), grid((unsigned)blocks_for(lanes, 32), (unsigned)a.row_blocks);
-                auto kernel = a.silu ? pd_causal_conv_grad_kernel<T, W, V, true> : pd_causal_conv_grad_kernel<T, W, V, false>;
-                kernel<<<grid, block, 256 * V * sizeof(float), st>>>(a);
-                cudaError_t err = cudaGetLastError();
-                if (err != cudaSuccess) return err;
-                pd_causal_conv_sum_kernel<W><<<(unsigned)blocks_for(a.channels * (W + 1), 128), 128, 0, st>>>(a);
-                return cudaGetLastError();
-            };
-            return a.vec > 1 ? run(Int<4>()) : run(Int<1>());
-        });
+        constexpr int W = decltype(w)::value, V = decltype(v)::value;
+        const int64_t lanes = (a.channels + V - 1) / V;
+        const dim3 block(32, 8), grid((unsigned)blocks_for(lanes, 32), (unsigned)a.row_blocks);
+        auto kernel = a.silu ? pd_causal_conv_grad_kernel<T, W, V, true> : pd_causal_conv_grad_kernel<T, W, V, false>;
+        kernel<<<grid, block, 256 * V * sizeof(float), st>>>(a);
+        cudaError_t err = cudaGetLastError();
+        if (err != cudaSuccess) return err;
+        pd_causal_conv_sum_kernel<W><<<(unsigned)blocks_for(a.channels * (W + 1), 128), 128, 0, st>>>(a);
+        return cudaGetLastError();
     });
 }
 
