@@ -220,7 +220,9 @@ __device__ __forceinline__ int64_t first_chunk(const PdTokens& t, int64_t s, int
 // Bound: memory, 2 bytes in and 2 out per bf16 element; next to them stand two
 // special-function operations (30 us of the 41 that 2 x 134 MB take) and two
 // packed multiply-adds, so what matters is to keep rows in flight: four of them
-// are fetched while the four before are worked on.
+// per thread, with four blocks of 256 threads on an SM (8 x 2048 x 4096 bf16 took
+// 82 us with two blocks and the next four rows fetched ahead, 76 with eight
+// channels per thread).
 // ===========================================================================
 // the taps and the bias of V channels, as 16-byte vectors where the channels are
 template <int W, int V>
@@ -314,7 +316,7 @@ __device__ __forceinline__ void silu(const pair_t (&pre)[kPairs<V>], float (&out
 }
 
 template <class T, int W, int V, bool SILU>
-__global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
+__global__ void __launch_bounds__(256, 4) pd_causal_conv_kernel(PdConvArgs a) {
     constexpr int P = kPairs<V>;
     const int64_t lanes = (a.channels + V - 1) / V;
     const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -367,20 +369,14 @@ __global__ void __launch_bounds__(256) pd_causal_conv_kernel(PdConvArgs a) {
             to += a.channels;
         };
         constexpr int F = 4;
-        Vec<T, V> got[F], next[F];
         const int blocks = (int)((upto - row) / F);
-        if (blocks > 0)
+        for (int k = 0; k < blocks; ++k) {
+            Vec<T, V> got[F];
 #pragma unroll
             for (int i = 0; i < F; ++i) got[i] = fetch<V>(from + i * a.channels);
-        for (int k = 0; k < blocks; ++k) {
             from += F * a.channels;
-            if (k + 1 < blocks)
-#pragma unroll
-                for (int i = 0; i < F; ++i) next[i] = fetch<V>(from + i * a.channels);
 #pragma unroll
             for (int i = 0; i < F; ++i) step(got[i]);
-#pragma unroll
-            for (int i = 0; i < F; ++i) got[i] = next[i];
         }
         for (row += (int64_t)blocks * F; row < upto; ++row, from += a.channels) step(fetch<V>(from));
         if (row == end && a.final_state)

@@ -51,12 +51,14 @@ int dims_of(const char* what, const int64_t grid[3], int64_t length, int64_t pac
     return PD_OK;
 }
 
-// Rows per thread of the convolution.  A run re-reads width - 1 rows of its predecessor (from L2), so long
-// runs move less and short ones fill the GPU sooner.
+// Rows per thread of the convolution.  A run re-reads width - 1 rows of its predecessor (from L2), so long runs
+// move less; 1024 threads per SM run at a time, so a call is cut into as few whole waves of them as give runs of
+// at most 128 rows.
 int conv_run(int64_t rows, int64_t lanes, int sms) {
-    int run = 32;
-    while (run > 4 && rows / run * lanes < (int64_t)sms * 1024) run /= 2;
-    return run;
+    const int64_t wave = (int64_t)sms * 1024, each = (rows * lanes + wave - 1) / wave;
+    const int64_t waves = (each + 127) / 128;
+    const int64_t run = waves ? (rows * lanes + waves * wave - 1) / (waves * wave) : 1;
+    return run < 4 ? 4 : (int)run;
 }
 // Channels per thread.  (Eight bf16 channels, 16 bytes, leave two blocks per SM their registers and ran
 // 8 x 2048 x 4096 in 67 us; four leave XX.)
