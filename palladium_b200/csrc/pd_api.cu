@@ -316,6 +316,7 @@ int build_plan(int family, const void* params, size_t params_bytes, int math_mod
         if (rc) return rc;
         plan->kernel_name = plan->scan.kernel_name;
         plan->grid[0] = plan->scan.grid;
+        plan->grid[1] = plan->scan.grid_y;
         plan->block[0] = plan->scan.block;
         plan->items = plan->scan.items;
         plan->launches = plan->scan.launches;

@@ -390,10 +390,10 @@ __global__ void __launch_bounds__(256, 4) pd_causal_conv_kernel(PdConvArgs a) {
 template <class T, int W, int V>
 __global__ void __launch_bounds__(128) pd_causal_conv_step_kernel(PdConvArgs a) {
     constexpr int P = kPairs<V>;
-    const int64_t lanes = (a.channels + V - 1) / V;
-    const int64_t id = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t s = id / lanes, c = id % lanes * V;
-    if (s >= a.tok.seqs) return;
+    const int lanes = (int)((a.channels + V - 1) / V), lane = blockIdx.x * blockDim.x + threadIdx.x;
+    if (lane >= lanes) return;
+    const int64_t c = (int64_t)lane * V;
+    for (int64_t s = blockIdx.y; s < a.tok.seqs; s += gridDim.y) {
     pair_t win[W - 1][P], now[P], pre[P], w[W][P], b[P];
     const int64_t at = s * (W - 1) * a.channels + c;
 #pragma unroll
@@ -411,6 +411,7 @@ __global__ void __launch_bounds__(128) pd_causal_conv_step_kernel(PdConvArgs a) 
     slide<W - 1, P>(win, now);
 #pragma unroll
     for (int i = 0; i < W - 1; ++i) store<V>((T*)a.final_state + at + i * a.channels, win[i]);
+    }
 }
 
 // Gradients.  With g_t = dy_t act'(pre_t):
@@ -605,34 +606,11 @@ __device__ __forceinline__ void load_states(const T* p, int first, int n, float 
     for (int i = 0; i < kStates; ++i) v[i] = first + i < n ? load1(p + first + i) : 0.0f;
 }
 
-// the same for parameters and states, four at a time where the call's sizes and alignment allow
-__device__ __forceinline__ void load_states(const float* p, int first, int n, bool vec, float (&v)[kStates]) {
-    if (vec && first + 4 <= n) {
-        const float4 q = *reinterpret_cast<const float4*>(p + first);
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else {
-        load_states(p, first, n, v);
-    }
-}
-
 template <int LN>
 __device__ __forceinline__ float sum_lanes(float v) {
 #pragma unroll
     for (int m = 1; m < LN; m *= 2) v += __shfl_xor_sync(kFull, v, m);
     return v;
-}
-
-// a warp's tile: 32 / LN channels of one group
-struct ScanTile { int64_t channel; int group; bool active; };
-template <int LN>
-__device__ __forceinline__ ScanTile scan_tile(const PdScanArgs& a, int64_t tile) {
-    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch;
-    ScanTile t;
-    t.group = (int)(tile / tiles);
-    const int64_t within = tile % tiles * ch + (threadIdx.x & 31) / LN;
-    t.active = within < per;
-    t.channel = t.group * per + (t.active ? within : per - 1);   // an idle lane repeats the last channel, stores nothing
-    return t;
 }
 
 // exp(d A) for a rate as scan_rate() prepares it: FAST folds log2(e) into the rate.  An infinite rate becomes
@@ -708,42 +686,60 @@ __device__ __forceinline__ Raw4<T> raw4(const T* p) {       // from shared memor
     return r;
 }
 
-// one token per sequence; state in and out may be the same memory
-template <class T, int LN>
-__global__ void __launch_bounds__(128) pd_selective_scan_step_kernel(PdScanArgs a) {
-    const int64_t per = a.channels / a.groups, ch = 32 / LN, tiles = (per + ch - 1) / ch * a.groups;
-    const int64_t job = (int64_t)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
-    const int64_t s = job / tiles;
-    if (s >= a.tok.seqs) return;
+// One token per sequence; state in and out may be the same memory.  Bound: the states, read and written once, 8
+// bytes per state: LN neighbouring lanes read a channel's states as one 16-byte vector each (VEC), a warp 512 bytes.
+template <class T, int LN, bool VEC>
+__global__ void __launch_bounds__(256) pd_selective_scan_step_kernel(PdScanArgs a) {
+    // blockIdx.x and the warps across channels, blockIdx.y across sequences: a thread works for one token, and a
+    // division for its place would cost it more than the rest (49 us for 256 x 4096 x 16 with four of them)
+    const int per = (int)(a.channels / a.groups), ch = 32 / LN, tiles = (per + ch - 1) / ch;
+    const int job = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, group = a.groups == 1 ? 0 : job / tiles;
+    if (group >= a.groups || (a.groups == 1 && job >= tiles)) return;
     const int lane = threadIdx.x & 31, sub = lane % LN, first = sub * kStates;
-    const ScanTile tile = scan_tile<LN>(a, job % tiles);
-    const int64_t c = tile.channel, state_at = (s * a.channels + c) * a.state;
+    const int within = (job - group * tiles) * ch + lane / LN;
+    const bool active = within < per;
+    const int64_t c = group * per + (active ? within : per - 1);     // an idle lane repeats the last channel
+    for (int64_t s = blockIdx.y; s < a.tok.seqs; s += gridDim.y) {
+    const int64_t at = s * a.channels + c, state_at = at * a.state;
+    const int64_t bc = (s * a.groups + group) * a.state;
     float A[kStates], B[kStates], C[kStates], h[kStates];
-    load_states(a.A + c * a.state, first, a.state, A);
-    load_states(a.initial + state_at, first, a.state, h);
-    const int64_t bc = (s * a.groups + tile.group) * a.state;
-    load_states((const T*)a.B + bc, first, a.state, B);
-    load_states((const T*)a.C + bc, first, a.state, C);
-    const float x = load1((const T*)a.x + s * a.channels + c);
-    float d = load1((const T*)a.delta + s * a.channels + c) + (a.bias ? a.bias[c] : 0.0f);
+    if (VEC) {
+        const float4 qh = *reinterpret_cast<const float4*>(a.initial + state_at + first);
+        const float4 qa = *reinterpret_cast<const float4*>(a.A + c * a.state + first);
+        h[0] = qh.x; h[1] = qh.y; h[2] = qh.z; h[3] = qh.w;
+        A[0] = qa.x; A[1] = qa.y; A[2] = qa.z; A[3] = qa.w;
+        load<4>((const T*)a.B + bc + first, B);
+        load<4>((const T*)a.C + bc + first, C);
+    } else {
+        load_states(a.A + c * a.state, first, a.state, A);
+        load_states(a.initial + state_at, first, a.state, h);
+        load_states((const T*)a.B + bc, first, a.state, B);
+        load_states((const T*)a.C + bc, first, a.state, C);
+    }
+    const float x = load1((const T*)a.x + at), z = a.z ? load1((const T*)a.z + at) : 0.0f;
+    float d = load1((const T*)a.delta + at) + (a.bias ? a.bias[c] : 0.0f);
+    const float skip = a.skip ? a.skip[c] : 0.0f;
     if (a.softplus) d = softplus_(d);
     const float u = d * x;
     float y = 0.0f;
 #pragma unroll
     for (int i = 0; i < kStates; ++i) {
-        h[i] = exp_(d * A[i]) * h[i] + (first + i < a.state ? u * B[i] : 0.0f);
-        y += first + i < a.state ? C[i] * h[i] : 0.0f;
+        const bool in = VEC || first + i < a.state;
+        h[i] = exp_(d * A[i]) * h[i] + (in ? u * B[i] : 0.0f);
+        y += in ? C[i] * h[i] : 0.0f;
     }
     y = sum_lanes<LN>(y);
-    if (a.skip) y += a.skip[c] * x;
-    if (a.z) {
-        const float z = load1((const T*)a.z + s * a.channels + c);
-        y *= z * sigmoid_(z);
+    if (a.skip) y += skip * x;
+    if (a.z) y *= z * sigmoid_(z);
+    if (!active) continue;
+    if (sub == 0) store1((T*)a.y + at, y);
+    if (VEC) {
+        *reinterpret_cast<float4*>(a.final_state + state_at + first) = make_float4(h[0], h[1], h[2], h[3]);
+    } else {
+        for (int i = 0; i < kStates; ++i)
+            if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
     }
-    if (!tile.active) return;
-    if (sub == 0) store1((T*)a.y + s * a.channels + c, y);
-    for (int i = 0; i < kStates; ++i)
-        if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -1500,8 +1496,9 @@ cudaError_t launch_conv_step(const PdConvArgs& a, cudaStream_t st) {
     return by_conv(a, [&](auto e, auto w, auto v) {
         using T = decltype(e);
         const int64_t lanes = (a.channels + v.value - 1) / v.value;
-        if (lanes * a.tok.seqs == 0) return cudaSuccess;
-        pd_causal_conv_step_kernel<T, decltype(w)::value, decltype(v)::value><<<(unsigned)blocks_for(lanes * a.tok.seqs, 128), 128, 0, st>>>(a);
+        if (a.tok.seqs == 0) return cudaSuccess;
+        const dim3 grid((unsigned)blocks_for(lanes, 128), (unsigned)(a.tok.seqs < 65535 ? a.tok.seqs : 65535));
+        pd_causal_conv_step_kernel<T, decltype(w)::value, decltype(v)::value><<<grid, 128, 0, st>>>(a);
         return cudaGetLastError();
     });
 }
@@ -1520,10 +1517,6 @@ cudaError_t launch_conv_grad(const PdConvArgs& a, cudaStream_t st) {
     });
 }
 
-int64_t scan_tiles(const PdScanArgs& a) {
-    const int64_t per = a.channels / a.groups, ch = 32 / pd_scan_lanes(a.state);
-    return (per + ch - 1) / ch;
-}
 cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
     return by_type(a.type, [&](auto e) {
         using T = decltype(e);
@@ -1548,9 +1541,13 @@ cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {
     return by_type(a.type, [&](auto e) {
         using T = decltype(e);
         return by_lanes(a.state, [&](auto ln) {
-            const int64_t jobs = scan_tiles(a) * a.groups * a.tok.seqs;
-            if (jobs == 0) return cudaSuccess;
-            pd_selective_scan_step_kernel<T, decltype(ln)::value><<<(unsigned)blocks_for(jobs, 4), 128, 0, st>>>(a);
+            constexpr int LN = decltype(ln)::value;
+            if (a.tok.seqs == 0) return cudaSuccess;
+            const dim3 grid((unsigned)pd_step_blocks(a.channels, a.groups, a.state, a.tok.seqs),
+                            (unsigned)(a.tok.seqs < 65535 ? a.tok.seqs : 65535));
+            const bool vec = a.state == 4 * LN && a.vec_states && a.vec_params;
+            auto kernel = vec ? pd_selective_scan_step_kernel<T, LN, true> : pd_selective_scan_step_kernel<T, LN, false>;
+            kernel<<<grid, 32 * pd_step_warps(a.channels, a.groups, a.state, a.tok.seqs), 0, st>>>(a);
             return cudaGetLastError();
         });
     });

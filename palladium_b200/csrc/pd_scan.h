@@ -58,6 +58,21 @@ inline int pd_scan_lanes(int state) { return state <= 4 ? 1 : state <= 8 ? 2 : s
 inline int pd_scan_slice_lanes(int state) { return state <= 4 ? 1 : state <= 8 ? 2 : 4; }
 inline int pd_scan_pad(int state) { const int w = 4 * pd_scan_slice_lanes(state); return (state + w - 1) / w * w; }
 
+// The step kernel's geometry: warps of 32 / lanes channels, up to eight to a block; a small call takes one to a
+// block, so that its warps spread over the SMs.
+inline int64_t pd_step_tiles(int64_t channels, int groups, int state) {
+    const int64_t per = channels / groups, ch = 32 / pd_scan_lanes(state);
+    return (per + ch - 1) / ch * groups;
+}
+inline int pd_step_warps(int64_t channels, int groups, int state, int64_t seqs) {
+    const int64_t tiles = pd_step_tiles(channels, groups, state);
+    return tiles * seqs < 1024 ? 1 : tiles < 8 ? (int)tiles : 8;
+}
+inline int64_t pd_step_blocks(int64_t channels, int groups, int state, int64_t seqs) {
+    const int warps = pd_step_warps(channels, groups, state, seqs);
+    return (pd_step_tiles(channels, groups, state) + warps - 1) / warps;
+}
+
 struct PdScanTable {
     cudaError_t (*conv)(const PdConvArgs&, cudaStream_t);
     cudaError_t (*conv_step)(const PdConvArgs&, cudaStream_t);
@@ -73,7 +88,7 @@ const PdScanTable* pd_scan_table_fast();
 // What the C ABI needs of a call: its buffers' sizes, its launches and its scratch.
 struct PdScanPlan {
     const char* kernel_name = "";
-    int64_t grid = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
+    int64_t grid = 1, grid_y = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
     int64_t row_blocks = 0;       // gradient of the convolution: blocks along the rows
     int64_t params_offset = 0;    // gradient of the scan: where in the scratch the parameters' sums begin
     std::vector<size_t> in_bytes, out_bytes;

@@ -81,10 +81,6 @@ int64_t conv_partial(const Dims& d, int64_t width, int64_t row_blocks) { return 
 int64_t scan_chunks(const pd_selective_scan_params* p, const Dims& d) {
     return p->packed ? p->length / PD_SCAN_CHUNK + d.seqs : d.seqs * ((p->length + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK);
 }
-int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d) {
-    const int64_t per = d.channels / p->groups, ch = 32 / pd_scan_lanes((int)p->state);
-    return (per + ch - 1) / ch * p->groups;
-}
 // Channels a warp takes one after another (a block is four warps; four blocks an SM for prompts, three for
 // gradients).  More of them share the fetched B and C and, in the gradient, one sum over the block's warps and one
 // partial sum of dB and dC in memory, worth about one channel's work per tile; fewer give more blocks.  The
@@ -127,7 +123,8 @@ int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3],
         out = {tokens, edge};
         plan->kernel_name = "pd_causal_conv_step_kernel";
         plan->block = 128;
-        plan->grid = (d.seqs * lanes + 127) / 128;
+        plan->grid = (lanes + 127) / 128;
+        plan->grid_y = d.seqs < 65535 ? d.seqs : 65535;
         return PD_OK;
     }
     in = {tokens, weight};
@@ -154,7 +151,8 @@ int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3],
     int grad_run;
     conv_grad_blocks(d.rows, p->initial ? d.seqs : 0, lanes, sms, &grad_run, &plan->row_blocks);
     plan->items = grad_run;
-    plan->grid = (lanes + 31) / 32 * plan->row_blocks;
+    plan->grid = (lanes + 31) / 32;
+    plan->grid_y = plan->row_blocks;
     plan->launches = 2;
     plan->scratch_bytes = conv_partial(d, p->width, plan->row_blocks);
     return PD_OK;
@@ -186,11 +184,13 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
     if (p->skip) in.push_back(vec);
     if (p->gate) in.push_back(tokens);
     plan->block = 128;
-    const int64_t tiles = scan_tiles(p, d), free_rows = p->packed ? 1 : 0;
+    const int64_t free_rows = p->packed ? 1 : 0;
     if (step) {
         out = {tokens, edge};
         plan->kernel_name = "pd_selective_scan_step_kernel";
-        plan->grid = (tiles * d.seqs + 3) / 4;
+        plan->grid = pd_step_blocks(d.channels, (int)p->groups, (int)p->state, d.seqs);
+        plan->grid_y = d.seqs < 65535 ? d.seqs : 65535;
+        plan->block = 32 * pd_step_warps(d.channels, (int)p->groups, (int)p->state, d.seqs);
         return PD_OK;
     }
     // one block per tile of channels and sequence
@@ -332,7 +332,7 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % four) a.vec = 0;
         a.vec_states = a.state % 4 == 0 && reinterpret_cast<uintptr_t>(a.B) % four == 0 && reinterpret_cast<uintptr_t>(a.C) % four == 0;
         a.per_warp = (int)plan.items;
-        a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries);
+        a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries) && aligned16(a.final_state);
         e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
     }
     if (e != cudaSuccess) {
