@@ -613,30 +613,6 @@ __device__ __forceinline__ float sum_lanes(float v) {
     return v;
 }
 
-// exp(d A) for a rate as scan_rate() prepares it: FAST folds log2(e) into the rate.  An infinite rate becomes
-// the largest finite one, whose decay over any step is the same, so that a tile's tokens behind the
-// sequence's end (steps of length zero) leave the state as it is instead of multiplying zero by infinity.
-__device__ __forceinline__ float scan_rate(float A) {
-#if PD_MODE == 2
-    A *= 1.4426950408889634f;
-#endif
-    return fabsf(A) == INFINITY ? copysignf(3.4028234e38f, A) : A;
-}
-__device__ __forceinline__ float exp2_approx(float v) {
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-    return r;
-}
-__device__ __forceinline__ pair_t decay2(pair_t d, pair_t rate) {
-    float x, y;
-    unpack(mul2(d, rate), x, y);
-#if PD_MODE == 2
-    return pack(exp2_approx(x), exp2_approx(y));
-#else
-    return pack(expf(x), expf(y));
-#endif
-}
-
 // four elements as stored, fetched ahead of their use
 template <class T> struct Raw4 { T e[4]; };
 template <class T>
@@ -686,12 +662,44 @@ __device__ __forceinline__ Raw4<T> raw4(const T* p) {       // from shared memor
     return r;
 }
 
+// exp(d A) for a rate as scan_rate() prepares it: FAST folds log2(e) into the rate.  An infinite rate becomes
+// the largest finite one, whose decay over any step is the same, so that a tile's tokens behind the
+// sequence's end (steps of length zero) leave the state as it is instead of multiplying zero by infinity.
+__device__ __forceinline__ float scan_rate(float A) {
+#if PD_MODE == 2
+    A *= 1.4426950408889634f;
+#endif
+    return fabsf(A) == INFINITY ? copysignf(3.4028234e38f, A) : A;
+}
+__device__ __forceinline__ float exp2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float decay(float d, float rate) {
+#if PD_MODE == 2
+    return exp2_approx(d * rate);
+#else
+    return expf(d * rate);
+#endif
+}
+__device__ __forceinline__ pair_t decay2(pair_t d, pair_t rate) {
+    float x, y;
+    unpack(mul2(d, rate), x, y);
+#if PD_MODE == 2
+    return pack(exp2_approx(x), exp2_approx(y));
+#else
+    return pack(expf(x), expf(y));
+#endif
+}
+
 // One token per sequence; state in and out may be the same memory.  Bound: the states, read and written once, 8
 // bytes per state: LN neighbouring lanes read a channel's states as one 16-byte vector each (VEC), a warp 512 bytes.
 template <class T, int LN, bool VEC>
 __global__ void __launch_bounds__(256) pd_selective_scan_step_kernel(PdScanArgs a) {
     // blockIdx.x and the warps across channels, blockIdx.y across sequences: a thread works for one token, and a
-    // division for its place would cost it more than the rest (49 us for 256 x 4096 x 16 with four of them)
+    // division for its place would cost it more than the rest (49 us for 256 x 4096 x 16 with four of them; 43 with one
+    // sequence per thread, two thirds of whose instructions were addresses)
     const int per = (int)(a.channels / a.groups), ch = 32 / LN, tiles = (per + ch - 1) / ch;
     const int job = blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32, group = a.groups == 1 ? 0 : job / tiles;
     if (group >= a.groups || (a.groups == 1 && job >= tiles)) return;
@@ -699,46 +707,75 @@ __global__ void __launch_bounds__(256) pd_selective_scan_step_kernel(PdScanArgs 
     const int within = (job - group * tiles) * ch + lane / LN;
     const bool active = within < per;
     const int64_t c = group * per + (active ? within : per - 1);     // an idle lane repeats the last channel
-    for (int64_t s = blockIdx.y; s < a.tok.seqs; s += gridDim.y) {
-    const int64_t at = s * a.channels + c, state_at = at * a.state;
-    const int64_t bc = (s * a.groups + group) * a.state;
-    float A[kStates], B[kStates], C[kStates], h[kStates];
+    float A[kStates];
     if (VEC) {
-        const float4 qh = *reinterpret_cast<const float4*>(a.initial + state_at + first);
-        const float4 qa = *reinterpret_cast<const float4*>(a.A + c * a.state + first);
-        h[0] = qh.x; h[1] = qh.y; h[2] = qh.z; h[3] = qh.w;
-        A[0] = qa.x; A[1] = qa.y; A[2] = qa.z; A[3] = qa.w;
-        load<4>((const T*)a.B + bc + first, B);
-        load<4>((const T*)a.C + bc + first, C);
+        const float4 q = *reinterpret_cast<const float4*>(a.A + c * a.state + first);
+        A[0] = q.x; A[1] = q.y; A[2] = q.z; A[3] = q.w;
     } else {
         load_states(a.A + c * a.state, first, a.state, A);
-        load_states(a.initial + state_at, first, a.state, h);
-        load_states((const T*)a.B + bc, first, a.state, B);
-        load_states((const T*)a.C + bc, first, a.state, C);
     }
-    const float x = load1((const T*)a.x + at), z = a.z ? load1((const T*)a.z + at) : 0.0f;
-    float d = load1((const T*)a.delta + at) + (a.bias ? a.bias[c] : 0.0f);
-    const float skip = a.skip ? a.skip[c] : 0.0f;
-    if (a.softplus) d = softplus_(d);
-    const float u = d * x;
-    float y = 0.0f;
 #pragma unroll
-    for (int i = 0; i < kStates; ++i) {
-        const bool in = VEC || first + i < a.state;
-        h[i] = exp_(d * A[i]) * h[i] + (in ? u * B[i] : 0.0f);
-        y += in ? C[i] * h[i] : 0.0f;
-    }
-    y = sum_lanes<LN>(y);
-    if (a.skip) y += skip * x;
-    if (a.z) y *= z * sigmoid_(z);
-    if (!active) continue;
-    if (sub == 0) store1((T*)a.y + at, y);
-    if (VEC) {
-        *reinterpret_cast<float4*>(a.final_state + state_at + first) = make_float4(h[0], h[1], h[2], h[3]);
-    } else {
-        for (int i = 0; i < kStates; ++i)
-            if (first + i < a.state) a.final_state[state_at + first + i] = h[i];
-    }
+    for (int i = 0; i < kStates; ++i) A[i] = scan_rate(A[i]);
+    const float bias = a.bias ? a.bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
+    // a block takes `run` sequences one after another, the next one's operands on their way
+    const int64_t s0 = (int64_t)blockIdx.y * a.run;
+    const int left = (int)(a.tok.seqs - s0 < a.run ? a.tok.seqs - s0 : a.run);
+    const int64_t step = a.channels, step_h = a.channels * a.state, step_bc = (int64_t)a.groups * a.state;
+    const T* px = (const T*)a.x + s0 * step + c;
+    const T* pd = (const T*)a.delta + s0 * step + c;
+    const T* pz = a.z ? (const T*)a.z + s0 * step + c : nullptr;
+    const T* pB = (const T*)a.B + s0 * step_bc + group * a.state;
+    const T* pC = (const T*)a.C + s0 * step_bc + group * a.state;
+    const float* ph = a.initial + s0 * step_h + c * a.state;
+    T* py = (T*)a.y + s0 * step + c;
+    float* po = a.final_state + s0 * step_h + c * a.state;
+    struct Operands { float h[kStates], B[kStates], C[kStates], x, d, z; };
+    auto fetch_next = [&](Operands& q) {
+        if (VEC) {
+            const float4 v = *reinterpret_cast<const float4*>(ph + first);
+            q.h[0] = v.x; q.h[1] = v.y; q.h[2] = v.z; q.h[3] = v.w;
+            load<4>(pB + first, q.B);
+            load<4>(pC + first, q.C);
+        } else {
+            load_states(ph, first, a.state, q.h);
+            load_states(pB, first, a.state, q.B);
+            load_states(pC, first, a.state, q.C);
+        }
+        q.x = load1(px);
+        q.d = load1(pd);
+        q.z = pz ? load1(pz) : 0.0f;
+        ph += step_h; pB += step_bc; pC += step_bc; px += step; pd += step;
+        if (pz) pz += step;
+    };
+    Operands now, next;
+    fetch_next(now);
+    for (int k = 0; k < left; ++k) {
+        if (k + 1 < left) fetch_next(next);
+        float d = now.d + bias;
+        if (a.softplus) d = softplus_(d);
+        const float u = d * now.x;
+        float h[kStates], y = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kStates; ++i) {
+            const bool in = VEC || first + i < a.state;
+            h[i] = decay(d, A[i]) * now.h[i] + (in ? u * now.B[i] : 0.0f);
+            y += in ? now.C[i] * h[i] : 0.0f;
+        }
+        y = sum_lanes<LN>(y);
+        if (a.skip) y += skip * now.x;
+        if (a.z) y *= now.z * sigmoid_(now.z);
+        if (active) {
+            if (sub == 0) store1(py, y);
+            if (VEC) {
+                *reinterpret_cast<float4*>(po + first) = make_float4(h[0], h[1], h[2], h[3]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kStates; ++i) if (first + i < a.state) po[first + i] = h[i];
+            }
+        }
+        py += step;
+        po += step_h;
+        now = next;
     }
 }
 
@@ -1544,7 +1581,7 @@ cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {
             constexpr int LN = decltype(ln)::value;
             if (a.tok.seqs == 0) return cudaSuccess;
             const dim3 grid((unsigned)pd_step_blocks(a.channels, a.groups, a.state, a.tok.seqs),
-                            (unsigned)(a.tok.seqs < 65535 ? a.tok.seqs : 65535));
+                            (unsigned)((a.tok.seqs + a.run - 1) / a.run));
             const bool vec = a.state == 4 * LN && a.vec_states && a.vec_params;
             auto kernel = vec ? pd_selective_scan_step_kernel<T, LN, true> : pd_selective_scan_step_kernel<T, LN, false>;
             kernel<<<grid, 32 * pd_step_warps(a.channels, a.groups, a.state, a.tok.seqs), 0, st>>>(a);

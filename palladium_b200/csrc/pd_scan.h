@@ -41,6 +41,7 @@ struct PdScanArgs {
     int vec;                  // tokens can be read four channels at a time
     int vec_states;           // B and C four states at a time
     int vec_params;           // A and the states four at a time
+    int run;                  // single tokens: sequences a block takes one after another
     int per_warp;             // channels a warp takes one after another
     int64_t channels;
     const void *x, *delta, *B, *C, *z, *dy;
@@ -71,6 +72,15 @@ inline int pd_step_warps(int64_t channels, int groups, int state, int64_t seqs) 
 inline int64_t pd_step_blocks(int64_t channels, int groups, int state, int64_t seqs) {
     const int warps = pd_step_warps(channels, groups, state, seqs);
     return (pd_step_tiles(channels, groups, state) + warps - 1) / warps;
+}
+
+// Sequences per block: a few where that leaves a full GPU of blocks, and what the second launch dimension asks for.
+inline int pd_step_run(int64_t channels, int groups, int state, int64_t seqs, int sms) {
+    const int64_t warps = pd_step_tiles(channels, groups, state) * seqs, full = (int64_t)sms * 64;
+    int64_t run = warps / full;
+    run = run < 1 ? 1 : run > 8 ? 8 : run;
+    const int64_t least = (seqs + 65534) / 65535;
+    return (int)(run < least ? least : run);
 }
 
 struct PdScanTable {

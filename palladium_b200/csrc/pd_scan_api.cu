@@ -189,7 +189,8 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         out = {tokens, edge};
         plan->kernel_name = "pd_selective_scan_step_kernel";
         plan->grid = pd_step_blocks(d.channels, (int)p->groups, (int)p->state, d.seqs);
-        plan->grid_y = d.seqs < 65535 ? d.seqs : 65535;
+        plan->items = pd_step_run(d.channels, (int)p->groups, (int)p->state, d.seqs, sms);
+        plan->grid_y = (d.seqs + plan->items - 1) / plan->items;
         plan->block = 32 * pd_step_warps(d.channels, (int)p->groups, (int)p->state, d.seqs);
         return PD_OK;
     }
@@ -331,7 +332,7 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         const void* tokens[] = {a.x, a.delta, a.z, a.dy, a.y, a.dx, a.ddelta, a.dz};
         for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % four) a.vec = 0;
         a.vec_states = a.state % 4 == 0 && reinterpret_cast<uintptr_t>(a.B) % four == 0 && reinterpret_cast<uintptr_t>(a.C) % four == 0;
-        a.per_warp = (int)plan.items;
+        a.per_warp = a.run = (int)plan.items;
         a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries) && aligned16(a.final_state);
         e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
     }
