@@ -825,256 +825,265 @@ __device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
 }
 
 // ---------------------------------------------------------------------------
-// The prompt kernel.  A block owns four warps' channels of one group and walks one sequence in tiles of 64
-// tokens.  A warp takes its channels one after another, each over the whole tile at once: a lane holds K tokens'
-// four states, LN lanes the states of a token group, 32 / LN lanes the token groups.  A pass from a zero state
-// keeps the decays exp(d A) in registers, a scan over the token groups by shuffles gives the state entering each,
-// and a second pass over the same registers the outputs: one exponential per (token, channel, state).  With tokens
-// across lanes a single sequence fills the GPU, and B and C, which all channels of a group share, are read from
-// shared memory once per tile and warp instead of once per channel (a layout with channels across lanes, decays
-// in registers and warps across tokens spent its time reading them: 5 words of shared memory per state).
+// The prompt kernel.  A lane holds four states of NCH neighbouring channels and walks the tokens one by one; LN
+// lanes share a channel, 32 / LN * NCH channels make a warp's, two warps a block.  A tile of 32 tokens is staged in
+// shared memory as float32 (step lengths, inputs, couplings), the next one's elements on their way meanwhile, and
+// the LN partial sums of each output meet there too.
+//
+// Bound: the exponentials, one per (token, channel, state), 16 per clock and SM: 8 cycles per warp instruction and
+// scheduler.  Beside each stand 2 packed multiply-adds and, with two channels per lane, 1.75 words of shared memory
+// (7 of the 8 cycles).  Forms that hold tokens across lanes or warps instead, so as to fill the GPU with one
+// sequence, needed 18 to 31 instructions per state for their scans (8192 x 2048 x 16 took 417 us); so a call with
+// few sequences and channels is cut into segments of tokens: a first launch (STATE) takes each from a zero state
+// to its end state and total step, and the blocks of the second compose the state entering theirs.
 // ---------------------------------------------------------------------------
-#ifndef PD_SCAN_BLOCKS
-#define PD_SCAN_BLOCKS 3
-#endif
-constexpr int kScanWarps = 4, kScanThreads = 32 * kScanWarps;
+constexpr int kScanWarps = 2, kScanThreads = 32 * kScanWarps;
 
 struct ScanShape {
-    int channels, pad, slices, pitch;
-    int x, d, z, y, carry, rate, skip, raw, couplings, bytes;
-    static constexpr int kRow = 64;
-    __host__ __device__ ScanShape(int ln, int state, int per_warp, int element) {
-        const int wide = 4 * ln;
-        channels = kScanWarps * per_warp;
-        slices = (state + wide - 1) / wide;
-        pad = slices * wide;
-        pitch = pad + 4;          // elements between two tokens' couplings: the token groups lie in different banks
-        const int cells = channels * kRow;
-        x = 0; d = x + cells; z = d + cells; y = z + cells;
-        carry = y + (slices > 1 ? cells : 0);
-        rate = carry + channels * pad;
-        skip = rate + channels * pad;
-        raw = (skip + channels) * 4;             // x, delta, z: (3, tokens, channels)
-        couplings = raw + 3 * cells * element;   // two buffers of B and C: (2, 2, tokens, pitch)
-        bytes = couplings + 4 * kRow * pitch * element;
-    }
+    int warp_channels, channels, pad;
+    int du, B, C, y, raw, bytes;      // offsets in floats, from `raw` on in bytes
+    static constexpr int kRow = PD_SCAN_CHUNK;
+    __host__ __device__ constexpr ScanShape(int ln, int nch, int element)
+        : warp_channels(32 / ln * nch), channels(kScanWarps * warp_channels), pad(4 * ln), du(0),
+          B(2 * kRow * channels), C(B + kRow * pad), y(C + kRow * pad), raw((y + kScanWarps * kRow * 32 * nch) * 4),
+          // two buffers of x, delta, z: (3, tokens, channels), and one of B and C: (2, tokens, pad)
+          bytes(raw + 6 * kRow * channels * element + 2 * kRow * pad * element) {}
 };
 
-template <class T, int LN, bool GATE, bool FULL>
-__global__ void __launch_bounds__(kScanThreads, PD_SCAN_BLOCKS) pd_selective_scan_kernel(PdScanArgs a) {
-    constexpr int K = 2 * LN, TL = 32 / LN, kRow = ScanShape::kRow, kWide = 4 * LN, kPart = K < 4 ? K : 4;
-    static_assert(K * TL == kRow && kRow % PD_SCAN_CHUNK == 0 && PD_SCAN_CHUNK % K == 0, "a warp covers a tile of whole chunks");
+// segments: where a sequence's first one is counted, and the sequence of the id-th (an empty one has one, too)
+__device__ __forceinline__ int64_t dense_segments(const PdScanArgs& a) {
+    return a.tok.length > a.segment ? (a.tok.length + a.segment - 1) / a.segment : 1;
+}
+__device__ __forceinline__ int64_t first_segment(const PdScanArgs& a, int64_t s, int64_t begin) {
+    return a.tok.offsets ? begin / a.segment + s : s * dense_segments(a);
+}
+__device__ __forceinline__ int64_t segment_owner(const PdScanArgs& a, int64_t id) {
+    if (!a.tok.offsets) return id / dense_segments(a);
+    int64_t lo = 0, hi = a.tok.seqs;    // the last s whose first segment is not behind id
+    while (lo < hi) {
+        const int64_t mid = (lo + hi) / 2;
+        if (first_segment(a, mid, clamp_row(a.tok.offsets[mid], a.tok.rows)) <= id) lo = mid + 1; else hi = mid;
+    }
+    return lo - 1;
+}
+
+template <class T, int LN, int NCH, bool FULL, bool STATE>
+__global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdScanArgs a) {
+    constexpr ScanShape G(LN, NCH, sizeof(T));
+    constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kScanThreads / quads;
+    static_assert(kScanThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");
     extern __shared__ float4 smem4[];
     float* smem = reinterpret_cast<float*>(smem4);
-    const ScanShape G(LN, a.state, a.per_warp, sizeof(T));
-    float *sX = smem + G.x, *sD = smem + G.d, *sZ = smem + G.z;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, tl = lane / LN;
-    const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
-    const int64_t job = blockIdx.x, s = job / (tiles * a.groups);
-    const int64_t group = job / tiles % a.groups, within = job % tiles * G.channels;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, cl = lane / LN, first = sub * 4;
+    const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels, all = tiles * a.groups;
+    const int64_t id = blockIdx.x / all, tile = blockIdx.x - id * all;
+    const int64_t group = a.groups == 1 ? 0 : tile / tiles, within = (tile - group * tiles) * G.channels;
     const int64_t c0 = group * per + within;                            // the block's first channel
     const int count = (int)(per - within < G.channels ? per - within : G.channels);
-    if (s == a.tok.seqs) {
+    if (id == a.segments) {     // (packed calls: one more)
         for_free_rows(a.tok, [&](int64_t r) {
             for (int c = tid; c < count; c += kScanThreads) store1((T*)a.y + r * a.channels + c0 + c, 0.0f);
         });
         return;
     }
+    const int64_t s = segment_owner(a, id);
+    if (s < 0) return;
     int64_t begin, end;
     bounds_of(a.tok, s, begin, end);
-    // swizzled places of (channel, token), as in the gradient kernel
-    auto place = [](int c, int t) { return c * kRow + (t ^ ((c >> 2 & 7) << 2)); };
-    for (int i = tid; i < G.channels * G.pad; i += kScanThreads) {
-        const int c = i / G.pad, n = i % G.pad;
-        const bool in = c < count && n < a.state;
-        smem[G.carry + i] = a.initial && in ? a.initial[(s * a.channels + c0 + c) * a.state + n] : 0.0f;
-        smem[G.rate + i] = in ? scan_rate(a.A[(c0 + c) * a.state + n]) : 0.0f;
-    }
-    if (tid < G.channels) smem[G.skip + tid] = a.skip && tid < count ? a.skip[c0 + tid] : 0.0f;
-    // staging: four channels of a token per thread, always the same channels
-    const int quads = G.channels / 4, rows = kScanThreads / quads, c4 = tid % quads * 4;
-    const int st = tid / quads < rows ? tid / quads : kRow;
-    const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
-    float bias[4];
+    const int64_t id0 = first_segment(a, s, begin), number = id - id0;
+    const int64_t start = begin + number * a.segment, stop = start + a.segment < end ? start + a.segment : end;
+    if (number < 0 || (number > 0 && start >= end)) return;
+    if (STATE && stop == end) return;         // nothing follows a last segment
+    // this lane's channels, their rates and the state entering
+    pair_t rate[NCH][2], h[NCH][2];
+    const int mine = warp * G.warp_channels + cl * NCH;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
+    for (int j = 0; j < NCH; ++j) {
+        const bool in = mine + j < count;
+        const int64_t c = c0 + (in ? mine + j : 0);
+        float A[4], v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        load_states(a.A + c * a.state, first, a.state, A);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) A[i] = scan_rate(A[i]);
+        if (!STATE) {
+            if (a.initial) load_states(a.initial + (s * a.channels + c) * a.state, first, a.state, v);
+            for (int64_t k = id0; k < id; ++k) {
+                const float total = a.totals[k * a.channels + c];
+                float e[4];
+                load_states(a.ends + (k * a.channels + c) * a.state, first, a.state, e);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = decay(total, A[i]) * v[i] + e[i];
+            }
+        }
+        rate[j][0] = pack(A[0], A[1]);
+        rate[j][1] = pack(A[2], A[3]);
+        h[j][0] = pack(v[0], v[1]);
+        h[j][1] = pack(v[2], v[3]);
+    }
+    auto keep = [&](float* to, int j) {        // the states of channel j
+        float v[4];
+        unpack(h[j][0], v[0], v[1]);
+        unpack(h[j][1], v[2], v[3]);
+        if (mine + j >= count) return;
+        to += (c0 + mine + j) * a.state + first;
+        if (FULL && a.vec_params) {
+            *reinterpret_cast<float4*>(to) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) if (first + i < a.state) to[i] = v[i];
+        }
+    };
+    // staging: four channels of a token per thread, always the same channels
+    const int c4 = tid % quads * 4, st = tid / quads;
+    const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
+    float bias[4], skip[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        bias[i] = a.bias && i < left ? a.bias[c0 + c4 + i] : 0.0f;
+        skip[i] = a.skip && i < left ? a.skip[c0 + c4 + i] : 0.0f;
+    }
     const int64_t chunk0 = first_chunk(a.tok, s, begin), stride = (int64_t)a.groups * a.state;
     T* raw = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.raw);
-    T* couplings = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.couplings);
-    const int cells = kRow * G.channels;
-    // a tile's operands on their way while the one before it is worked on
+    T* couplings = raw + 6 * kRow * G.channels;
+    constexpr int cells = kRow * G.channels;
+    const bool gate = !STATE && a.z;
     auto copy_tile = [&](int64_t from, int buffer) {
-        for (int t = st; t < kRow; t += rows) {
-            const int n = from + t < end ? left : 0, to = t * G.channels + c4;
-            const int64_t at = (from + t) * a.channels + c0 + c4;
-            copy4(raw + to, (const T*)a.x + at, a.vec, n);
-            copy4(raw + cells + to, (const T*)a.delta + at, a.vec, n);
-            if (GATE) copy4(raw + 2 * cells + to, (const T*)a.z + at, a.vec, n);
+        T* to = raw + buffer * 3 * cells + st * G.channels + c4;
+        int64_t at = (from + st) * a.channels + c0 + c4;
+#pragma unroll 2
+        for (int t = st; t < kRow; t += kPass) {
+            const int n = from + t < stop ? left : 0;
+            copy4(to, (const T*)a.x + at, a.vec, n);
+            copy4(to + cells, (const T*)a.delta + at, a.vec, n);
+            if (gate) copy4(to + 2 * cells, (const T*)a.z + at, a.vec, n);
+            to += kPass * G.channels;
+            at += kPass * a.channels;
         }
-        for (int i = tid; i < kRow * (G.pad / 4); i += kScanThreads) {
-            const int t = i / (G.pad / 4), n4 = i % (G.pad / 4) * 4;
-            int n = from + t < end ? a.state - n4 : 0;
+#pragma unroll 2
+        for (int i = tid; i < kRow * LN; i += kScanThreads) {
+            const int t = i / LN, n4 = i % LN * 4;
+            int n = from + t < stop ? a.state - n4 : 0;
             n = n < 0 ? 0 : n > 4 ? 4 : n;
             const int64_t at = (from + t) * stride + group * a.state + n4;
-            T* to = couplings + (buffer * 2 * kRow + t) * G.pitch + n4;
-            copy4(to, (const T*)a.B + at, a.vec_states, n);
-            copy4(to + kRow * G.pitch, (const T*)a.C + at, a.vec_states, n);
+            copy4(couplings + 4 * i, (const T*)a.B + at, a.vec_states, n);
+            if (!STATE) copy4(couplings + kRow * G.pad + 4 * i, (const T*)a.C + at, a.vec_states, n);
         }
         copies_commit();
     };
-    if (begin < end) copy_tile(begin, 0);
+    float total[NCH] = {};
+    if (start < stop) copy_tile(start, 0);
     int buffer = 0;
-    for (int64_t from = begin; from < end; from += kRow, buffer ^= 1) {
+    for (int64_t from = start; from < stop; from += kRow, buffer ^= 1) {
+        const int tokens = (int)(stop - from < kRow ? stop - from : kRow);
         copies_wait();
         // (each thread reads back what it has fetched itself)
-        for (int t = st; t < kRow; t += rows) {
-            const int n = from + t < end ? left : 0, to = t * G.channels + c4, row = place(c4, t);
-            const Raw4<T> rx = raw4(raw + to), rd = raw4(raw + cells + to);
-            Raw4<T> rz;
-            if (GATE) rz = raw4(raw + 2 * cells + to);
+        const T* got = raw + buffer * 3 * cells + st * G.channels + c4;
+        for (int t = st; t < kRow; t += kPass, got += kPass * G.channels) {
+            const Raw4<T> rx = raw4(got), rd = raw4(got + cells);
+            float2 v[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float d = load1(&rd.e[i]) + bias[i];
                 if (a.softplus) d = softplus_(d);
-                sX[row + i * kRow] = load1(&rx.e[i]);
-                sD[row + i * kRow] = i < n ? d : 0.0f;
-                if (GATE) {
-                    const float z = load1(&rz.e[i]);
-                    sZ[row + i * kRow] = z * sigmoid_(z);
-                }
+                v[i] = make_float2(d, d * load1(&rx.e[i]));
+            }
+            float4* to = reinterpret_cast<float4*>(smem + G.du + 2 * (t * G.channels + c4));
+            to[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+            to[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        }
+        for (int i = tid; i < kRow * LN; i += kScanThreads) {
+            const Raw4<T> b = raw4(couplings + 4 * i);
+            reinterpret_cast<float4*>(smem + G.B)[i] = make_float4(load1(&b.e[0]), load1(&b.e[1]), load1(&b.e[2]), load1(&b.e[3]));
+            if (!STATE) {
+                const Raw4<T> c = raw4(couplings + kRow * G.pad + 4 * i);
+                reinterpret_cast<float4*>(smem + G.C)[i] = make_float4(load1(&c.e[0]), load1(&c.e[1]), load1(&c.e[2]), load1(&c.e[3]));
             }
         }
-        if (from + kRow < end) copy_tile(from + kRow, buffer ^ 1);
-        __syncthreads();
-        for (int q = 0; q < G.slices; ++q) {
-            const int first = q * kWide + sub * 4;
-            // (FULL: all of a slice's states exist; else those beyond the last one stay zero whatever the input is)
-            pair_t B[K][2], C[K][2];
+        if (from + kRow < stop) copy_tile(from + kRow, buffer ^ 1);
+        if (!STATE && a.carries) {
+            float* to = a.carries + (chunk0 + (from - begin) / PD_SCAN_CHUNK) * a.channels * a.state;
 #pragma unroll
-            for (int i = 0; i < K; ++i) {
-                const T* from_row = couplings + (buffer * 2 * kRow + tl * K + i) * G.pitch + first;
-                const Raw4<T> b = raw4(from_row), c = raw4(from_row + kRow * G.pitch);
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    B[i][p] = pack(load1(&b.e[2 * p]), load1(&b.e[2 * p + 1]));
-                    C[i][p] = pack(load1(&c.e[2 * p]), load1(&c.e[2 * p + 1]));
-                }
-            }
-            for (int cc = 0; cc < a.per_warp; ++cc) {
-                const int c = warp * a.per_warp + cc;
-                if (c >= count) break;
-                float* kept = smem + G.carry + c * G.pad + first;
-                const float* rates = smem + G.rate + c * G.pad + first;
-                pair_t entry[2], rate[2], w[K][2], h[2], span[2];
-                entry[0] = reinterpret_cast<const pair_t*>(kept)[0];
-                entry[1] = reinterpret_cast<const pair_t*>(kept)[1];
-                rate[0] = reinterpret_cast<const pair_t*>(rates)[0];
-                rate[1] = reinterpret_cast<const pair_t*>(rates)[1];
-                float u[K];
-                {
-                    float x[K], d[K];
-#pragma unroll
-                    for (int i = 0; i < K; i += kPart) {
-                        load_steps<kPart>(sX + place(c, tl * K + i), reinterpret_cast<float(&)[kPart]>(x[i]));
-                        load_steps<kPart>(sD + place(c, tl * K + i), reinterpret_cast<float(&)[kPart]>(d[i]));
-                    }
-                    // from a zero state, and the decay over this lane's tokens
-#pragma unroll
-                    for (int i = 0; i < K; ++i) {
-                        const pair_t step = pack(d[i], d[i]);
-                        u[i] = d[i] * x[i];
-                        const pair_t uu = pack(u[i], u[i]);
-#pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            w[i][p] = decay2(step, rate[p]);
-                            const pair_t b = mul2(uu, B[i][p]);
-                            h[p] = i == 0 ? b : mad2(w[i][p], h[p], b);
-                            span[p] = i == 0 ? w[i][p] : mul2(span[p], w[i][p]);
-                        }
-                    }
-                }
-                // over the token groups.  The first one takes in the carried state; its decay then counts as zero,
-                // so that a group that has seen everything before it adds nothing more (a shuffle from beyond the
-                // edge returns the lane's own value).
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    h[p] = mad2(span[p], tl == 0 ? entry[p] : 0, h[p]);
-                    span[p] = tl == 0 ? 0 : span[p];
-                }
-#pragma unroll
-                for (int off = 1; off < TL; off *= 2)
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        h[p] = mad2(span[p], shift_up(h[p], off * LN), h[p]);
-                        if (2 * off < TL) span[p] = mul2(span[p], shift_up(span[p], off * LN));
-                    }
-                __syncwarp();
-                if (tl == TL - 1) {
-                    reinterpret_cast<pair_t*>(kept)[0] = FULL ? h[0] : keep_states(h[0], a.state - first);
-                    reinterpret_cast<pair_t*>(kept)[1] = FULL ? h[1] : keep_states(h[1], a.state - first - 2);
-                }
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    h[p] = shift_up(h[p], LN);
-                    h[p] = tl == 0 ? entry[p] : h[p];
-                }
-                if (a.carries && tl * K % PD_SCAN_CHUNK == 0 && from + tl * K < end) {
-                    float v[4];
-                    unpack(h[0], v[0], v[1]);
-                    unpack(h[1], v[2], v[3]);
-                    float* to = a.carries + ((chunk0 + (from - begin + tl * K) / PD_SCAN_CHUNK) * a.channels + c0 + c) * a.state;
-                    if (FULL && a.vec_params) {
-                        *reinterpret_cast<float4*>(to + first) = make_float4(v[0], v[1], v[2], v[3]);
-                    } else {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) if (first + i < a.state) to[first + i] = v[i];
-                    }
-                }
-                // from the true state
-                float y[K];
-#pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    const pair_t uu = pack(u[i], u[i]);
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) h[p] = mad2(w[i][p], h[p], mul2(uu, B[i][p]));
-                    const pair_t low = FULL ? h[0] : keep_states(h[0], a.state - first);
-                    const pair_t high = FULL ? h[1] : keep_states(h[1], a.state - first - 2);
-                    y[i] = halves(mad2(C[i][1], high, mul2(C[i][0], low)));
-                }
-                // a token's sum over its lanes; each lane finishes two tokens
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    float part[LN];
-#pragma unroll
-                    for (int j = 0; j < LN; ++j) part[j] = y[i * LN + j];
-                    float v = sum_to_lane<LN>(part, sub);
-                    const int at = place(c, tl * K + i * LN + sub);
-                    if (G.slices > 1) {
-                        if (q > 0) v += smem[G.y + at];
-                        smem[G.y + at] = v;
-                    }
-                    if (q == G.slices - 1) {
-                        __syncwarp();     // the tile's inputs of this channel give way to its outputs
-                        v += smem[G.skip + c] * sX[at];
-                        sX[at] = GATE ? v * sZ[at] : v;
-                    }
-                }
-            }
+            for (int j = 0; j < NCH; ++j) keep(to, j);
         }
         __syncthreads();
-        for (int t = st; t < kRow; t += rows) {
-            const int n = from + t < end ? left : 0, row = place(c4, t);
-            float v[4];
+        const float* du = smem + G.du + 2 * mine;
+        float* out = smem + G.y + warp * kRow * 32 * NCH + sub * G.warp_channels + cl * NCH;
+        float sums[NCH] = {};
+        auto token = [&](int t) {
+            float d[NCH], u[NCH], y[NCH];
+            if constexpr (NCH == 2) {
+                const float4 q = *reinterpret_cast<const float4*>(du + 2 * t * G.channels);
+                d[0] = q.x; u[0] = q.y; d[1] = q.z; u[1] = q.w;
+            } else {
+                const float2 q = *reinterpret_cast<const float2*>(du + 2 * t * G.channels);
+                d[0] = q.x; u[0] = q.y;
+            }
+            const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(smem + G.B + t * G.pad + first);
+            ulonglong2 C;
+            if (!STATE) C = *reinterpret_cast<const ulonglong2*>(smem + G.C + t * G.pad + first);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = sX[row + i * kRow];
-            put4((T*)a.y + (from + t) * a.channels + c0 + c4, a.vec, n, v);
+            for (int j = 0; j < NCH; ++j) {
+                const pair_t step = pack(d[j], d[j]), in = pack(u[j], u[j]);
+                pair_t b0 = mul2(in, B.x), b1 = mul2(in, B.y);
+                if (!FULL) {     // states beyond the last one stay zero whatever the input is
+                    b0 = keep_states(b0, a.state - first);
+                    b1 = keep_states(b1, a.state - first - 2);
+                }
+                h[j][0] = mad2(decay2(step, rate[j][0]), h[j][0], b0);
+                h[j][1] = mad2(decay2(step, rate[j][1]), h[j][1], b1);
+                if (STATE) sums[j] += d[j];
+                else y[j] = halves(mad2(C.y, h[j][1], mul2(C.x, h[j][0])));
+            }
+            if (!STATE) {
+                if constexpr (NCH == 2) *reinterpret_cast<float2*>(out + t * 32 * NCH) = make_float2(y[0], y[1]);
+                else out[t * 32 * NCH] = y[0];
+            }
+        };
+        if (tokens == kRow) {
+#pragma unroll 8
+            for (int t = 0; t < kRow; ++t) token(t);
+        } else {
+            for (int t = 0; t < tokens; ++t) token(t);
         }
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) total[j] += sums[j];
         __syncthreads();
+        if (!STATE) {
+            // an output's LN partial sums, the skip and the gate
+            got = raw + buffer * 3 * cells + st * G.channels + c4;
+            const float* sum = smem + G.y + c4 / G.warp_channels * kRow * 32 * NCH + c4 % G.warp_channels;
+            T* to = (T*)a.y + (from + st) * a.channels + c0 + c4;
+            for (int t = st; t < tokens; t += kPass, got += kPass * G.channels, to += kPass * a.channels) {
+                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                const Raw4<T> rx = raw4(got);
+#pragma unroll
+                for (int k = 0; k < LN; ++k) {
+                    const float4 q = *reinterpret_cast<const float4*>(sum + t * 32 * NCH + k * G.warp_channels);
+                    v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += skip[i] * load1(&rx.e[i]);
+                if (gate) {
+                    const Raw4<T> rz = raw4(got + 2 * cells);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float z = load1(&rz.e[i]);
+                        v[i] *= z * sigmoid_(z);
+                    }
+                }
+                put4(to, a.vec, left, v);
+            }
+        }
     }
-    if (a.final_state) {
-        __syncthreads();
-        for (int i = tid; i < count * G.pad; i += kScanThreads)
-            if (i % G.pad < a.state) a.final_state[(s * a.channels + c0 + i / G.pad) * a.state + i % G.pad] = smem[G.carry + i];
+    if (STATE) {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) {
+            keep(a.ends + id * a.channels * a.state, j);
+            if (sub == 0 && mine + j < count) a.totals[id * a.channels + c0 + mine + j] = total[j];
+        }
+    } else if (a.final_state && stop == end) {
+#pragma unroll
+        for (int j = 0; j < NCH; ++j) keep(a.final_state + s * a.channels * a.state, j);
     }
 }
 
@@ -1557,21 +1566,38 @@ cudaError_t launch_conv_grad(const PdConvArgs& a, cudaStream_t st) {
 cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
     return by_type(a.type, [&](auto e) {
         using T = decltype(e);
-        auto run = [&](auto ln) -> cudaError_t {
+        return by_lanes(a.state, [&](auto ln) -> cudaError_t {
             constexpr int LN = decltype(ln)::value;
-            const ScanShape G(LN, a.state, a.per_warp, sizeof(T));
-            const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels * a.groups;
-            const int64_t blocks = tiles * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
-            if (blocks == 0) return cudaSuccess;
-            const bool full = a.state % (4 * LN) == 0;
-            auto kernel = a.z ? (full ? pd_selective_scan_kernel<T, LN, true, true> : pd_selective_scan_kernel<T, LN, true, false>)
-                              : (full ? pd_selective_scan_kernel<T, LN, false, true> : pd_selective_scan_kernel<T, LN, false, false>);
-            cudaError_t err = allow_smem(kernel, G.bytes);
-            if (err != cudaSuccess) return err;
-            kernel<<<(unsigned)blocks, kScanThreads, G.bytes, st>>>(a);
-            return cudaGetLastError();
-        };
-        return a.state <= 4 ? run(Int<1>()) : a.state <= 8 ? run(Int<2>()) : run(Int<4>());
+            const bool full = a.state == 4 * LN;
+            auto run = [&](auto nch) -> cudaError_t {
+                constexpr int NCH = decltype(nch)::value;
+                constexpr ScanShape G(LN, NCH, sizeof(T));
+                const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels * a.groups;
+                if (a.ends && a.segments > 0) {
+                    auto first = full ? pd_selective_scan_kernel<T, LN, NCH, true, true> : pd_selective_scan_kernel<T, LN, NCH, false, true>;
+                    cudaError_t err = allow_smem(first, G.bytes);
+                    if (err != cudaSuccess) return err;
+                    first<<<(unsigned)(tiles * a.segments), kScanThreads, G.bytes, st>>>(a);
+                    err = cudaGetLastError();
+                    if (err != cudaSuccess) return err;
+                }
+                const int64_t blocks = tiles * (a.segments + (a.tok.offsets ? 1 : 0));
+                if (blocks == 0) return cudaSuccess;
+                auto kernel = full ? pd_selective_scan_kernel<T, LN, NCH, true, false> : pd_selective_scan_kernel<T, LN, NCH, false, false>;
+                cudaError_t err = allow_smem(kernel, G.bytes);
+                if (err != cudaSuccess) return err;
+                kernel<<<(unsigned)blocks, kScanThreads, G.bytes, st>>>(a);
+                return cudaGetLastError();
+            };
+            if constexpr (LN == 16) {
+                return run(Int<2>());      // (one channel per lane would leave a warp two)
+            } else {
+                if constexpr (LN >= 4) {
+                    if (a.per_warp == 2) return run(Int<2>());
+                }
+                return run(Int<1>());
+            }
+        });
     });
 }
 cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {

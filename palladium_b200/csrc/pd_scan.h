@@ -42,7 +42,7 @@ struct PdScanArgs {
     int vec_states;           // B and C four states at a time
     int vec_params;           // A and the states four at a time
     int run;                  // single tokens: sequences a block takes one after another
-    int per_warp;             // channels a warp takes one after another
+    int per_warp;             // gradient: channels a warp takes one after another; prompts: channels per lane
     int64_t channels;
     const void *x, *delta, *B, *C, *z, *dy;
     const float *A, *bias, *skip, *initial, *carries_in, *dfinal;
@@ -51,6 +51,10 @@ struct PdScanArgs {
     // gradient: sums over the channels of one tile, (tiles, rows, 2, states rounded up), and over the tokens of
     // one sequence, (seqs, channels, state + 2)
     float *partial_bc, *partial_params;
+    // prompts cut into segments of `segment` tokens (`segments` of them in all): their end states from zero,
+    // (segments, channels, state), and total steps, (segments, channels); null where no sequence is cut
+    int64_t segment, segments;
+    float *ends, *totals;
 };
 
 // Lanes that share one channel: each holds four states.
@@ -99,6 +103,7 @@ const PdScanTable* pd_scan_table_fast();
 struct PdScanPlan {
     const char* kernel_name = "";
     int64_t grid = 1, grid_y = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
+    int64_t segment = 1, segments = 0, totals_offset = 0;    // prompts: see PdScanArgs
     int64_t row_blocks = 0;       // gradient of the convolution: blocks along the rows
     int64_t params_offset = 0;    // gradient of the scan: where in the scratch the parameters' sums begin
     std::vector<size_t> in_bytes, out_bytes;

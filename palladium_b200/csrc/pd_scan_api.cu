@@ -81,11 +81,10 @@ int64_t conv_partial(const Dims& d, int64_t width, int64_t row_blocks) { return 
 int64_t scan_chunks(const pd_selective_scan_params* p, const Dims& d) {
     return p->packed ? p->length / PD_SCAN_CHUNK + d.seqs : d.seqs * ((p->length + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK);
 }
-// Channels a warp takes one after another (a block is four warps; four blocks an SM for prompts, three for
-// gradients).  More of them share the fetched B and C and, in the gradient, one sum over the block's warps and one
-// partial sum of dB and dC in memory, worth about one channel's work per tile; fewer give more blocks.  The
-// smallest product of waves and work per wave wins.
-int scan_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms, bool grad) {
+// Channels a warp of the gradient kernel takes one after another (a block is four warps, three blocks an SM).
+// More of them share one sum over the block's warps and one partial sum of dB and dC in memory, worth about one
+// channel's work per chunk; fewer give more blocks.  The smallest product of waves and work per wave wins.
+int grad_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
     const int64_t per = d.channels / p->groups, slots = (int64_t)sms * 3;
     const int most = p->state > 16 ? 4 : 8;    // (slices of sixteen states need shared memory for as many sums)
     int best = 1;
@@ -97,8 +96,38 @@ int scan_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms, boo
     }
     return best;
 }
+int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lane) {
+    const int64_t per = d.channels / p->groups, ch = 2 * 32 / pd_scan_lanes((int)p->state) * per_lane;
+    return (per + ch - 1) / ch * p->groups;
+}
+// The prompt kernel's channels per lane and segments.  Two channels per lane halve the reads of B and C; one gives
+// twice the blocks.  A call of fewer blocks than SMs is cut into segments, which costs a first pass over all but
+// the last of a sequence (some 60 % of the second), so that about four warps per scheduler work; so are packed
+// calls, where one long sequence would outlast all others, at twice a block's share.
+void scan_cut(const pd_selective_scan_params* p, const Dims& d, int sms, PdScanPlan* plan) {
+    const int64_t rows = d.rows > 0 ? d.rows : 1;
+    int64_t blocks = scan_tiles(p, d, 2) * (d.seqs > 0 ? d.seqs : 1);
+    int per_lane = p->state > 32 || (p->state > 8 && blocks >= (int64_t)sms * 2) ? 2 : 1;
+    const int64_t mean = d.seqs > 0 ? (rows + d.seqs - 1) / d.seqs : rows;
+    int64_t segment = INT32_MAX;
+    blocks = scan_tiles(p, d, per_lane) * (d.seqs > 0 ? d.seqs : 1);
+    if (blocks < sms && mean >= 512) {
+        per_lane = p->state > 8 ? 2 : 1;
+        segment = rows * scan_tiles(p, d, per_lane) / ((int64_t)sms * 8);
+        if (segment < 256) segment = 256;
+    } else if (p->packed && d.seqs > 1) {
+        segment = 2 * rows * scan_tiles(p, d, per_lane) / ((int64_t)sms * 4);
+        if (segment < 512) segment = 512;
+    }
+    segment = (segment + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK * PD_SCAN_CHUNK;     // (carries are kept at whole chunks)
+    plan->items = per_lane;
+    plan->segment = segment;
+    if (p->packed) plan->segments = d.rows / segment + d.seqs;
+    else plan->segments = d.seqs * (p->length > 0 ? (p->length + segment - 1) / segment : 1);
+}
+
 int64_t scan_partial_bc(const pd_selective_scan_params* p, const Dims& d, int sms) {
-    const int64_t per = d.channels / p->groups, ch = 4 * scan_per_warp(p, d, sms, true);
+    const int64_t per = d.channels / p->groups, ch = 4 * grad_per_warp(p, d, sms);
     return align256((per + ch - 1) / ch * p->groups * d.rows * 2 * pd_scan_pad((int)p->state) * 4);
 }
 
@@ -194,12 +223,24 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         plan->block = 32 * pd_step_warps(d.channels, (int)p->groups, (int)p->state, d.seqs);
         return PD_OK;
     }
-    // one block per tile of channels and sequence
-    const int64_t per = d.channels / p->groups;
-    const int per_warp = scan_per_warp(p, d, sms, grad);
-    const int64_t ch = 4 * per_warp;
-    plan->grid = (per + ch - 1) / ch * p->groups * (d.seqs + free_rows);
-    plan->items = per_warp;
+    if (grad) {
+        // one block per tile of channels and sequence
+        const int64_t per = d.channels / p->groups;
+        plan->items = grad_per_warp(p, d, sms);
+        plan->grid = (per + 4 * plan->items - 1) / (4 * plan->items) * p->groups * (d.seqs + free_rows);
+    } else {
+        scan_cut(p, d, sms, plan);
+        plan->grid = scan_tiles(p, d, (int)plan->items) * (plan->segments + free_rows);
+        plan->block = 64;
+        if (d.rows > plan->segment) {
+            // (a dense call is cut only where a sequence is longer than a segment)
+            if (p->packed || p->length > plan->segment) {
+                plan->totals_offset = align256(plan->segments * d.channels * p->state * 4);
+                plan->scratch_bytes = plan->totals_offset + plan->segments * d.channels * 4;
+                plan->launches = 2;
+            }
+        }
+    }
     if (grad) {
         in.push_back(carries);
         if (p->final) in.push_back(edge);
@@ -321,6 +362,12 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
             a.partial_bc = (float*)scratch;
             a.partial_params = (float*)((char*)scratch + plan.params_offset);
         } else {
+            a.segment = plan.segment;
+            a.segments = plan.segments;
+            if (!step && plan.scratch_bytes > 0) {
+                a.ends = (float*)scratch;
+                a.totals = (float*)((char*)scratch + plan.totals_offset);
+            }
             if (!step && p->initial) a.initial = (const float*)in[i++];
             a.y = out[o++];
             if (step || p->final) a.final_state = (float*)out[o++];
@@ -333,7 +380,8 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % four) a.vec = 0;
         a.vec_states = a.state % 4 == 0 && reinterpret_cast<uintptr_t>(a.B) % four == 0 && reinterpret_cast<uintptr_t>(a.C) % four == 0;
         a.per_warp = a.run = (int)plan.items;
-        a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries) && aligned16(a.final_state);
+        a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries) && aligned16(a.final_state) &&
+                       aligned16(a.ends);
         e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
     }
     if (e != cudaSuccess) {
