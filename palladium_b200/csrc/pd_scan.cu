@@ -15,6 +15,11 @@
 
 #include "../../include/palladium_cuda.h"
 
+#ifndef SC_F
+#define SC_F 4
+#define SC_U "unroll 1"
+#define SC_B 8
+#endif
 #ifndef PD_MODE
 #error "PD_MODE must be 0 (SAFE), 1 (RELAXED) or 2 (FAST)"
 #endif
@@ -827,8 +832,7 @@ __device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
 // ---------------------------------------------------------------------------
 // The prompt kernel.  A lane holds four states of NCH neighbouring channels and walks the tokens one by one; LN
 // lanes share a channel, 32 / LN * NCH channels make a warp's, two warps a block.  A tile of 32 tokens is staged in
-// shared memory as float32 (step lengths, inputs, couplings), the next one's elements on their way meanwhile, and
-// the LN partial sums of each output meet there too.
+// shared memory as float32 (step lengths, inputs, couplings), the next one's elements on their way meanwhile.
 //
 // Bound: the exponentials, one per (token, channel, state), 16 per clock and SM: 8 cycles per warp instruction and
 // scheduler.  Beside each stand 2 packed multiply-adds and, with two channels per lane, 1.75 words of shared memory
@@ -845,7 +849,7 @@ struct ScanShape {
     static constexpr int kRow = PD_SCAN_CHUNK;
     __host__ __device__ constexpr ScanShape(int ln, int nch, int element)
         : warp_channels(32 / ln * nch), channels(kScanWarps * warp_channels), pad(4 * ln), du(0),
-          B(2 * kRow * channels), C(B + kRow * pad), y(C + kRow * pad), raw((y + kScanWarps * kRow * 32 * nch) * 4),
+          B(2 * kRow * channels), C(B + kRow * pad), y(C + kRow * pad), raw((y + kRow * channels) * 4),
           // two buffers of x, delta, z: (3, tokens, channels), and one of B and C: (2, tokens, pad)
           bytes(raw + 6 * kRow * channels * element + 2 * kRow * pad * element) {}
 };
@@ -868,7 +872,7 @@ __device__ __forceinline__ int64_t segment_owner(const PdScanArgs& a, int64_t id
 }
 
 template <class T, int LN, int NCH, bool FULL, bool STATE>
-__global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, SC_B) pd_selective_scan_kernel(PdScanArgs a) {
     constexpr ScanShape G(LN, NCH, sizeof(T));
     constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kScanThreads / quads;
     static_assert(kScanThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");
@@ -985,11 +989,15 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
             for (int i = 0; i < 4; ++i) {
                 float d = load1(&rd.e[i]) + bias[i];
                 if (a.softplus) d = softplus_(d);
+                d = t < tokens ? d : 0.0f;
                 v[i] = make_float2(d, d * load1(&rx.e[i]));
             }
+            // (every other four threads store their second half first: no two of eight meet in a bank)
             float4* to = reinterpret_cast<float4*>(smem + G.du + 2 * (t * G.channels + c4));
-            to[0] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-            to[1] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+            const float4 low = make_float4(v[0].x, v[0].y, v[1].x, v[1].y), high = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+            const int turn = lane >> 2 & 1;
+            to[turn] = turn ? high : low;
+            to[turn ^ 1] = turn ? low : high;
         }
         for (int i = tid; i < kRow * LN; i += kScanThreads) {
             const Raw4<T> b = raw4(couplings + 4 * i);
@@ -1007,60 +1015,92 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
         }
         __syncthreads();
         const float* du = smem + G.du + 2 * mine;
-        float* out = smem + G.y + warp * kRow * 32 * NCH + sub * G.warp_channels + cl * NCH;
+        float* out = smem + G.y + warp * kRow * G.warp_channels + cl * NCH;     // (warp, token, channel)
         float sums[NCH] = {};
-        auto token = [&](int t) {
-            float d[NCH], u[NCH], y[NCH];
-            if constexpr (NCH == 2) {
-                const float4 q = *reinterpret_cast<const float4*>(du + 2 * t * G.channels);
-                d[0] = q.x; u[0] = q.y; d[1] = q.z; u[1] = q.w;
-            } else {
-                const float2 q = *reinterpret_cast<const float2*>(du + 2 * t * G.channels);
-                d[0] = q.x; u[0] = q.y;
-            }
-            const ulonglong2 B = *reinterpret_cast<const ulonglong2*>(smem + G.B + t * G.pad + first);
-            ulonglong2 C;
-            if (!STATE) C = *reinterpret_cast<const ulonglong2*>(smem + G.C + t * G.pad + first);
+        // Four tokens at a time: their operands are read before the outputs of the four before them are stored (the
+        // compiler would not move a read of shared memory past a store to it), so that sixteen exponentials are
+        // under way at once.
+        constexpr int F = SC_F;
+        struct Operands { float d[F][NCH], u[F][NCH]; ulonglong2 B[F], C[F]; };
+        auto fetch_tokens = [&](int t, Operands& q) {
 #pragma unroll
-            for (int j = 0; j < NCH; ++j) {
-                const pair_t step = pack(d[j], d[j]), in = pack(u[j], u[j]);
-                pair_t b0 = mul2(in, B.x), b1 = mul2(in, B.y);
-                if (!FULL) {     // states beyond the last one stay zero whatever the input is
-                    b0 = keep_states(b0, a.state - first);
-                    b1 = keep_states(b1, a.state - first - 2);
+            for (int i = 0; i < F; ++i) {
+                if constexpr (NCH == 2) {
+                    const float4 v = *reinterpret_cast<const float4*>(du + 2 * (t + i) * G.channels);
+                    q.d[i][0] = v.x; q.u[i][0] = v.y; q.d[i][NCH - 1] = v.z; q.u[i][NCH - 1] = v.w;
+                } else {
+                    const float2 v = *reinterpret_cast<const float2*>(du + 2 * (t + i) * G.channels);
+                    q.d[i][0] = v.x; q.u[i][0] = v.y;
                 }
-                h[j][0] = mad2(decay2(step, rate[j][0]), h[j][0], b0);
-                h[j][1] = mad2(decay2(step, rate[j][1]), h[j][1], b1);
-                if (STATE) sums[j] += d[j];
-                else y[j] = halves(mad2(C.y, h[j][1], mul2(C.x, h[j][0])));
-            }
-            if (!STATE) {
-                if constexpr (NCH == 2) *reinterpret_cast<float2*>(out + t * 32 * NCH) = make_float2(y[0], y[1]);
-                else out[t * 32 * NCH] = y[0];
+                q.B[i] = *reinterpret_cast<const ulonglong2*>(smem + G.B + (t + i) * G.pad + first);
+                if (!STATE) q.C[i] = *reinterpret_cast<const ulonglong2*>(smem + G.C + (t + i) * G.pad + first);
             }
         };
-        if (tokens == kRow) {
-#pragma unroll 8
-            for (int t = 0; t < kRow; ++t) token(t);
-        } else {
-            for (int t = 0; t < tokens; ++t) token(t);
+        Operands q;
+        fetch_tokens(0, q);
+_Pragma(SC_U)
+        for (int t = 0; t < kRow; t += F) {
+            // (tokens behind the segment's end have steps and inputs of zero)
+            pair_t w[F][NCH][2], b[F][NCH][2];
+            float y[F][NCH];
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < NCH; ++j) {
+                    const pair_t step = pack(q.d[i][j], q.d[i][j]), in = pack(q.u[i][j], q.u[i][j]);
+                    w[i][j][0] = decay2(step, rate[j][0]);
+                    w[i][j][1] = decay2(step, rate[j][1]);
+                    b[i][j][0] = mul2(in, q.B[i].x);
+                    b[i][j][1] = mul2(in, q.B[i].y);
+                    if (!FULL) {     // states beyond the last one stay zero whatever the input is
+                        b[i][j][0] = keep_states(b[i][j][0], a.state - first);
+                        b[i][j][1] = keep_states(b[i][j][1], a.state - first - 2);
+                    }
+                    if (STATE) sums[j] += q.d[i][j];
+                }
+#pragma unroll
+            for (int i = 0; i < F; ++i)
+#pragma unroll
+                for (int j = 0; j < NCH; ++j) {
+                    h[j][0] = mad2(w[i][j][0], h[j][0], b[i][j][0]);
+                    h[j][1] = mad2(w[i][j][1], h[j][1], b[i][j][1]);
+                    if (!STATE) y[i][j] = halves(mad2(q.C[i].y, h[j][1], mul2(q.C[i].x, h[j][0])));
+                }
+            if (t + F < kRow) fetch_tokens(t + F, q);
+            if (!STATE)
+#pragma unroll
+                for (int i = 0; i < F; i += (LN < 4 ? LN : 4)) {
+                    // an output's sum over its lanes; lane k keeps the k-th of LN (at most four) tokens
+                    float v[NCH];
+#pragma unroll
+                    for (int j = 0; j < NCH; ++j) {
+                        constexpr int K = LN < 4 ? LN : 4;
+                        float part[K];
+#pragma unroll
+                        for (int k = 0; k < K; ++k) part[k] = y[i + k][j];
+                        v[j] = sum_to_lane<K>(part, sub);
+#pragma unroll
+                        for (int m = 4; m < LN; m *= 2) v[j] += __shfl_xor_sync(kFull, v[j], m);
+                    }
+                    if (LN <= 4 || sub < 4) {
+                        float* to = out + (t + i + (LN > 1 ? sub : 0)) * G.warp_channels;
+                        if constexpr (NCH == 2) *reinterpret_cast<float2*>(to) = make_float2(v[0], v[NCH - 1]);
+                        else to[0] = v[0];
+                    }
+                }
         }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) total[j] += sums[j];
         __syncthreads();
         if (!STATE) {
-            // an output's LN partial sums, the skip and the gate
+            // the skip and the gate
             got = raw + buffer * 3 * cells + st * G.channels + c4;
-            const float* sum = smem + G.y + c4 / G.warp_channels * kRow * 32 * NCH + c4 % G.warp_channels;
+            const float* sum = smem + G.y + c4 / G.warp_channels * kRow * G.warp_channels + c4 % G.warp_channels;
             T* to = (T*)a.y + (from + st) * a.channels + c0 + c4;
             for (int t = st; t < tokens; t += kPass, got += kPass * G.channels, to += kPass * a.channels) {
-                float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
                 const Raw4<T> rx = raw4(got);
-#pragma unroll
-                for (int k = 0; k < LN; ++k) {
-                    const float4 q = *reinterpret_cast<const float4*>(sum + t * 32 * NCH + k * G.warp_channels);
-                    v[0] += q.x; v[1] += q.y; v[2] += q.z; v[3] += q.w;
-                }
+                const float4 q = *reinterpret_cast<const float4*>(sum + t * G.warp_channels);
+                float v[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v[i] += skip[i] * load1(&rx.e[i]);
                 if (gate) {

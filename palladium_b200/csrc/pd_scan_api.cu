@@ -101,29 +101,30 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lan
     return (per + ch - 1) / ch * p->groups;
 }
 // The prompt kernel's channels per lane and segments.  Two channels per lane halve the reads of B and C; one gives
-// twice the blocks.  A call of fewer blocks than SMs is cut into segments, which costs a first pass over all but
-// the last of a sequence (some 60 % of the second), so that about four warps per scheduler work; so are packed
-// calls, where one long sequence would outlast all others, at twice a block's share.
+// twice the blocks, for calls that do not fill the GPU otherwise.  Eight blocks of two warps run on an SM, four warps
+// on a scheduler; fewer leave it waiting (1.7 warps issue 0.36 instructions a clock, four about twice that), so
+// a call that leaves room for it is cut into segments, of at least 64 tokens, until the blocks are one wave:
+// that costs a first pass over all but the last segment of a sequence.  A packed call is cut at an even share,
+// so that one long sequence does not outlast all others.
 void scan_cut(const pd_selective_scan_params* p, const Dims& d, int sms, PdScanPlan* plan) {
-    const int64_t rows = d.rows > 0 ? d.rows : 1;
-    int64_t blocks = scan_tiles(p, d, 2) * (d.seqs > 0 ? d.seqs : 1);
-    int per_lane = p->state > 32 || (p->state > 8 && blocks >= (int64_t)sms * 2) ? 2 : 1;
-    const int64_t mean = d.seqs > 0 ? (rows + d.seqs - 1) / d.seqs : rows;
-    int64_t segment = INT32_MAX;
-    blocks = scan_tiles(p, d, per_lane) * (d.seqs > 0 ? d.seqs : 1);
-    if (blocks < sms && mean >= 512) {
-        per_lane = p->state > 8 ? 2 : 1;
-        segment = rows * scan_tiles(p, d, per_lane) / ((int64_t)sms * 8);
-        if (segment < 256) segment = 256;
-    } else if (p->packed && d.seqs > 1) {
-        segment = 2 * rows * scan_tiles(p, d, per_lane) / ((int64_t)sms * 4);
-        if (segment < 512) segment = 512;
+    const int64_t seqs = d.seqs > 0 ? d.seqs : 1, rows = d.rows > 0 ? d.rows : 1, mean = (rows + seqs - 1) / seqs;
+    const int64_t wave = (int64_t)sms * 8, most = mean / 64 > 0 ? mean / 64 : 1;
+    int per_lane = p->state > 32 ? 2 : 1;
+    if (p->state > 8 && scan_tiles(p, d, 2) * seqs * most >= wave / 2) per_lane = 2;
+    const int64_t tiles = scan_tiles(p, d, per_lane);
+    int64_t cuts = wave / (tiles * seqs), segment = INT32_MAX;
+    if (cuts > most) cuts = most;
+    if (p->packed) {
+        segment = rows * tiles / wave;
+        if (segment < 64) segment = 64;
+    } else if (cuts > 1) {
+        segment = (mean + cuts - 1) / cuts;
     }
     segment = (segment + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK * PD_SCAN_CHUNK;     // (carries are kept at whole chunks)
     plan->items = per_lane;
     plan->segment = segment;
     if (p->packed) plan->segments = d.rows / segment + d.seqs;
-    else plan->segments = d.seqs * (p->length > 0 ? (p->length + segment - 1) / segment : 1);
+    else plan->segments = d.seqs * (p->length > segment ? (p->length + segment - 1) / segment : 1);
 }
 
 int64_t scan_partial_bc(const pd_selective_scan_params* p, const Dims& d, int sms) {
