@@ -15,11 +15,6 @@
 
 #include "../../include/palladium_cuda.h"
 
-#ifndef SC_F
-#define SC_F 4
-#define SC_U "unroll 1"
-#define SC_B 8
-#endif
 #ifndef PD_MODE
 #error "PD_MODE must be 0 (SAFE), 1 (RELAXED) or 2 (FAST)"
 #endif
@@ -817,15 +812,16 @@ __device__ __forceinline__ pair_t keep_states(pair_t v, int n) {
     return pack(n > 0 ? x : 0.0f, n > 1 ? y : 0.0f);
 }
 template <int K>
-__device__ __forceinline__ void load_steps(const float* p, float (&v)[K]) {
-    if constexpr (K == 4) {
-        const float4 q = *reinterpret_cast<const float4*>(p);
-        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
-    } else if constexpr (K == 2) {
-        const float2 q = *reinterpret_cast<const float2*>(p);
-        v[0] = q.x; v[1] = q.y;
+__device__ __forceinline__ void load_pairs(const float2* p, pair_t (&v)[K]) {
+    if constexpr (K == 1) {
+        v[0] = *reinterpret_cast<const pair_t*>(p);
     } else {
-        v[0] = p[0];
+#pragma unroll
+        for (int i = 0; i < K; i += 2) {
+            const ulonglong2 q = *reinterpret_cast<const ulonglong2*>(p + i);
+            v[i] = q.x;
+            v[i + 1] = q.y;
+        }
     }
 }
 
@@ -872,7 +868,7 @@ __device__ __forceinline__ int64_t segment_owner(const PdScanArgs& a, int64_t id
 }
 
 template <class T, int LN, int NCH, bool FULL, bool STATE>
-__global__ void __launch_bounds__(kScanThreads, SC_B) pd_selective_scan_kernel(PdScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdScanArgs a) {
     constexpr ScanShape G(LN, NCH, sizeof(T));
     constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kScanThreads / quads;
     static_assert(kScanThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");
@@ -1020,7 +1016,7 @@ __global__ void __launch_bounds__(kScanThreads, SC_B) pd_selective_scan_kernel(P
         // Four tokens at a time: their operands are read before the outputs of the four before them are stored (the
         // compiler would not move a read of shared memory past a store to it), so that sixteen exponentials are
         // under way at once.
-        constexpr int F = SC_F;
+        constexpr int F = 4;
         struct Operands { float d[F][NCH], u[F][NCH]; ulonglong2 B[F], C[F]; };
         auto fetch_tokens = [&](int t, Operands& q) {
 #pragma unroll
@@ -1038,7 +1034,7 @@ __global__ void __launch_bounds__(kScanThreads, SC_B) pd_selective_scan_kernel(P
         };
         Operands q;
         fetch_tokens(0, q);
-_Pragma(SC_U)
+#pragma unroll 2
         for (int t = 0; t < kRow; t += F) {
             // (tokens behind the segment's end have steps and inputs of zero)
             pair_t w[F][NCH][2], b[F][NCH][2];
@@ -1140,27 +1136,29 @@ _Pragma(SC_U)
 // ---------------------------------------------------------------------------
 constexpr int kGradWarps = 4, kGradThreads = 32 * kGradWarps;
 
+// (ONE: all states in one slice, and with it all but the channels known when compiling)
+template <int LN, bool ONE>
 struct GradShape {
-    int channels, pad, slices;    // channels per block, states rounded up, slices of 4 LN states
+    int channels, slices, pad;    // channels per block, slices of 4 LN states, states rounded up
     // offsets in shared memory: float32 arrays in floats, the chunks as stored behind them in bytes
-    int x, d, g, s, z, y, du, dd, carry, rate, entry, dA, red, skip, raw, couplings, bytes;
+    int d, u, g, x, s, z, y, du, dd, carry, rate, entry, dA, red, skip, raw, couplings, bytes;
     int pitch;                    // elements between two tokens' couplings
-    static constexpr int kRow = PD_SCAN_CHUNK;
-    __host__ __device__ GradShape(int ln, int state, int per_warp, int element) {
-        const int wide = 4 * ln;
+    static constexpr int kRow = PD_SCAN_CHUNK, kWide = 4 * LN;
+    __host__ __device__ GradShape(int state, int per_warp, int element) {
         channels = kGradWarps * per_warp;
-        slices = (state + wide - 1) / wide;
-        pad = slices * wide;
+        slices = ONE ? 1 : (state + kWide - 1) / kWide;
+        pad = slices * kWide;
         pitch = pad + 4;          // (the token groups' rows then lie in different banks)
-        const int cells = channels * kRow;
-        x = 0; d = x + cells; g = d + cells; s = g + cells; z = s + cells;
-        y = z + cells; du = y + (slices > 1 ? cells : 0); dd = du + (slices > 1 ? cells : 0);
-        carry = dd + (slices > 1 ? cells : 0);
+        const int cells = channels * kRow, more = slices > 1 ? cells : 0;
+        d = 0; u = d + 2 * cells; g = u + 2 * cells;     // as pairs of equal halves, which packed operations take
+        x = g + 2 * cells; s = x + cells; z = s + cells;
+        y = z + cells; du = y + more; dd = du + more;
+        carry = dd + more;
         rate = carry + channels * pad;
         entry = rate + channels * pad;           // two buffers
         dA = entry + 2 * channels * pad;
         red = dA + channels * slices * 128;
-        const int warps = kGradWarps * kRow * (2 * wide + 4), staged = kGradThreads * 8;   // at different times
+        const int warps = kGradWarps * kRow * (2 * kWide + 4), staged = kGradThreads * 8;   // at different times
         skip = red + (warps > staged ? warps : staged);
         raw = (skip + channels) * 4;             // x, delta, dy, z: (4, tokens, channels)
         couplings = raw + 4 * cells * element;   // two buffers of B and C: (2, 2, tokens, pitch)
@@ -1168,14 +1166,15 @@ struct GradShape {
     }
 };
 
-template <class T, int LN, bool GATE>
+template <class T, int LN, bool GATE, bool ONE>
 __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel(PdScanArgs a) {
     constexpr int K = LN, TL = 32 / LN, kRow = PD_SCAN_CHUNK, kWide = 4 * LN;
     static_assert(K * TL == kRow, "a warp covers a chunk");
     extern __shared__ float4 smem4[];
     float* smem = reinterpret_cast<float*>(smem4);
-    const GradShape G(LN, a.state, a.per_warp, sizeof(T));
-    float *sX = smem + G.x, *sD = smem + G.d, *sG = smem + G.g, *sS = smem + G.s, *sZ = smem + G.z;
+    const GradShape<LN, ONE> G(a.state, a.per_warp, sizeof(T));
+    float *sX = smem + G.x, *sS = smem + G.s, *sZ = smem + G.z;
+    float2 *sD = reinterpret_cast<float2*>(smem + G.d), *sU = reinterpret_cast<float2*>(smem + G.u), *sG = reinterpret_cast<float2*>(smem + G.g);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, tl = lane / LN;
     const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
     const int64_t job = blockIdx.x, s = job / (tiles * a.groups);
@@ -1276,9 +1275,11 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                     g *= z * sig;
                 }
                 // (what lies behind the sequence's end was fetched as zeros)
+                d = i < n ? d : 0.0f;
                 sX[at] = x;
-                sD[at] = i < n ? d : 0.0f;
-                sG[at] = g;
+                sD[at] = make_float2(d, d);
+                sU[at] = make_float2(d * x, d * x);
+                sG[at] = make_float2(g, g);
                 sS[at] = slope;
                 dskip[i] += g * x;
             }
@@ -1312,24 +1313,25 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                 float* kept = smem + G.carry + c * G.pad + first;
                 leave[0] = *reinterpret_cast<const pair_t*>(kept);
                 leave[1] = *reinterpret_cast<const pair_t*>(kept + 2);
-                float x[K], d[K], g[K], y[K], du[K], dd[K];
-                load_steps<K>(sX + place(c, tl * K), x);
-                load_steps<K>(sD + place(c, tl * K), d);
-                load_steps<K>(sG + place(c, tl * K), g);
+                float y[K], du[K], dd[K];
+                const int here = place(c, tl * K);
+                pair_t u[K], gg[K];
+                load_pairs<K>(sU + here, u);
+                load_pairs<K>(sG + here, gg);
                 // both directions from zero: h[i + 1] after token i, e before token 0, and the decay over all
-                pair_t w[K][2], u[K], gg[K], h[K + 1][2], up[2], down[2], e[2];
+                pair_t w[K][2], h[K + 1][2], up[2], down[2], e[2];
+                {
+                    pair_t step[K];
+                    load_pairs<K>(sD + here, step);
 #pragma unroll
-                for (int i = 0; i < K; ++i) {
-                    const pair_t step = pack(d[i], d[i]);
-                    u[i] = mul2(step, pack(x[i], x[i]));
-                    gg[i] = pack(g[i], g[i]);
+                    for (int i = 0; i < K; ++i)
 #pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        w[i][p] = decay2(step, rate[p]);
-                        const pair_t b = mul2(u[i], B[i][p]);
-                        h[i + 1][p] = i == 0 ? b : mad2(w[i][p], h[i][p], b);
-                        up[p] = i == 0 ? w[i][p] : mul2(up[p], w[i][p]);
-                    }
+                        for (int p = 0; p < 2; ++p) {
+                            w[i][p] = decay2(step[i], rate[p]);
+                            const pair_t b = mul2(u[i], B[i][p]);
+                            h[i + 1][p] = i == 0 ? b : mad2(w[i][p], h[i][p], b);
+                            up[p] = i == 0 ? w[i][p] : mul2(up[p], w[i][p]);
+                        }
                 }
 #pragma unroll
                 for (int i = K - 1; i >= 0; --i)
@@ -1384,10 +1386,10 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                     for (int i = 0; i < K; ++i) y[i] = halves(mad2(C[i][1], h[i + 1][1], mul2(C[i][0], h[i + 1][0])));
                 // backwards from the true gradient
                 pair_t* sums = reinterpret_cast<pair_t*>(smem + G.dA + ((c * G.slices + q) * 32 + lane) * 4);
-                pair_t dA[2] = {sums[0], sums[1]};
+                pair_t dA[2] = {sums[0], sums[1]}, step[K];
+                load_pairs<K>(sD + here, step);
 #pragma unroll
                 for (int i = K - 1; i >= 0; --i) {
-                    const pair_t step = pack(d[i], d[i]);
                     pair_t to_u, to_d;
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
@@ -1398,7 +1400,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                         to_u = p == 0 ? mul2(now, B[i][p]) : mad2(now, B[i][p], to_u);
                         const pair_t moved = mul2(e[p], h[i][p]);
                         to_d = p == 0 ? mul2(moved, rate[p]) : mad2(moved, rate[p], to_d);
-                        dA[p] = mad2(moved, step, dA[p]);
+                        dA[p] = mad2(moved, step[i], dA[p]);
                     }
                     du[i] = halves(to_u);
                     dd[i] = halves(to_d);
@@ -1417,9 +1419,9 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
 #if PD_MODE == 2
                     td *= 0.6931471805599453f;     // rates are in units of log2(e)
 #endif
-                    const float tx = sX[at], tstep = sD[at], tg = sG[at], skip = smem[G.skip + c];
+                    const float tx = sX[at], tstep = sD[at].x, tg = sG[at].x, skip = smem[G.skip + c];
                     sX[at] = tu * tstep + skip * tg;
-                    sD[at] = (td + tu * tx) * sS[at];
+                    sS[at] *= td + tu * tx;
                     if (GATE) sZ[at] *= ty + skip * tx;
                 }
             }
@@ -1433,6 +1435,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                 *reinterpret_cast<ulonglong2*>(to + kWide) = make_ulonglong2(dC[i][0], dC[i][1]);
             }
             __syncthreads();
+#pragma unroll
             for (int v = tid; v < kRow * 2 * LN; v += kGradThreads) {
                 const int t = v / (2 * LN), part = v % (2 * LN) * 4;
                 float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -1457,7 +1460,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
             for (int i = 0; i < 4; ++i) {
                 const int p = row + i * kRow;
                 vx[i] = sX[p];
-                vd[i] = sD[p];
+                vd[i] = sS[p];
                 if (GATE) vz[i] = sZ[p];
                 if (i < n) dbias[i] += vd[i];
             }
@@ -1496,19 +1499,25 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
     }
 }
 
-// dB and dC: the tiles of a group added up in order
+// dB and dC: the tiles of a group added up in order, four states per thread
 template <class T>
-__global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArgs a, int pad, int64_t tiles) {
-    const int64_t wide = a.tok.rows * 2 * pad, i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if (i >= wide * a.groups) return;
-    const int64_t at = i % wide, g = i / wide, r = at / (2 * pad);
-    const int n = (int)(at % pad), which = (int)(at / pad % 2);
-    if (n >= a.state) return;
+__global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArgs a, int pad, int tiles) {
+    const int64_t wide = a.tok.rows * 2 * pad;
+    const int64_t at = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) * 4, g = blockIdx.y;
+    if (at >= wide) return;
+    const int64_t r = at / (2 * pad);
+    const int n = (int)(at - r * 2 * pad), which = n >= pad, first = n - which * pad;
     const float* p = a.partial_bc + g * tiles * wide + at;
-    float total = 0.0f;
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 8
-    for (int64_t t = 0; t < tiles; ++t) total += p[t * wide];
-    store1((T*)(which ? a.dC : a.dB) + (r * a.groups + g) * a.state + n, total);
+    for (int t = 0; t < tiles; ++t) {
+        const float4 q = *reinterpret_cast<const float4*>(p + t * wide);
+        total.x += q.x; total.y += q.y; total.z += q.z; total.w += q.w;
+    }
+    const float v[4] = {total.x, total.y, total.z, total.w};
+    T* to = (T*)(which ? a.dC : a.dB) + (r * a.groups + g) * a.state;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (first + i < a.state) store1(to + first + i, v[i]);
 }
 
 __global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdScanArgs a) {
@@ -1660,20 +1669,24 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
         using T = decltype(e);
         auto run = [&](auto ln) -> cudaError_t {
             constexpr int LN = decltype(ln)::value;
-            const GradShape G(LN, a.state, a.per_warp, sizeof(T));
+            const bool one = a.state <= 4 * LN;
+            const GradShape<LN, false> G(a.state, a.per_warp, sizeof(T));
             const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
             const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
             if (blocks > 0) {
-                auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true> : pd_selective_scan_grad_kernel<T, LN, false>;
+                auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true, true> : pd_selective_scan_grad_kernel<T, LN, false, true>;
+                if constexpr (LN == 4)
+                    if (!one) kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true, false> : pd_selective_scan_grad_kernel<T, LN, false, false>;
                 cudaError_t err = allow_smem(kernel, G.bytes);
                 if (err != cudaSuccess) return err;
                 kernel<<<(unsigned)blocks, kGradThreads, G.bytes, st>>>(a);
                 err = cudaGetLastError();
                 if (err != cudaSuccess) return err;
             }
-            const int64_t cells = a.tok.rows * 2 * G.pad * a.groups;
-            if (cells > 0) {
-                pd_selective_scan_sum_bc_kernel<T><<<(unsigned)blocks_for(cells, 256), 256, 0, st>>>(a, G.pad, tiles);
+            const int64_t fours = a.tok.rows * 2 * G.pad / 4;
+            if (fours > 0) {
+                const dim3 grid((unsigned)blocks_for(fours, 256), (unsigned)a.groups);
+                pd_selective_scan_sum_bc_kernel<T><<<grid, 256, 0, st>>>(a, G.pad, (int)tiles);
                 cudaError_t err = cudaGetLastError();
                 if (err != cudaSuccess) return err;
             }

@@ -86,7 +86,7 @@ int64_t scan_chunks(const pd_selective_scan_params* p, const Dims& d) {
 // channel's work per chunk; fewer give more blocks.  The smallest product of waves and work per wave wins.
 int grad_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
     const int64_t per = d.channels / p->groups, slots = (int64_t)sms * 3;
-    const int most = p->state > 16 ? 4 : 8;    // (slices of sixteen states need shared memory for as many sums)
+    const int most = p->state > 16 ? 4 : 6;    // (shared memory for three blocks; more states need more sums)
     int best = 1;
     int64_t least = INT64_MAX;
     for (int n = most; n >= 1; --n) {
@@ -101,25 +101,23 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lan
     return (per + ch - 1) / ch * p->groups;
 }
 // The prompt kernel's channels per lane and segments.  Two channels per lane halve the reads of B and C; one gives
-// twice the blocks, for calls that do not fill the GPU otherwise.  Eight blocks of two warps run on an SM, four warps
-// on a scheduler; fewer leave it waiting (1.7 warps issue 0.36 instructions a clock, four about twice that), so
-// a call that leaves room for it is cut into segments, of at least 64 tokens, until the blocks are one wave:
-// that costs a first pass over all but the last segment of a sequence.  A packed call is cut at an even share,
-// so that one long sequence does not outlast all others.
+// twice the blocks, for calls that do not fill the GPU otherwise.  Seven blocks of two warps run on an SM.  Cutting a
+// sequence costs a first pass over all but its last segment, which takes two thirds of the second's time: it pays
+// where a call has fewer than two blocks per SM (1 x 8192 x 2048: 16 segments 256 us, uncut about 800; 4 x 2048 x
+// 2048: uncut 237 us, two segments 283, four 248).  A packed call is cut at three times an even share, so that one
+// long sequence does not outlast all others (17 of them, 8200 x 2560: 252 us, at one share 358, at six 264).
 void scan_cut(const pd_selective_scan_params* p, const Dims& d, int sms, PdScanPlan* plan) {
     const int64_t seqs = d.seqs > 0 ? d.seqs : 1, rows = d.rows > 0 ? d.rows : 1, mean = (rows + seqs - 1) / seqs;
-    const int64_t wave = (int64_t)sms * 8, most = mean / 64 > 0 ? mean / 64 : 1;
+    const int64_t wave = (int64_t)sms * 7, most = mean / 64 > 0 ? mean / 64 : 1;
+    const bool cut = scan_tiles(p, d, 1) * seqs < sms * 2;
     int per_lane = p->state > 32 ? 2 : 1;
-    if (p->state > 8 && scan_tiles(p, d, 2) * seqs * most >= wave / 2) per_lane = 2;
+    if (p->state > 8 && scan_tiles(p, d, 2) * seqs * (cut ? most : 1) >= wave * 3 / 4) per_lane = 2;
     const int64_t tiles = scan_tiles(p, d, per_lane);
-    int64_t cuts = wave / (tiles * seqs), segment = INT32_MAX;
+    int64_t cuts = cut ? wave / (tiles * seqs) : 1, segment = INT32_MAX;
     if (cuts > most) cuts = most;
-    if (p->packed) {
-        segment = rows * tiles / wave;
-        if (segment < 64) segment = 64;
-    } else if (cuts > 1) {
-        segment = (mean + cuts - 1) / cuts;
-    }
+    if (cuts > 1) segment = (mean + cuts - 1) / cuts;
+    else if (p->packed) segment = rows * tiles / wave * 3;
+    if (segment < 64) segment = 64;
     segment = (segment + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK * PD_SCAN_CHUNK;     // (carries are kept at whole chunks)
     plan->items = per_lane;
     plan->segment = segment;
@@ -197,6 +195,7 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
     if (rc) return rc;
     if (p->state < 1 || p->state > PD_SCAN_MAX_STATE)
         return fail(err, cap, "%s: state must lie in [1, %d], got %lld", what, PD_SCAN_MAX_STATE, (long long)p->state);
+    if (p->groups > 65535) return fail(err, cap, "%s: more than 65535 groups", what);
     if (p->groups < 1 || d.channels % p->groups != 0)
         return fail(err, cap, "%s: %lld channels do not divide into %lld groups", what, (long long)d.channels, (long long)p->groups);
     if (!flag(p->softplus) || !flag(p->bias) || !flag(p->skip) || !flag(p->gate) || !flag(p->initial) || !flag(p->final) ||

@@ -403,7 +403,7 @@ def causal_conv_grad(length: int, width: int = 4, *, silu: bool = True, bias: bo
 def _scan_family(name: str, length, state, groups, softplus, bias, skip, gate, initial, final, carries, packed,
                  dtype) -> Family:
     return Family(name, dict(length=_whole(name, "length", length, 0, 2**31 - 1), state=_whole(name, "state", state, 1, 64),
-                             groups=_whole(name, "groups", groups, 1, 2**20), softplus=bool(softplus), bias=bool(bias),
+                             groups=_whole(name, "groups", groups, 1, 65535), softplus=bool(softplus), bias=bool(bias),
                              skip=bool(skip), gate=bool(gate), initial=bool(initial), final=bool(final),
                              carries=bool(carries), packed=bool(packed), dtype=_element_type(name, dtype)))
 
