@@ -215,8 +215,8 @@ typedef struct pd_source_kernel_params {
  * [0, length] and a decreasing pair is an empty sequence; output rows of no
  * sequence are zero.  Parameters and recurrent states are float32.  Arithmetic
  * is float32, rounded once at the store.  Zero values in a flag leave the
- * operands and results in [ ] out.  Scratch for the gradients' partial sums
- * comes from `workspace`, or from the library's pool, which a stream that is
+ * operands and results in [ ] out.  Scratch (the gradients' partial sums, the
+ * states between the segments of a long prompt) comes from `workspace`, or from the library's pool, which a stream that is
  * being captured into a graph cannot use. */
 #define PD_TYPE_F32 0
 #define PD_TYPE_F16 1

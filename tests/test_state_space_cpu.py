@@ -186,6 +186,7 @@ def test_native_conv_refusals(fields, grid, words):
     (dict(state=65), (2, 8), "state must lie"),
     (dict(groups=3), (2, 8), "do not divide"),
     (dict(groups=0), (2, 8), "do not divide"),
+    (dict(groups=70000), (2, 70000), "65535 groups"),
     (dict(gate=-1), (2, 8), "flags must be"),
     (dict(packed=2), (2, 8), "flags must be"),
 ])
