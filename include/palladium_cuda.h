@@ -217,7 +217,8 @@ typedef struct pd_source_kernel_params {
  * is float32, rounded once at the store.  Zero values in a flag leave the
  * operands and results in [ ] out.  Scratch (the gradients' partial sums, the
  * states between the segments of a long prompt) comes from `workspace`, or from the library's pool, which a stream that is
- * being captured into a graph cannot use. */
+ * being captured into a graph cannot use.  No result may share memory with an
+ * operand or another result (refused), but for a step's state. */
 #define PD_TYPE_F32 0
 #define PD_TYPE_F16 1
 #define PD_TYPE_BF16 2

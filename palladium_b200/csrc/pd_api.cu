@@ -732,6 +732,10 @@ int launch_impl(int family, const void* params, size_t params_bytes, int math_mo
         rc = check_buffers("output", n_out, (int)want_out.size(), out_bytes, want_out.data(),
                            const_cast<const void* const*>(out), err, err_cap);
         if (rc) return rc;
+        if (pd_is_scan_family(family)) {
+            rc = pd_scan_overlap(family, n_in, in, in_bytes, n_out, out, out_bytes, err, err_cap);
+            if (rc) return rc;
+        }
     } else {
         if (n_in + n_out > 64)
             return fail(PD_ERR_INVALID_ARGUMENT, err, err_cap, "source kernel: at most 64 buffers, got %d", n_in + n_out);

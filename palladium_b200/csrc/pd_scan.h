@@ -111,6 +111,9 @@ struct PdScanPlan {
 bool pd_is_scan_family(int family);
 int pd_scan_plan(int family, const void* params, size_t params_bytes, const int64_t grid[3], const int64_t block[3],
                  int sms, PdScanPlan* plan, char* err, size_t err_cap);
+// Refuses results that share memory with an operand or with one another; a step's new state may be its old one.
+int pd_scan_overlap(int family, int n_in, const void* const* in, const size_t* in_bytes, int n_out, void* const* out,
+                    const size_t* out_bytes, char* err, size_t err_cap);
 int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
                    const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap);
 

@@ -281,6 +281,25 @@ int pd_scan_plan(int family, const void* params, size_t params_bytes, const int6
     return rc;
 }
 
+int pd_scan_overlap(int family, int n_in, const void* const* in, const size_t* in_bytes, int n_out, void* const* out,
+                    const size_t* out_bytes, char* err, size_t err_cap) {
+    // the state of a step: operand 1 of the convolution's, 0 of the scan's; result 1 of both
+    const int state = family == PD_FAMILY_CAUSAL_CONV_STEP ? 1 : family == PD_FAMILY_SELECTIVE_SCAN_STEP ? 0 : -1;
+    auto meet = [](const void* p, size_t n, const void* q, size_t m) {
+        const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+        return n && m && a < b + m && b < a + n;
+    };
+    for (int o = 0; o < n_out; ++o) {
+        for (int i = 0; i < n_in; ++i)
+            if (meet(out[o], out_bytes[o], in[i], in_bytes[i]) && !(o == 1 && i == state && out[o] == in[i]))
+                return fail(err, err_cap, "output %d shares memory with input %d", o, i);
+        for (int p = 0; p < o; ++p)
+            if (meet(out[o], out_bytes[o], out[p], out_bytes[p]))
+                return fail(err, err_cap, "output %d shares memory with output %d", o, p);
+    }
+    return PD_OK;
+}
+
 int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
                    const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap) {
     const PdScanTable* table = math_mode == PD_MATH_SAFE ? pd_scan_table_safe()

@@ -363,6 +363,25 @@ def test_strided_and_host_tensors_are_refused():
         call(x.half(), weight, bias)
 
 
+def test_results_over_operands_are_refused():
+    case = Case("conv", [8, 8], 16)
+    call = case.call(pd.cuda_call_jit)
+    x, weight, bias = [device(a) for a in case.operands()]
+    with pytest.raises(DispatchError, match="output 0 shares memory with input 0"):
+        call.on_device(x, weight, bias, out=x)
+    room = torch.empty(x.numel() + 16, device="cuda")
+    room[16:] = x.reshape(-1)
+    with pytest.raises(DispatchError, match="output 0 shares memory with input 0"):
+        call.on_device(room[16:].view(x.shape), weight, bias, out=room[:-16].view(x.shape))
+    step = families.causal_conv_step()
+    call = pd.cuda_call_jit(step, grid=(2, 16), out_shape=families.out_shapes(step, (2, 16)))
+    token, state = torch.randn(2, 16, device="cuda"), torch.randn(2, 3, 16, device="cuda")
+    with pytest.raises(DispatchError, match="output 1 shares memory with input 1"):
+        moved = torch.randn(3 * 2 * 16 + 4, device="cuda")
+        call.on_device(token, moved[4:].view(2, 3, 16), weight, bias, out=(torch.empty_like(token), moved[:-4].view(2, 3, 16)))
+    call.on_device(token, state, weight, bias, out=(torch.empty_like(token), state))
+
+
 @pytest.mark.parametrize("kind", ["conv", "scan"])
 def test_side_streams_and_equal_bits(kind):
     case = Case(kind, [300, 300], 72, dtype="bfloat16", **({} if kind == "conv" else dict(gate=True)))
