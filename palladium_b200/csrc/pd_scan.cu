@@ -653,7 +653,8 @@ __device__ __forceinline__ void copy4(T* to, const T* from, bool vec, int n) {
     }
 }
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group 0;" ::: "memory"); }
+template <int LEFT = 0>     // groups that may still be under way
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
 template <class T>
 __device__ __forceinline__ Raw4<T> raw4(const T* p) {       // from shared memory, aligned to four elements
     Raw4<T> r;
@@ -847,19 +848,24 @@ __device__ __forceinline__ void load_pairs(const float2* p, pair_t (&v)[K]) {
 
 // ---------------------------------------------------------------------------
 // The prompt kernel.  A lane holds four states of NCH neighbouring channels and walks the tokens one by one; LN
-// lanes share a channel, 32 / LN * NCH channels make a warp's, two warps a block.  A tile of 32 tokens is staged in
-// shared memory as float32 (step lengths, inputs, couplings), the next one's elements on their way meanwhile.
+// lanes share a channel, 32 / LN * NCH channels make a warp's.  Two of a block's four warps walk; the other two bring
+// tiles of 32 tokens to shared memory as float32 (step lengths, inputs, couplings) ahead of them, the elements of the
+// tile after on their way, and finish the outputs behind them (skip, gate, rounding), with one barrier per tile.
 //
 // Bound: the exponentials, one per (token, channel, state), 16 per clock and SM: 8 cycles per warp instruction and
 // scheduler.  Beside each stand 2 packed multiply-adds and, with two channels per lane, 1.75 words of shared memory
-// (7 of the 8 cycles).  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 212 us, 62 of them what the
-// exponentials cannot do without: 9.6 instructions per state, 0.36 a clock and scheduler, since 512 blocks are 1.7
-// warps per scheduler.  Forms that hold tokens across lanes or warps instead, so as to fill the GPU with one
-// sequence, needed 18 to 31 instructions per state for their scans (8192 x 2048 x 16 took 417 us); so a call with
-// few sequences and channels is cut into segments of tokens: a first launch (STATE) takes each from a zero state
-// to its end state and total step, and the blocks of the second compose the state entering theirs.
+// (7 of the 8 cycles).  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 178 us, 58 of them what the
+// exponentials cannot do without: 512 blocks are 1.7 walking warps per scheduler, too few to hide what each waits
+// for (212 us with staging and walking in turn by the same two warps).  Forms that hold tokens across lanes or warps
+// instead, so as to fill the GPU with one sequence, needed 18 to 31 instructions per state for their scans (8192 x
+// 2048 x 16 took 417 us); so a call with few sequences and channels is cut into segments of tokens: a first launch
+// (STATE) takes each from a zero state to its end state and total step, and the blocks of the second compose the state
+// entering theirs.
 // ---------------------------------------------------------------------------
-constexpr int kScanWarps = 2, kScanThreads = 32 * kScanWarps;
+constexpr int kScanWarps = 2, kStageThreads = 64, kScanThreads = 32 * kScanWarps + kStageThreads;
+
+// all of the block's warps, which reach it from different places
+__device__ __forceinline__ void tile_barrier() { asm volatile("barrier.sync 1, %0;" ::"n"(kScanThreads) : "memory"); }
 
 struct ScanShape {
     int warp_channels, channels, pad;
@@ -867,9 +873,10 @@ struct ScanShape {
     static constexpr int kRow = PD_SCAN_CHUNK;
     __host__ __device__ constexpr ScanShape(int ln, int nch, int element)
         : warp_channels(32 / ln * nch), channels(kScanWarps * warp_channels), pad(4 * ln), du(0),
-          B(2 * kRow * channels), C(B + kRow * pad), y(C + kRow * pad), raw((y + kRow * channels) * 4),
-          // two buffers of x, delta, z: (3, tokens, channels), and one of B and C: (2, tokens, pad)
-          bytes(raw + 6 * kRow * channels * element + 2 * kRow * pad * element) {}
+          // two buffers of each: (tokens, channels) steps and inputs, (tokens, pad) B and C, (tokens, channels) sums
+          B(4 * kRow * channels), C(B + 2 * kRow * pad), y(C + 2 * kRow * pad), raw((y + 2 * kRow * channels) * 4),
+          // as stored: four buffers of x, delta, z, (3, tokens, channels), and two of B and C, (2, tokens, pad)
+          bytes(raw + 12 * kRow * channels * element + 4 * kRow * pad * element) {}
 };
 
 // segments: where a sequence's first one is counted, and the sequence of the id-th (an empty one has one, too)
@@ -890,10 +897,10 @@ __device__ __forceinline__ int64_t segment_owner(const PdScanArgs& a, int64_t id
 }
 
 template <class T, int LN, int NCH, bool FULL, bool STATE>
-__global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, 4) pd_selective_scan_kernel(PdScanArgs a) {
     constexpr ScanShape G(LN, NCH, sizeof(T));
-    constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kScanThreads / quads;
-    static_assert(kScanThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");
+    constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kStageThreads / quads;
+    static_assert(kStageThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");
     extern __shared__ float4 smem4[];
     float* smem = reinterpret_cast<float*>(smem4);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, cl = lane / LN, first = sub * 4;
@@ -916,18 +923,19 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
     const int64_t start = begin + number * a.segment, stop = start + a.segment < end ? start + a.segment : end;
     if (number < 0 || (number > 0 && start >= end)) return;
     if (STATE && stop == end) return;         // nothing follows a last segment
+    const bool computes = warp < kScanWarps;
     // this lane's channels, their rates and the state entering
     pair_t rate[NCH][2], h[NCH][2];
     const int mine = warp * G.warp_channels + cl * NCH;
 #pragma unroll
     for (int j = 0; j < NCH; ++j) {
-        const bool in = mine + j < count;
+        const bool in = computes && mine + j < count;
         const int64_t c = c0 + (in ? mine + j : 0);
         float A[4], v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
         load_states(a.A + c * a.state, first, a.state, A);
 #pragma unroll
         for (int i = 0; i < 4; ++i) A[i] = scan_rate(A[i]);
-        if (!STATE) {
+        if (!STATE && computes) {
             if (a.initial) load_states(a.initial + (s * a.channels + c) * a.state, first, a.state, v);
             for (int64_t k = id0; k < id; ++k) {
                 const float total = a.totals[k * a.channels + c];
@@ -956,7 +964,7 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
         }
     };
     // staging: four channels of a token per thread, always the same channels
-    const int c4 = tid % quads * 4, st = tid / quads;
+    const int stid = tid & (kStageThreads - 1), c4 = stid % quads * 4, st = stid / quads;
     const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
     float bias[4], skip[4];
 #pragma unroll
@@ -966,11 +974,15 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
     }
     const int64_t chunk0 = first_chunk(a.tok, s, begin), stride = (int64_t)a.groups * a.state;
     T* raw = reinterpret_cast<T*>(reinterpret_cast<char*>(smem) + G.raw);
-    T* couplings = raw + 6 * kRow * G.channels;
+    T* couplings = raw + 12 * kRow * G.channels;
     constexpr int cells = kRow * G.channels;
     const bool gate = !STATE && a.z;
-    auto copy_tile = [&](int64_t from, int buffer) {
-        T* to = raw + buffer * 3 * cells + st * G.channels + c4;
+    const int tiles_here = (int)((stop - start + kRow - 1) / kRow);
+    auto copy_tile = [&](int k) {
+        const int64_t from = start + (int64_t)k * kRow;
+        if (k >= tiles_here) { copies_commit(); return; }      // (each tile one group, for the wait to count)
+        T* to = raw + (k & 3) * 3 * cells + st * G.channels + c4;
+        T* to_bc = couplings + (k & 1) * 2 * kRow * G.pad;
         int64_t at = (from + st) * a.channels + c0 + c4;
 #pragma unroll 2
         for (int t = st; t < kRow; t += kPass) {
@@ -982,24 +994,21 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
             at += kPass * a.channels;
         }
 #pragma unroll 2
-        for (int i = tid; i < kRow * LN; i += kScanThreads) {
+        for (int i = stid; i < kRow * LN; i += kStageThreads) {
             const int t = i / LN, n4 = i % LN * 4;
             int n = from + t < stop ? a.state - n4 : 0;
             n = n < 0 ? 0 : n > 4 ? 4 : n;
             const int64_t at = (from + t) * stride + group * a.state + n4;
-            copy4(couplings + 4 * i, (const T*)a.B + at, a.vec_states, n);
-            if (!STATE) copy4(couplings + kRow * G.pad + 4 * i, (const T*)a.C + at, a.vec_states, n);
+            copy4(to_bc + 4 * i, (const T*)a.B + at, a.vec_states, n);
+            if (!STATE) copy4(to_bc + kRow * G.pad + 4 * i, (const T*)a.C + at, a.vec_states, n);
         }
         copies_commit();
     };
-    float total[NCH] = {};
-    if (start < stop) copy_tile(start, 0);
-    int buffer = 0;
-    for (int64_t from = start; from < stop; from += kRow, buffer ^= 1) {
-        const int tokens = (int)(stop - from < kRow ? stop - from : kRow);
-        copies_wait();
-        // (each thread reads back what it has fetched itself)
-        const T* got = raw + buffer * 3 * cells + st * G.channels + c4;
+    // a tile's elements to float32 (each thread reads back what it has fetched itself)
+    auto stage = [&](int k) {
+        const int tokens = (int)(stop - start - (int64_t)k * kRow < kRow ? stop - start - (int64_t)k * kRow : kRow);
+        const T* got = raw + (k & 3) * 3 * cells + st * G.channels + c4;
+        float* du = smem + G.du + (k & 1) * 2 * cells;
         for (int t = st; t < kRow; t += kPass, got += kPass * G.channels) {
             const Raw4<T> rx = raw4(got), rd = raw4(got + cells);
             float2 v[4];
@@ -1011,29 +1020,79 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
                 v[i] = make_float2(d, d * load1(&rx.e[i]));
             }
             // (every other four threads store their second half first: no two of eight meet in a bank)
-            float4* to = reinterpret_cast<float4*>(smem + G.du + 2 * (t * G.channels + c4));
+            float4* to = reinterpret_cast<float4*>(du + 2 * (t * G.channels + c4));
             const float4 low = make_float4(v[0].x, v[0].y, v[1].x, v[1].y), high = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
             const int turn = lane >> 2 & 1;
             to[turn] = turn ? high : low;
             to[turn ^ 1] = turn ? low : high;
         }
-        for (int i = tid; i < kRow * LN; i += kScanThreads) {
-            const Raw4<T> b = raw4(couplings + 4 * i);
-            reinterpret_cast<float4*>(smem + G.B)[i] = make_float4(load1(&b.e[0]), load1(&b.e[1]), load1(&b.e[2]), load1(&b.e[3]));
+        const T* bc = couplings + (k & 1) * 2 * kRow * G.pad;
+        for (int i = stid; i < kRow * LN; i += kStageThreads) {
+            const Raw4<T> b = raw4(bc + 4 * i);
+            reinterpret_cast<float4*>(smem + G.B + (k & 1) * kRow * G.pad)[i] =
+                make_float4(load1(&b.e[0]), load1(&b.e[1]), load1(&b.e[2]), load1(&b.e[3]));
             if (!STATE) {
-                const Raw4<T> c = raw4(couplings + kRow * G.pad + 4 * i);
-                reinterpret_cast<float4*>(smem + G.C)[i] = make_float4(load1(&c.e[0]), load1(&c.e[1]), load1(&c.e[2]), load1(&c.e[3]));
+                const Raw4<T> c = raw4(bc + kRow * G.pad + 4 * i);
+                reinterpret_cast<float4*>(smem + G.C + (k & 1) * kRow * G.pad)[i] =
+                    make_float4(load1(&c.e[0]), load1(&c.e[1]), load1(&c.e[2]), load1(&c.e[3]));
             }
         }
-        if (from + kRow < stop) copy_tile(from + kRow, buffer ^ 1);
+    };
+    // a tile's outputs: the sums, the skip and the gate
+    auto finish = [&](int k) {
+        const int64_t from = start + (int64_t)k * kRow;
+        const int tokens = (int)(stop - from < kRow ? stop - from : kRow);
+        const T* got = raw + (k & 3) * 3 * cells + st * G.channels + c4;
+        const float* sum = smem + G.y + (k & 1) * cells + c4 / G.warp_channels * kRow * G.warp_channels + c4 % G.warp_channels;
+        T* to = (T*)a.y + (from + st) * a.channels + c0 + c4;
+        for (int t = st; t < tokens; t += kPass, got += kPass * G.channels, to += kPass * a.channels) {
+            const Raw4<T> rx = raw4(got);
+            const float4 q = *reinterpret_cast<const float4*>(sum + t * G.warp_channels);
+            float v[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[i] += skip[i] * load1(&rx.e[i]);
+            if (gate) {
+                const Raw4<T> rz = raw4(got + 2 * cells);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float z = load1(&rz.e[i]);
+                    v[i] *= z * sigmoid_(z);
+                }
+            }
+            put4(to, a.vec, left, v);
+        }
+    };
+    float total[NCH] = {};
+    if (!computes && tiles_here > 0) {
+        copy_tile(0);
+        copy_tile(1);
+        copies_wait<1>();
+        stage(0);
+    }
+    tile_barrier();
+    // One barrier per tile: while two warps walk tile k, the other two finish tile k - 1 and stage tile k + 1, with
+    // tile k + 2 on its way.
+    for (int k = 0; k < tiles_here; ++k) {
+        const int64_t from = start + (int64_t)k * kRow;
+        if (!computes) {
+            if (!STATE && k > 0) finish(k - 1);
+            if (k + 1 < tiles_here) {
+                copy_tile(k + 2);
+                copies_wait<1>();
+                stage(k + 1);
+            }
+            tile_barrier();
+            continue;
+        }
         if (!STATE && a.carries) {
             float* to = a.carries + (chunk0 + (from - begin) / PD_SCAN_CHUNK) * a.channels * a.state;
 #pragma unroll
             for (int j = 0; j < NCH; ++j) keep(to, j);
         }
-        __syncthreads();
-        const float* du = smem + G.du + 2 * mine;
-        float* out = smem + G.y + warp * kRow * G.warp_channels + cl * NCH;     // (warp, token, channel)
+        const float* du = smem + G.du + (k & 1) * 2 * cells + 2 * mine;
+        const float* tile_B = smem + G.B + (k & 1) * kRow * G.pad + first;
+        const float* tile_C = smem + G.C + (k & 1) * kRow * G.pad + first;
+        float* out = smem + G.y + (k & 1) * cells + warp * kRow * G.warp_channels + cl * NCH;     // (warp, token, channel)
         float sums[NCH] = {};
         // Four tokens at a time: their operands are read before the outputs of the four before them are stored (the
         // compiler would not move a read of shared memory past a store to it), so that sixteen exponentials are
@@ -1050,8 +1109,8 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
                     const float2 v = *reinterpret_cast<const float2*>(du + 2 * (t + i) * G.channels);
                     q.d[i][0] = v.x; q.u[i][0] = v.y;
                 }
-                q.B[i] = *reinterpret_cast<const ulonglong2*>(smem + G.B + (t + i) * G.pad + first);
-                if (!STATE) q.C[i] = *reinterpret_cast<const ulonglong2*>(smem + G.C + (t + i) * G.pad + first);
+                q.B[i] = *reinterpret_cast<const ulonglong2*>(tile_B + (t + i) * G.pad);
+                if (!STATE) q.C[i] = *reinterpret_cast<const ulonglong2*>(tile_C + (t + i) * G.pad);
             }
         };
         Operands q;
@@ -1109,29 +1168,11 @@ __global__ void __launch_bounds__(kScanThreads, 8) pd_selective_scan_kernel(PdSc
         }
 #pragma unroll
         for (int j = 0; j < NCH; ++j) total[j] += sums[j];
-        __syncthreads();
-        if (!STATE) {
-            // the skip and the gate
-            got = raw + buffer * 3 * cells + st * G.channels + c4;
-            const float* sum = smem + G.y + c4 / G.warp_channels * kRow * G.warp_channels + c4 % G.warp_channels;
-            T* to = (T*)a.y + (from + st) * a.channels + c0 + c4;
-            for (int t = st; t < tokens; t += kPass, got += kPass * G.channels, to += kPass * a.channels) {
-                const Raw4<T> rx = raw4(got);
-                const float4 q = *reinterpret_cast<const float4*>(sum + t * G.warp_channels);
-                float v[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] += skip[i] * load1(&rx.e[i]);
-                if (gate) {
-                    const Raw4<T> rz = raw4(got + 2 * cells);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float z = load1(&rz.e[i]);
-                        v[i] *= z * sigmoid_(z);
-                    }
-                }
-                put4(to, a.vec, left, v);
-            }
-        }
+        tile_barrier();
+    }
+    if (!computes) {
+        if (!STATE && tiles_here > 0) finish(tiles_here - 1);
+        return;
     }
     if (STATE) {
 #pragma unroll

@@ -100,23 +100,22 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lan
     const int64_t per = d.channels / p->groups, ch = 2 * 32 / pd_scan_lanes((int)p->state) * per_lane;
     return (per + ch - 1) / ch * p->groups;
 }
-// The prompt kernel's channels per lane and segments.  Two channels per lane halve the reads of B and C; one gives
-// twice the blocks, for calls that do not fill the GPU otherwise.  Seven blocks of two warps run on an SM.  Cutting a
-// sequence costs a first pass over all but its last segment, which takes two thirds of the second's time: it pays
-// where a call has fewer than two blocks per SM (1 x 8192 x 2048: 16 segments 256 us, uncut about 800; 4 x 2048 x
-// 2048: uncut 237 us, two segments 283, four 248).  A packed call is cut at three times an even share, so that one
-// long sequence does not outlast all others (17 of them, 8200 x 2560: 252 us, at one share 358, at six 264).
+// The prompt kernel's channels per lane and segments.  Two channels per lane halve the reads of B and C, one gives
+// twice the blocks and four instead of three of them on an SM: two from 12 blocks per SM on (16 x 1024 tokens x 4096
+// channels x 16 states: 571 against 604 us; 4 x 2048 x 2048: 211 against 182).  Cutting a sequence into segments
+// costs a first pass over all but its last, which takes two thirds of the second's time: it pays where a call has
+// fewer than two blocks per SM (1 x 8192 x 2048: 16 segments 269 us, 4 segments 279; 4 x 2048 x 2048: uncut 182 us,
+// two segments 236).  A packed call is cut at three times an even share, so that one long sequence does not
+// outlast all others (17 of them, 8200 x 2560: 249 us, cut at 1024 tokens 298).
 void scan_cut(const pd_selective_scan_params* p, const Dims& d, int sms, PdScanPlan* plan) {
     const int64_t seqs = d.seqs > 0 ? d.seqs : 1, rows = d.rows > 0 ? d.rows : 1, mean = (rows + seqs - 1) / seqs;
-    const int64_t wave = (int64_t)sms * 7, most = mean / 64 > 0 ? mean / 64 : 1;
-    const bool cut = scan_tiles(p, d, 1) * seqs < sms * 2;
-    int per_lane = p->state > 32 ? 2 : 1;
-    if (p->state > 8 && scan_tiles(p, d, 2) * seqs * (cut ? most : 1) >= wave * 3 / 4) per_lane = 2;
+    const int64_t most = mean / 64 > 0 ? mean / 64 : 1;
+    const int per_lane = p->state > 32 || (p->state > 8 && scan_tiles(p, d, 2) * seqs >= (int64_t)sms * 12) ? 2 : 1;
     const int64_t tiles = scan_tiles(p, d, per_lane);
-    int64_t cuts = cut ? wave / (tiles * seqs) : 1, segment = INT32_MAX;
+    int64_t cuts = tiles * seqs < sms * 2 ? (int64_t)sms * 14 / (tiles * seqs) : 1, segment = INT32_MAX;
     if (cuts > most) cuts = most;
     if (cuts > 1) segment = (mean + cuts - 1) / cuts;
-    else if (p->packed) segment = rows * tiles / wave * 3;
+    else if (p->packed) segment = rows * tiles / ((int64_t)sms * 4) * 3;
     if (segment < 64) segment = 64;
     segment = (segment + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK * PD_SCAN_CHUNK;     // (carries are kept at whole chunks)
     plan->items = per_lane;
@@ -231,7 +230,7 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
     } else {
         scan_cut(p, d, sms, plan);
         plan->grid = scan_tiles(p, d, (int)plan->items) * (plan->segments + free_rows);
-        plan->block = 64;
+        plan->block = 128;
         if (d.rows > plan->segment) {
             // (a dense call is cut only where a sequence is longer than a segment)
             if (p->packed || p->length > plan->segment) {
