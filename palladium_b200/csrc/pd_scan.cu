@@ -856,7 +856,8 @@ __device__ __forceinline__ void load_pairs(const float2* p, pair_t (&v)[K]) {
 // scheduler.  Beside each stand 2 packed multiply-adds and, with two channels per lane, 1.75 words of shared memory
 // (7 of the 8 cycles).  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 178 us, 58 of them what the
 // exponentials cannot do without: 512 blocks are 1.7 walking warps per scheduler, too few to hide what each waits
-// for (212 us with staging and walking in turn by the same two warps).  Forms that hold tokens across lanes or warps
+// for (212 us with staging and walking in turn by the same two warps; five blocks of 96 registers on an SM
+// instead of four of 120 take 3 % more here and 8 % less where a sequence is cut).  Forms that hold tokens across lanes or warps
 // instead, so as to fill the GPU with one sequence, needed 18 to 31 instructions per state for their scans (8192 x
 // 2048 x 16 took 417 us); so a call with few sequences and channels is cut into segments of tokens: a first launch
 // (STATE) takes each from a zero state to its end state and total step, and the blocks of the second compose the state
@@ -897,7 +898,7 @@ __device__ __forceinline__ int64_t segment_owner(const PdScanArgs& a, int64_t id
 }
 
 template <class T, int LN, int NCH, bool FULL, bool STATE>
-__global__ void __launch_bounds__(kScanThreads, 4) pd_selective_scan_kernel(PdScanArgs a) {
+__global__ void __launch_bounds__(kScanThreads, NCH == 1 ? 5 : 4) pd_selective_scan_kernel(PdScanArgs a) {
     constexpr ScanShape G(LN, NCH, sizeof(T));
     constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kStageThreads / quads;
     static_assert(kStageThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");

@@ -105,6 +105,15 @@ def test_scan_cut_into_segments(state, groups):
     compare(packed)
 
 
+@pytest.mark.parametrize("state, dtype", [(16, "bfloat16"), (13, "float32"), (24, "float16")])
+def test_scan_two_channels_per_lane(state, dtype):
+    """Calls of many blocks: each lane takes two channels."""
+    case = Case("scan", [37] * 60, 1024, state=state, dtype=dtype, gate=True, initial=True, final=True)
+    assert case.call(pd.cuda_call).explain(*case.operands()).items_per_thread == 2
+    forward, _ = run(case, grad=False)
+    check(case, case.forward_names(), forward, case.oracle(grad=False))
+
+
 def test_conv_many_runs():
     for flags in (dict(), dict(packed=True, lead=2, spare=3, initial=True, final=True)):
         compare(Case("conv", [900, 900] if not flags else [700, 1, 0, 1100], 72, **flags))
