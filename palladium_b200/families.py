@@ -454,7 +454,8 @@ def selective_scan_grad(length: int, state: int = 16, *, groups: int = 1, softpl
     Outputs: dx, ddelta, dA float32, dB, dC, then dbias and dskip float32, dz and
     dinitial float32 where the constants have them.  B and C are shared by the channels of
     a group and the parameters by all tokens: their sums are float32 in a fixed order, so
-    equal calls on one device give equal bits."""
+    equal calls on one device give equal bits.  Scratch: about 8 bytes per token, state and
+    block of up to 24 channels (`call.explain(...).scratch_bytes` says how much)."""
     return _scan_family("selective_scan_grad", length, state, groups, softplus, bias, skip, gate, initial, final, False,
                         packed, dtype)
 

@@ -314,8 +314,8 @@ def test_offsets_outside_the_rows_are_clamped():
 
 def test_empty_calls():
     for kind in ("conv", "scan"):
-        for lengths in ([0, 0], []):
-            case = Case(kind, lengths, 6, initial=True, final=True)
+        for lengths, packed in (([0, 0], False), ([], False), ([0, 0], True), ([], True)):
+            case = Case(kind, lengths, 6, packed=packed, initial=True, final=True)
             forward, grads = run(case)
             assert forward[0].size == 0 and np.array_equal(forward[1], case.v["initial"].astype(np.float32))
             named = dict(zip(case.grad_names(), grads))
