@@ -613,20 +613,8 @@ __device__ __forceinline__ float sum_lanes(float v) {
     return v;
 }
 
-// four elements as stored, fetched ahead of their use
+// four elements as stored
 template <class T> struct Raw4 { T e[4]; };
-template <class T>
-__device__ __forceinline__ Raw4<T> fetch4(const T* p, bool vec, int n) {
-    Raw4<T> r;
-    if (vec && n == 4) {
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(r.e) = *reinterpret_cast<const uint4*>(p);
-        else *reinterpret_cast<uint2*>(r.e) = *reinterpret_cast<const uint2*>(p);
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.e[i] = i < n ? p[i] : T(0.0f);
-    }
-    return r;
-}
 template <class T>
 __device__ __forceinline__ void put4(T* p, bool vec, int n, const float (&v)[4]) {
     if (vec && n == 4) {
@@ -641,7 +629,7 @@ __device__ __forceinline__ void put4(T* p, bool vec, int n, const float (&v)[4])
     }
 }
 
-// The same straight to shared memory: asynchronous where it is one aligned access of a whole vector.
+// To shared memory: asynchronous where it is one aligned access of a whole vector; the first n, zeros for the rest.
 template <class T>
 __device__ __forceinline__ void copy4(T* to, const T* from, bool vec, int n) {
     if (vec && n == 4) {
