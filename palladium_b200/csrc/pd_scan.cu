@@ -672,6 +672,14 @@ __device__ __forceinline__ float decay(float d, float rate) {
     return expf(d * rate);
 #endif
 }
+// exp(total A) v over many tokens at once.  The factor may leave float32's range where the product does not (a state
+// of zero, or a small one, that grows): it is then taken as two halves, and a state of zero stays zero.
+__device__ __forceinline__ float carried(float v, float total, float rate) {
+    const float whole = decay(total, rate);
+    if (whole >= 1.1754944e-38f && whole <= 3.4028234e38f) return whole * v;
+    const float half = decay(0.5f * total, rate);
+    return v == 0.0f ? 0.0f : half * (half * v);
+}
 __device__ __forceinline__ pair_t decay2(pair_t d, pair_t rate) {
     float x, y;
     unpack(mul2(d, rate), x, y);
@@ -931,7 +939,7 @@ __global__ void __launch_bounds__(kScanThreads, NCH == 1 ? 5 : 4) pd_selective_s
                 float e[4];
                 load_states(a.ends + (k * a.channels + c) * a.state, first, a.state, e);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) v[i] = decay(total, A[i]) * v[i] + e[i];
+                for (int i = 0; i < 4; ++i) v[i] = carried(v[i], total, A[i]) + e[i];
             }
         }
         rate[j][0] = pack(A[0], A[1]);
