@@ -809,6 +809,22 @@ __device__ __forceinline__ pair_t shift_down(pair_t v, int by) {
     unpack(v, x, y);
     return pack(__shfl_down_sync(kFull, x, by), __shfl_down_sync(kFull, y, by));
 }
+__device__ __forceinline__ pair_t from_lane(pair_t v, int lane) {
+    float x, y;
+    unpack(v, x, y);
+    return pack(__shfl_sync(kFull, x, lane), __shfl_sync(kFull, y, lane));
+}
+// Whether products of the decays `up` of up to TL / 2 token groups stay finite, for all of a warp (decays of negative
+// rates are at most one): an infinite one would turn a state of zero into NaN.
+template <int TL>
+__device__ __forceinline__ bool within_range(const pair_t (&up)[2]) {
+    constexpr float most = TL == 8 ? 2147483648.0f : TL == 16 ? 32768.0f : 128.0f;      // 2^(126 / (TL / 2)) or less
+    static_assert(TL == 8 || TL == 16 || TL == 32, "");
+    float a, b, c, d;
+    unpack(up[0], a, b);
+    unpack(up[1], c, d);
+    return __all_sync(kFull, a <= most && b <= most && c <= most && d <= most);
+}
 // v[i] summed over the K lanes of a group, lane i keeping the i-th sum
 template <int K>
 __device__ __forceinline__ float sum_to_lane(const float (&v)[K], int sub) {
@@ -1403,47 +1419,74 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
                         e[p] = mul2(w[i][p], i == K - 1 ? mul2(C[i][p], gg[i]) : mad2(C[i][p], gg[i], e[p]));
-                // scans over the token groups.  The first group takes in the state kept for the chunk, the last the
-                // gradient that follows it; their decay then counts as zero, so that a group that has seen
-                // everything before it adds nothing more (a shuffle from beyond the edge returns the lane's own value).
                 pair_t in[2];
-#pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    in[p] = h[K][p];
-                    down[p] = up[p];
-                    in[p] = mad2(up[p], tl == 0 ? entry[p] : 0, in[p]);
-                    e[p] = mad2(down[p], tl == TL - 1 ? leave[p] : 0, e[p]);
-                    up[p] = tl == 0 ? 0 : up[p];
-                    down[p] = tl == TL - 1 ? 0 : down[p];
-                }
-#pragma unroll
-                for (int off = 1; off < TL; off *= 2)
+                if (within_range<TL>(up)) {
+                    // scans over the token groups.  The first group takes in the state kept for the chunk, the last the
+                    // gradient that follows it; their decay then counts as zero, so that a group that has seen
+                    // everything before it adds nothing more (a shuffle from beyond the edge returns the lane's own value).
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        in[p] = mad2(up[p], shift_up(in[p], off * LN), in[p]);
-                        e[p] = mad2(down[p], shift_down(e[p], off * LN), e[p]);
-                        if (2 * off < TL) {
-                            up[p] = mul2(up[p], shift_up(up[p], off * LN));
-                            down[p] = mul2(down[p], shift_down(down[p], off * LN));
+                        in[p] = h[K][p];
+                        down[p] = up[p];
+                        in[p] = mad2(up[p], tl == 0 ? entry[p] : 0, in[p]);
+                        e[p] = mad2(down[p], tl == TL - 1 ? leave[p] : 0, e[p]);
+                        up[p] = tl == 0 ? 0 : up[p];
+                        down[p] = tl == TL - 1 ? 0 : down[p];
+                    }
+#pragma unroll
+                    for (int off = 1; off < TL; off *= 2)
+#pragma unroll
+                        for (int p = 0; p < 2; ++p) {
+                            in[p] = mad2(up[p], shift_up(in[p], off * LN), in[p]);
+                            e[p] = mad2(down[p], shift_down(e[p], off * LN), e[p]);
+                            if (2 * off < TL) {
+                                up[p] = mul2(up[p], shift_up(up[p], off * LN));
+                                down[p] = mul2(down[p], shift_down(down[p], off * LN));
+                            }
+                        }
+                    __syncwarp();
+                    if (tl == 0) {
+                        *reinterpret_cast<pair_t*>(kept) = e[0];
+                        *reinterpret_cast<pair_t*>(kept + 2) = e[1];
+                    }
+                    // the true states
+#pragma unroll
+                    for (int p = 0; p < 2; ++p) {
+                        in[p] = shift_up(in[p], LN);
+                        e[p] = shift_down(e[p], LN);
+                        in[p] = tl == 0 ? entry[p] : in[p];
+                        e[p] = tl == TL - 1 ? leave[p] : e[p];
+                        h[0][p] = in[p];
+#pragma unroll
+                        for (int i = 0; i < K; ++i) {
+                            in[p] = mul2(in[p], w[i][p]);
+                            h[i + 1][p] = add2(h[i + 1][p], in[p]);
                         }
                     }
-                __syncwarp();
-                if (tl == 0) {
-                    *reinterpret_cast<pair_t*>(kept) = e[0];
-                    *reinterpret_cast<pair_t*>(kept + 2) = e[1];
-                }
-                // the true states
+                } else {
+                    // growing rates: group after group, token after token, no product of decays
 #pragma unroll
-                for (int p = 0; p < 2; ++p) {
-                    in[p] = shift_up(in[p], LN);
-                    e[p] = shift_down(e[p], LN);
-                    in[p] = tl == 0 ? entry[p] : in[p];
-                    e[p] = tl == TL - 1 ? leave[p] : e[p];
-                    h[0][p] = in[p];
+                    for (int p = 0; p < 2; ++p) {
+                        pair_t now = entry[p];
+#pragma unroll 1
+                        for (int t = 0; t < TL; ++t) {
+                            if (tl == t) h[0][p] = now;
 #pragma unroll
-                    for (int i = 0; i < K; ++i) {
-                        in[p] = mul2(in[p], w[i][p]);
-                        h[i + 1][p] = add2(h[i + 1][p], in[p]);
+                            for (int i = 0; i < K; ++i) now = mad2(w[i][p], now, mul2(u[i], B[i][p]));
+                            now = from_lane(now, t * LN + sub);
+                        }
+#pragma unroll
+                        for (int i = 0; i < K; ++i) h[i + 1][p] = mad2(w[i][p], h[i][p], mul2(u[i], B[i][p]));
+                        now = leave[p];
+#pragma unroll 1
+                        for (int t = TL - 1; t >= 0; --t) {
+                            if (tl == t) e[p] = now;
+#pragma unroll
+                            for (int i = K - 1; i >= 0; --i) now = mul2(w[i][p], mad2(C[i][p], gg[i], now));
+                            now = from_lane(now, t * LN + sub);
+                        }
+                        __syncwarp();
+                        if (tl == 0) *reinterpret_cast<pair_t*>(kept + 2 * p) = now;
                     }
                 }
                 if (GATE)
