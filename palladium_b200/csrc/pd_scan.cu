@@ -1215,37 +1215,7 @@ __global__ void __launch_bounds__(kScanThreads, NCH == 1 ? 5 : 4) pd_selective_s
 // registers on an SM (eight warps of 128 registers a block spilled, 1120 us; operands read where they are used
 // instead of a chunk ahead, 1030 us).
 // ---------------------------------------------------------------------------
-constexpr int kGradWarps = 4, kGradThreads = 32 * kGradWarps;
-
-// (ONE: all states in one slice, and with it all but the channels known when compiling)
-template <int LN, bool ONE>
-struct GradShape {
-    int channels, slices, pad;    // channels per block, slices of 4 LN states, states rounded up
-    // offsets in shared memory: float32 arrays in floats, the chunks as stored behind them in bytes
-    int d, u, g, x, s, z, y, du, dd, carry, rate, entry, dA, red, skip, raw, couplings, bytes;
-    int pitch;                    // elements between two tokens' couplings
-    static constexpr int kRow = PD_SCAN_CHUNK, kWide = 4 * LN;
-    __host__ __device__ GradShape(int state, int per_warp, int element) {
-        channels = kGradWarps * per_warp;
-        slices = ONE ? 1 : (state + kWide - 1) / kWide;
-        pad = slices * kWide;
-        pitch = pad + 4;          // (the token groups' rows then lie in different banks)
-        const int cells = channels * kRow, more = slices > 1 ? cells : 0;
-        d = 0; u = d + 2 * cells; g = u + 2 * cells;     // as pairs of equal halves, which packed operations take
-        x = g + 2 * cells; s = x + cells; z = s + cells;
-        y = z + cells; du = y + more; dd = du + more;
-        carry = dd + more;
-        rate = carry + channels * pad;
-        entry = rate + channels * pad;           // two buffers
-        dA = entry + 2 * channels * pad;
-        red = dA + channels * slices * 128;
-        const int warps = kGradWarps * kRow * (2 * kWide + 4), staged = kGradThreads * 8;   // at different times
-        skip = red + (warps > staged ? warps : staged);
-        raw = (skip + channels) * 4;             // x, delta, dy, z: (4, tokens, channels)
-        couplings = raw + 4 * cells * element;   // two buffers of B and C: (2, 2, tokens, pitch)
-        bytes = couplings + 4 * kRow * pitch * element;
-    }
-};
+constexpr int kGradThreads = 32 * PD_SCAN_GRAD_WARPS;
 
 template <class T, int LN, bool GATE, bool ONE>
 __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel(PdScanArgs a) {
@@ -1253,7 +1223,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
     static_assert(K * TL == kRow, "a warp covers a chunk");
     extern __shared__ float4 smem4[];
     float* smem = reinterpret_cast<float*>(smem4);
-    const GradShape<LN, ONE> G(a.state, a.per_warp, sizeof(T));
+    const PdGradShape<LN, ONE> G(a.state, a.per_warp, sizeof(T));
     float *sX = smem + G.x, *sS = smem + G.s, *sZ = smem + G.z;
     float2 *sD = reinterpret_cast<float2*>(smem + G.d), *sU = reinterpret_cast<float2*>(smem + G.u), *sG = reinterpret_cast<float2*>(smem + G.g);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, sub = lane % LN, tl = lane / LN;
@@ -1548,7 +1518,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
                 const int t = v / (2 * LN), part = v % (2 * LN) * 4;
                 float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-                for (int k2 = 0; k2 < kGradWarps; ++k2) {
+                for (int k2 = 0; k2 < PD_SCAN_GRAD_WARPS; ++k2) {
                     const float4 p = *reinterpret_cast<const float4*>(red + (k2 * kRow + t) * kStep + part);
                     total.x += p.x; total.y += p.y; total.z += p.z; total.w += p.w;
                 }
@@ -1778,7 +1748,7 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
         auto run = [&](auto ln) -> cudaError_t {
             constexpr int LN = decltype(ln)::value;
             const bool one = a.state <= 4 * LN;
-            const GradShape<LN, false> G(a.state, a.per_warp, sizeof(T));
+            const PdGradShape<LN, false> G(a.state, a.per_warp, sizeof(T));
             const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
             const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
             if (blocks > 0) {

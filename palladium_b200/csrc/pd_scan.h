@@ -11,6 +11,8 @@
 
 #include <vector>
 
+#include "../../include/palladium_cuda.h"
+
 // A sequence's tokens are rows of `x`.  Dense calls: sequence s has rows [s * length, (s + 1) * length).
 // Packed calls: rows [offsets[s], offsets[s + 1]), every value clamped to [0, rows], a decreasing pair an
 // empty sequence; whatever the offsets hold, no kernel leaves its arrays.
@@ -86,6 +88,47 @@ inline int pd_step_run(int64_t channels, int groups, int state, int64_t seqs, in
     const int64_t least = (seqs + 65534) / 65535;
     return (int)(run < least ? least : run);
 }
+
+// The gradient kernel's block: four warps' channels, `per_warp` of them one after another in each, and its shared
+// memory.  (ONE: all states in one slice, and with it all but the channels known when compiling)
+constexpr int PD_SCAN_GRAD_WARPS = 4;
+template <int LN, bool ONE>
+struct PdGradShape {
+    int channels, slices, pad;    // channels per block, slices of 4 LN states, states rounded up
+    // offsets in shared memory: float32 arrays in floats, the chunks as stored behind them in bytes
+    int d, u, g, x, s, z, y, du, dd, carry, rate, entry, dA, red, skip, raw, couplings, bytes;
+    int pitch;                    // elements between two tokens' couplings
+    static constexpr int kRow = PD_SCAN_CHUNK, kWide = 4 * LN;
+    __host__ __device__ PdGradShape(int state, int per_warp, int element) {
+        channels = PD_SCAN_GRAD_WARPS * per_warp;
+        slices = ONE ? 1 : (state + kWide - 1) / kWide;
+        pad = slices * kWide;
+        pitch = pad + 4;          // (the token groups' rows then lie in different banks)
+        const int cells = channels * kRow, more = slices > 1 ? cells : 0;
+        d = 0; u = d + 2 * cells; g = u + 2 * cells;     // as pairs of equal halves, which packed operations take
+        x = g + 2 * cells; s = x + cells; z = s + cells;
+        y = z + cells; du = y + more; dd = du + more;
+        carry = dd + more;
+        rate = carry + channels * pad;
+        entry = rate + channels * pad;           // two buffers
+        dA = entry + 2 * channels * pad;
+        red = dA + channels * slices * 128;
+        // at different times: the warps' sums of dB and dC, the staging threads' of dbias and dskip
+        const int warps = PD_SCAN_GRAD_WARPS * kRow * (2 * kWide + 4), staged = 32 * PD_SCAN_GRAD_WARPS * 8;
+        skip = red + (warps > staged ? warps : staged);
+        raw = (skip + channels) * 4;             // x, delta, dy, z: (4, tokens, channels)
+        couplings = raw + 4 * cells * element;   // two buffers of B and C: (2, 2, tokens, pitch)
+        bytes = couplings + 4 * kRow * pitch * element;
+    }
+};
+inline int pd_scan_grad_bytes(int state, int per_warp, int element) {
+    const int lanes = pd_scan_slice_lanes(state);
+    if (lanes == 1) return PdGradShape<1, false>(state, per_warp, element).bytes;
+    if (lanes == 2) return PdGradShape<2, false>(state, per_warp, element).bytes;
+    return PdGradShape<4, false>(state, per_warp, element).bytes;
+}
+// Blocks of that much shared memory on an SM: it has 228 KB, of which each block takes 1 KB more than it asks for.
+inline int pd_scan_resident(int bytes) { return 228 * 1024 / (bytes + 1024); }
 
 struct PdScanTable {
     cudaError_t (*conv)(const PdConvArgs&, cudaStream_t);

@@ -81,17 +81,22 @@ int64_t conv_partial(const Dims& d, int64_t width, int64_t row_blocks) { return 
 int64_t scan_chunks(const pd_selective_scan_params* p, const Dims& d) {
     return p->packed ? p->length / PD_SCAN_CHUNK + d.seqs : d.seqs * ((p->length + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK);
 }
-// Channels a warp of the gradient kernel takes one after another (a block is four warps, three blocks an SM).
-// More of them share one sum over the block's warps and one partial sum of dB and dC in memory, worth about one
-// channel's work per chunk; fewer give more blocks.  The smallest product of waves and work per wave wins.
+// Channels a warp of the gradient kernel takes one after another (a block is four warps, three blocks an SM where
+// shared memory allows).  More of them share one sum over the block's warps and one partial sum of dB and dC in memory,
+// worth about one channel's work per chunk, two with more than sixteen states; fewer give more blocks.  The smallest
+// product of waves and work per wave wins, where a wave of two blocks an SM takes nine tenths of one of three, and one
+// of one block eight tenths (4 x 2048 tokens x 2048 channels, one to six channels a warp: bf16 x 16 states 1060, 794,
+// 744, 767, 687, 763 us, of which it takes 687; float32 x 16 states 1031, 765, 716, 751, 810, 908, of which 716).
 int grad_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
-    const int64_t per = d.channels / p->groups, slots = (int64_t)sms * 3;
-    const int most = p->state > 16 ? 4 : 6;    // (shared memory for three blocks; more states need more sums)
+    const int64_t per = d.channels / p->groups;
+    const int most = p->state > 16 ? 4 : 6;    // (the sums' staging has room for six, the wide states' for four)
     int best = 1;
     int64_t least = INT64_MAX;
     for (int n = most; n >= 1; --n) {
+        const int fit = pd_scan_resident(pd_scan_grad_bytes((int)p->state, n, (int)element(p->type)));
+        const int64_t slots = (int64_t)sms * (fit < 3 ? fit : 3), wave = fit >= 3 ? 10 : fit == 2 ? 9 : 8;
         const int64_t blocks = (per + 4 * n - 1) / (4 * n) * p->groups * (d.seqs > 0 ? d.seqs : 1);
-        const int64_t cost = (blocks + slots - 1) / slots * (n + 1);
+        const int64_t cost = (blocks + slots - 1) / slots * (n + (p->state > 16 ? 2 : 1)) * wave;
         if (cost < least) { least = cost; best = n; }
     }
     return best;
