@@ -1261,7 +1261,8 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
     if (tid < G.channels) smem[G.skip + tid] = a.skip && tid < count ? a.skip[c0 + tid] : 0.0f;
     // staging: four channels of a token per thread, always the same channels
     const int quads = G.channels / 4, rows = kGradThreads / quads, c4 = tid % quads * 4;
-    const int st = tid / quads < rows ? tid / quads : kRow;
+    const bool stages = tid < rows * quads;     // (128 threads need not divide into rows: the last ones rest)
+    const int st = stages ? tid / quads : kRow;
     const int left = count - c4 < 0 ? 0 : count - c4 > 4 ? 4 : count - c4;
     float bias[4], dbias[4], dskip[4];
 #pragma unroll
@@ -1563,7 +1564,7 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
         out[c * (a.state + 2) + n] = total;
     }
     float* part = smem + G.red;      // (staging row, channel, 2)
-    if (st < rows)
+    if (stages)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             part[(st * G.channels + c4 + i) * 2] = dbias[i];

@@ -5,6 +5,8 @@ import numpy as np
 import pytest
 
 import palladium_b200 as pd
+from palladium_b200 import families
+from palladium_b200.pl import ShapeDtypeStruct
 from tests.state_space import Case, check
 from tests.test_gpu_state_space import compare, run
 
@@ -59,3 +61,45 @@ def test_gradient_through_tokens_whose_decays_grow(math_mode, state, rate):
             every[:] = 2.0 ** -7
         every[:, rows] = 1.0 if name == "delta" else 0.0
     compare(case, math_mode)
+
+
+# ------------------------------------------------------------------ gradients of several channels per warp
+# (sequences, channels) that are given one to six channels a warp; 128 staging threads divide into neither three, five nor six
+SIZES = [(30, 63, 2), (50, 66, 3), (80, 63, 4), (50, 130, 5), (120, 63, 6)]
+
+
+def _reached(case, items):
+    carries = ShapeDtypeStruct(families.out_shapes(case.family(carries=True), case.grid)[-1].shape, np.float32)
+    return case.call(pd.cuda_call, "_grad").explain(*case.operands(grad=True, carries=carries)).items_per_thread == items
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("state", [3, 8, 16])
+@pytest.mark.parametrize("seqs, channels, items", SIZES)
+@pytest.mark.parametrize("packed", [False, True])
+def test_gradient_with_several_channels_per_warp(packed, seqs, channels, items, state, dtype):
+    if packed:
+        lengths = [(s * 7) % 13 for s in range(seqs)]       # empty ones and single tokens among them
+        lengths[1], lengths[seqs // 2] = 33, 70             # and some of more than one chunk
+    else:
+        lengths = [9] * seqs
+    case = Case("scan", lengths, channels, dtype=dtype, state=state, packed=packed, lead=2 * packed, spare=3 * packed,
+                gate=packed, initial=packed, final=packed, seed=items)
+    if not (dtype == "float32" and state == 16 and items > 4):      # (there shared memory has room for fewer)
+        assert _reached(case, items)
+    compare(case)
+
+
+@pytest.mark.parametrize("dtype, state, seqs, channels, items", [
+    ("bfloat16", 24, 50, 66, 3), ("float32", 24, 50, 66, 4), ("bfloat16", 64, 50, 66, 4), ("float32", 64, 30, 63, 2)])
+def test_gradient_with_several_channels_per_warp_and_slices_of_states(dtype, state, seqs, channels, items):
+    for more in (dict(), dict(gate=True, initial=True, final=True)):
+        case = Case("scan", [5 if more else 34] * seqs, channels, dtype=dtype, state=state, **more)
+        assert _reached(case, items)
+        compare(case)
+
+
+def test_gradient_with_several_channels_per_warp_and_groups():
+    case = Case("scan", [40] * 30, 120, dtype="float32", state=11, groups=3, gate=True, initial=True, final=True)
+    assert _reached(case, 3)
+    compare(case)
