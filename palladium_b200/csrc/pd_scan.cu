@@ -875,22 +875,10 @@ __device__ __forceinline__ void load_pairs(const float2* p, pair_t (&v)[K]) {
 // (STATE) takes each from a zero state to its end state and total step, and the blocks of the second compose the state
 // entering theirs.
 // ---------------------------------------------------------------------------
-constexpr int kScanWarps = 2, kStageThreads = 64, kScanThreads = 32 * kScanWarps + kStageThreads;
+constexpr int kStageThreads = 64, kScanThreads = 32 * PD_SCAN_WALKING_WARPS + kStageThreads;
 
 // all of the block's warps, which reach it from different places
 __device__ __forceinline__ void tile_barrier() { asm volatile("barrier.sync 1, %0;" ::"n"(kScanThreads) : "memory"); }
-
-struct ScanShape {
-    int warp_channels, channels, pad;
-    int du, B, C, y, raw, bytes;      // offsets in floats, from `raw` on in bytes
-    static constexpr int kRow = PD_SCAN_CHUNK;
-    __host__ __device__ constexpr ScanShape(int ln, int nch, int element)
-        : warp_channels(32 / ln * nch), channels(kScanWarps * warp_channels), pad(4 * ln), du(0),
-          // two buffers of each: (tokens, channels) steps and inputs, (tokens, pad) B and C, (tokens, channels) sums
-          B(4 * kRow * channels), C(B + 2 * kRow * pad), y(C + 2 * kRow * pad), raw((y + 2 * kRow * channels) * 4),
-          // as stored: four buffers of x, delta, z, (3, tokens, channels), and two of B and C, (2, tokens, pad)
-          bytes(raw + 12 * kRow * channels * element + 4 * kRow * pad * element) {}
-};
 
 // segments: where a sequence's first one is counted, and the sequence of the id-th (an empty one has one, too)
 __device__ __forceinline__ int64_t dense_segments(const PdScanArgs& a) {
@@ -910,8 +898,8 @@ __device__ __forceinline__ int64_t segment_owner(const PdScanArgs& a, int64_t id
 }
 
 template <class T, int LN, int NCH, bool FULL, bool STATE>
-__global__ void __launch_bounds__(kScanThreads, NCH == 1 ? 5 : 4) pd_selective_scan_kernel(PdScanArgs a) {
-    constexpr ScanShape G(LN, NCH, sizeof(T));
+__global__ void __launch_bounds__(kScanThreads, PdScanShape(LN, NCH, sizeof(T)).resident()) pd_selective_scan_kernel(PdScanArgs a) {
+    constexpr PdScanShape G(LN, NCH, sizeof(T));
     constexpr int kRow = G.kRow, quads = G.channels / 4, kPass = kStageThreads / quads;
     static_assert(kStageThreads % quads == 0 && kRow % kPass == 0 && G.warp_channels % 4 == 0, "staging covers a tile");
     extern __shared__ float4 smem4[];
@@ -936,7 +924,7 @@ __global__ void __launch_bounds__(kScanThreads, NCH == 1 ? 5 : 4) pd_selective_s
     const int64_t start = begin + number * a.segment, stop = start + a.segment < end ? start + a.segment : end;
     if (number < 0 || (number > 0 && start >= end)) return;
     if (STATE && stop == end) return;         // nothing follows a last segment
-    const bool computes = warp < kScanWarps;
+    const bool computes = warp < PD_SCAN_WALKING_WARPS;
     // this lane's channels, their rates and the state entering
     pair_t rate[NCH][2], h[NCH][2];
     const int mine = warp * G.warp_channels + cl * NCH;
@@ -1699,7 +1687,7 @@ cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
             const bool full = a.state == 4 * LN;
             auto run = [&](auto nch) -> cudaError_t {
                 constexpr int NCH = decltype(nch)::value;
-                constexpr ScanShape G(LN, NCH, sizeof(T));
+                constexpr PdScanShape G(LN, NCH, sizeof(T));
                 const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels * a.groups;
                 if (a.ends && a.segments > 0) {
                     auto first = full ? pd_selective_scan_kernel<T, LN, NCH, true, true> : pd_selective_scan_kernel<T, LN, NCH, false, true>;

@@ -89,6 +89,29 @@ inline int pd_step_run(int64_t channels, int groups, int state, int64_t seqs, in
     return (int)(run < least ? least : run);
 }
 
+// Blocks of that much shared memory on an SM: it has 228 KB, of which each block takes 1 KB more than it asks for.
+__host__ __device__ constexpr int pd_scan_resident(int bytes) { return 228 * 1024 / (bytes + 1024); }
+
+// The prompt kernel's block and its shared memory: `ln` lanes a channel, `nch` channels a lane, `element` bytes a value.
+constexpr int PD_SCAN_WALKING_WARPS = 2;
+struct PdScanShape {
+    int lane_channels, warp_channels, channels, pad;    // channels of a lane, of a walking warp, of the block; states rounded up
+    int du, B, C, y, raw, bytes;      // offsets in floats, from `raw` on in bytes
+    static constexpr int kRow = PD_SCAN_CHUNK;
+    __host__ __device__ constexpr PdScanShape(int ln, int nch, int element)
+        : lane_channels(nch), warp_channels(32 / ln * nch), channels(PD_SCAN_WALKING_WARPS * warp_channels), pad(4 * ln), du(0),
+          // two buffers of each: (tokens, channels) steps and inputs, (tokens, pad) B and C, (tokens, channels) sums
+          B(4 * kRow * channels), C(B + 2 * kRow * pad), y(C + 2 * kRow * pad), raw((y + 2 * kRow * channels) * 4),
+          // as stored: four buffers of x, delta, z, (3, tokens, channels), and two of B and C, (2, tokens, pad)
+          bytes(raw + 12 * kRow * channels * element + 4 * kRow * pad * element) {}
+    // the blocks an SM is to hold: what shared memory has room for, five at most (96 registers a thread), four where a
+    // lane has two channels (128)
+    __host__ __device__ constexpr int resident() const {
+        const int most = lane_channels > 1 ? 4 : 5, fit = pd_scan_resident(bytes);
+        return fit < most ? fit : most;
+    }
+};
+
 // The gradient kernel's block: four warps' channels, `per_warp` of them one after another in each, and its shared
 // memory.  (ONE: all states in one slice, and with it all but the channels known when compiling)
 constexpr int PD_SCAN_GRAD_WARPS = 4;
@@ -127,8 +150,6 @@ inline int pd_scan_grad_bytes(int state, int per_warp, int element) {
     if (lanes == 2) return PdGradShape<2, false>(state, per_warp, element).bytes;
     return PdGradShape<4, false>(state, per_warp, element).bytes;
 }
-// Blocks of that much shared memory on an SM: it has 228 KB, of which each block takes 1 KB more than it asks for.
-inline int pd_scan_resident(int bytes) { return 228 * 1024 / (bytes + 1024); }
 
 struct PdScanTable {
     cudaError_t (*conv)(const PdConvArgs&, cudaStream_t);

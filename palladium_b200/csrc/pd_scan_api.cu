@@ -106,7 +106,7 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lan
     return (per + ch - 1) / ch * p->groups;
 }
 // The prompt kernel's channels per lane and segments.  Two channels per lane halve the reads of B and C, one gives
-// twice the blocks and five instead of three of them on an SM: two from 12 blocks per SM on (16 x 1024 tokens x 4096
+// twice the blocks and more of them on an SM (2-byte tokens, 16 states: five instead of three): two from 12 blocks per SM on (16 x 1024 tokens x 4096
 // channels x 16 states: 571 against 604 us; 4 x 2048 x 2048: 211 against 182).  Cutting a sequence into segments
 // costs a first pass over all but its last, which takes two thirds of the second's time: it pays where a call has
 // fewer than two blocks per SM (1 x 8192 x 2048: 16 segments 252 us; 4 x 2048 x 2048: uncut 182 us,
