@@ -201,12 +201,32 @@ __device__ __forceinline__ bool sequence_of(const PdTokens& t, int64_t row, int6
     bounds_of(t, s, begin, end);
     return begin <= row && row < end;
 }
-// f(row) for the rows before the first and behind the last sequence of a packed call
-template <class F>
-__device__ __forceinline__ void for_free_rows(const PdTokens& t, F f) {
-    const int64_t head = clamp_row(t.offsets[0], t.rows), tail = clamp_row(t.offsets[t.seqs], t.rows);
-    for (int64_t r = 0; r < head; ++r) f(r);
-    for (int64_t r = tail < head ? head : tail; r < t.rows; ++r) f(r);
+// Rows of no sequence in a packed call: those before the first one, [0, head), and behind the last one, [tail, rows).
+__device__ __forceinline__ void free_rows(const PdTokens& t, int64_t& head, int64_t& tail) {
+    head = clamp_row(t.offsets[0], t.rows);
+    tail = clamp_row(t.offsets[t.seqs], t.rows);
+    if (tail < head) tail = head;
+}
+// a block's share, one of `parts`, of n elements set to zero
+template <class T>
+__device__ __forceinline__ void clear_share(T* p, int64_t n, int64_t part, int64_t parts) {
+    constexpr int V = 16 / sizeof(T);
+    const int64_t share = ((n + parts - 1) / parts + V - 1) / V * V, from = part * share;
+    if (from >= n) return;
+    const int64_t to = from + share < n ? from + share : n;
+    const int64_t up = from + (int64_t)(-reinterpret_cast<uintptr_t>(p + from) & 15) / (int64_t)sizeof(T);
+    const int64_t low = up < to ? up : to, high = low + (to - low) / V * V;      // 16-byte stores in [low, high)
+    for (int64_t i = from + threadIdx.x; i < low; i += blockDim.x) store1(p + i, 0.0f);
+    for (int64_t i = low + (int64_t)threadIdx.x * V; i < high; i += (int64_t)blockDim.x * V)
+        *reinterpret_cast<uint4*>(p + i) = make_uint4(0, 0, 0, 0);
+    for (int64_t i = high + threadIdx.x; i < to; i += blockDim.x) store1(p + i, 0.0f);
+}
+template <class T>
+__device__ __forceinline__ void clear_free_rows(const PdTokens& t, int64_t channels, T* p, int64_t part, int64_t parts) {
+    int64_t head, tail;
+    free_rows(t, head, tail);
+    clear_share(p, head * channels, part, parts);
+    clear_share(p + tail * channels, (t.rows - tail) * channels, part, parts);
 }
 // where the state entering each chunk of a sequence is kept
 __device__ __forceinline__ int64_t first_chunk(const PdTokens& t, int64_t s, int64_t begin) {
@@ -910,10 +930,8 @@ __global__ void __launch_bounds__(kScanThreads, PdScanShape(LN, NCH, sizeof(T)).
     const int64_t group = a.groups == 1 ? 0 : tile / tiles, within = (tile - group * tiles) * G.channels;
     const int64_t c0 = group * per + within;                            // the block's first channel
     const int count = (int)(per - within < G.channels ? per - within : G.channels);
-    if (id == a.segments) {     // (packed calls: one more)
-        for_free_rows(a.tok, [&](int64_t r) {
-            for (int c = tid; c < count; c += kScanThreads) store1((T*)a.y + r * a.channels + c0 + c, 0.0f);
-        });
+    if (id >= a.segments) {     // (packed calls: a few more)
+        clear_free_rows(a.tok, a.channels, (T*)a.y, (id - a.segments) * all + tile, a.free_blocks * all);
         return;
     }
     const int64_t s = segment_owner(a, id);
@@ -1221,17 +1239,6 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
     const int64_t c0 = group * per + within;
     const int count = (int)(per - within < G.channels ? per - within : G.channels);
     float* bc_out = a.partial_bc + job % (tiles * a.groups) * a.tok.rows * 2 * G.pad;
-    if (s == a.tok.seqs) {
-        for_free_rows(a.tok, [&](int64_t r) {
-            for (int c = tid; c < count; c += kGradThreads) {
-                store1((T*)a.dx + r * a.channels + c0 + c, 0.0f);
-                store1((T*)a.ddelta + r * a.channels + c0 + c, 0.0f);
-                if (a.dz) store1((T*)a.dz + r * a.channels + c0 + c, 0.0f);
-            }
-            for (int i = tid; i < 2 * G.pad; i += kGradThreads) bc_out[r * 2 * G.pad + i] = 0.0f;
-        });
-        return;
-    }
     int64_t begin, end;
     bounds_of(a.tok, s, begin, end);
     // swizzled places of (channel, token): four channels of a token and four tokens of a channel are both
@@ -1576,6 +1583,11 @@ __global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArg
     const int n = (int)(at - r * 2 * pad), which = n >= pad, first = n - which * pad;
     const float* p = a.partial_bc + g * tiles * wide + at;
     float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (a.tok.offsets) {        // no tile has sums of a row of no sequence
+        int64_t head, tail;
+        free_rows(a.tok, head, tail);
+        if (r < head || r >= tail) tiles = 0;
+    }
 #pragma unroll 8
     for (int t = 0; t < tiles; ++t) {
         const float4 q = *reinterpret_cast<const float4*>(p + t * wide);
@@ -1587,9 +1599,18 @@ __global__ void __launch_bounds__(256) pd_selective_scan_sum_bc_kernel(PdScanArg
     for (int i = 0; i < 4; ++i) if (first + i < a.state) store1(to + first + i, v[i]);
 }
 
+// dA, dbias and dskip: the sequences added up in order; the blocks behind clear the rows of no sequence
+template <class T>
 __global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdScanArgs a) {
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     const int64_t wide = a.channels * (a.state + 2);
+    const int64_t part = blockIdx.x - (int64_t)(gridDim.x - a.free_blocks);
+    if (part >= 0) {
+        clear_free_rows(a.tok, a.channels, (T*)a.dx, part, a.free_blocks);
+        clear_free_rows(a.tok, a.channels, (T*)a.ddelta, part, a.free_blocks);
+        if (a.dz) clear_free_rows(a.tok, a.channels, (T*)a.dz, part, a.free_blocks);
+        return;
+    }
     if (i >= wide) return;
     float total = 0.0f;
 #pragma unroll 4
@@ -1697,7 +1718,7 @@ cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
                     err = cudaGetLastError();
                     if (err != cudaSuccess) return err;
                 }
-                const int64_t blocks = tiles * (a.segments + (a.tok.offsets ? 1 : 0));
+                const int64_t blocks = tiles * (a.segments + a.free_blocks);
                 if (blocks == 0) return cudaSuccess;
                 auto kernel = full ? pd_selective_scan_kernel<T, LN, NCH, true, false> : pd_selective_scan_kernel<T, LN, NCH, false, false>;
                 cudaError_t err = allow_smem(kernel, G.bytes);
@@ -1739,7 +1760,7 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
             const bool one = a.state <= 4 * LN;
             const PdGradShape<LN, false> G(a.state, a.per_warp, sizeof(T));
             const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
-            const int64_t blocks = tiles * a.groups * (a.tok.seqs + (a.tok.offsets ? 1 : 0));
+            const int64_t blocks = tiles * a.groups * a.tok.seqs;
             if (blocks > 0) {
                 auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true, true> : pd_selective_scan_grad_kernel<T, LN, false, true>;
                 if constexpr (LN == 4)
@@ -1757,7 +1778,7 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
                 cudaError_t err = cudaGetLastError();
                 if (err != cudaSuccess) return err;
             }
-            pd_selective_scan_sum_params_kernel<<<(unsigned)blocks_for(a.channels * (a.state + 2), 128), 128, 0, st>>>(a);
+            pd_selective_scan_sum_params_kernel<T><<<(unsigned)(blocks_for(a.channels * (a.state + 2), 128) + a.free_blocks), 128, 0, st>>>(a);
             return cudaGetLastError();
         };
         return a.state <= 4 ? run(Int<1>()) : a.state <= 8 ? run(Int<2>()) : run(Int<4>());

@@ -57,6 +57,7 @@ struct PdScanArgs {
     // (segments, channels, state), and total steps, (segments, channels); null where no sequence is cut
     int64_t segment, segments;
     float *ends, *totals;
+    int64_t free_blocks;      // packed: blocks that clear the rows of no sequence; prompts: for each tile of channels
 };
 
 // Lanes that share one channel: each holds four states.
@@ -168,6 +169,7 @@ struct PdScanPlan {
     const char* kernel_name = "";
     int64_t grid = 1, grid_y = 1, block = 1, items = 1, launches = 1, scratch_bytes = 0, dynamic_smem = 0;
     int64_t segment = 1, segments = 0, totals_offset = 0;    // prompts: see PdScanArgs
+    int64_t free_blocks = 0;      // see PdScanArgs
     int64_t row_blocks = 0;       // gradient of the convolution: blocks along the rows
     int64_t params_offset = 0;    // gradient of the scan: where in the scratch the parameters' sums begin
     std::vector<size_t> in_bytes, out_bytes;

@@ -101,6 +101,13 @@ int grad_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
     }
     return best;
 }
+// How many blocks of a packed call, per tile of channels, clear the rows of no sequence, which only the device knows:
+// one for every 128 KB that a token array holds, two per SM at most.
+int64_t scan_free_blocks(const pd_selective_scan_params* p, const Dims& d, int64_t tiles, int sms) {
+    if (!p->packed) return 0;
+    const int64_t most = (int64_t)sms * 2, want = (int64_t)(d.cells * element(p->type) >> 17) + 1;
+    return ((want < most ? want : most) + tiles - 1) / tiles;
+}
 int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lane) {
     const int64_t per = d.channels / p->groups, ch = 2 * 32 / pd_scan_lanes((int)p->state) * per_lane;
     return (per + ch - 1) / ch * p->groups;
@@ -217,7 +224,6 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
     if (p->skip) in.push_back(vec);
     if (p->gate) in.push_back(tokens);
     plan->block = 128;
-    const int64_t free_rows = p->packed ? 1 : 0;
     if (step) {
         out = {tokens, edge};
         plan->kernel_name = "pd_selective_scan_step_kernel";
@@ -231,10 +237,14 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         // one block per tile of channels and sequence
         const int64_t per = d.channels / p->groups;
         plan->items = grad_per_warp(p, d, sms);
-        plan->grid = (per + 4 * plan->items - 1) / (4 * plan->items) * p->groups * (d.seqs + free_rows);
+        const int64_t tiles = (per + 4 * plan->items - 1) / (4 * plan->items) * p->groups;
+        plan->free_blocks = scan_free_blocks(p, d, 1, sms);      // (in the launch that adds up the parameters' sums)
+        plan->grid = tiles * d.seqs;
     } else {
         scan_cut(p, d, sms, plan);
-        plan->grid = scan_tiles(p, d, (int)plan->items) * (plan->segments + free_rows);
+        const int64_t tiles = scan_tiles(p, d, (int)plan->items);
+        plan->free_blocks = scan_free_blocks(p, d, tiles, sms);
+        plan->grid = tiles * (plan->segments + plan->free_blocks);
         plan->block = 128;
         if (d.rows > plan->segment) {
             // (a dense call is cut only where a sequence is longer than a segment)
@@ -403,6 +413,7 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         for (const void* t : tokens) if (reinterpret_cast<uintptr_t>(t) % four) a.vec = 0;
         a.vec_states = a.state % 4 == 0 && reinterpret_cast<uintptr_t>(a.B) % four == 0 && reinterpret_cast<uintptr_t>(a.C) % four == 0;
         a.per_warp = a.run = (int)plan.items;
+        a.free_blocks = plan.free_blocks;
         a.vec_params = a.state % 4 == 0 && aligned16(a.A) && aligned16(a.carries_in) && aligned16(a.initial) && aligned16(a.carries) && aligned16(a.final_state) &&
                        aligned16(a.ends);
         e = step ? table->scan_step(a, st) : grad ? table->scan_grad(a, st) : table->scan(a, st);
