@@ -19,10 +19,13 @@ import numpy as np
 __all__ = ["BlockSpec", "ShapeDtypeStruct", "as_dtype", "bfloat16", "dtype_name"]
 
 bfloat16 = np.dtype([("bfloat16", np.uint16)])
+_NAMES: dict[np.dtype, str] = {}
 
 
 def as_dtype(dtype) -> np.dtype:
     """`np.dtype(dtype)`, with every way of writing bfloat16 read as `pl.bfloat16`."""
+    if isinstance(dtype, np.dtype) and dtype.kind != "V":
+        return dtype        # (what every call on host arrays asks for each of them; ml_dtypes' types are of kind V)
     if str(dtype).rsplit(".", 1)[-1] == "bfloat16" or getattr(dtype, "__name__", "") == "bfloat16":
         return bfloat16
     try:
@@ -32,7 +35,12 @@ def as_dtype(dtype) -> np.dtype:
 
 
 def dtype_name(dtype: np.dtype) -> str:
-    return "bfloat16" if dtype == bfloat16 else dtype.name
+    if dtype.kind == "V" and dtype == bfloat16:
+        return "bfloat16"
+    name = _NAMES.get(dtype)
+    if name is None:
+        name = _NAMES[dtype] = dtype.name      # (NumPy spells it out anew each time, 4 us)
+    return name
 
 
 @dataclasses.dataclass(frozen=True)
