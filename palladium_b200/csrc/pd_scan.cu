@@ -692,14 +692,6 @@ __device__ __forceinline__ float decay(float d, float rate) {
     return expf(d * rate);
 #endif
 }
-// exp(total A) v over many tokens at once.  The factor may leave float32's range where the product does not (a state
-// of zero, or a small one, that grows): it is then taken as two halves, and a state of zero stays zero.
-__device__ __forceinline__ float carried(float v, float total, float rate) {
-    const float whole = decay(total, rate);
-    if (whole >= 1.1754944e-38f && whole <= 3.4028234e38f) return whole * v;
-    const float half = decay(0.5f * total, rate);
-    return v == 0.0f ? 0.0f : half * (half * v);
-}
 __device__ __forceinline__ pair_t decay2(pair_t d, pair_t rate) {
     float x, y;
     unpack(mul2(d, rate), x, y);
@@ -710,16 +702,22 @@ __device__ __forceinline__ pair_t decay2(pair_t d, pair_t rate) {
 #endif
 }
 
-// The same for the gradients, whose sums over thousands of tokens carry a decay's own error along: near one, where a
-// state remembers for long, the approximate power's 2^-22 is four times a rounding.  There, |d A log2(e)| < 0.1, the
-// series of 2^v to the fourth power takes its place; it ends 1.3e-8 short of the sum.
+// The same where a decay's own error matters: in the gradients, whose sums over thousands of tokens carry it along, in
+// single steps, whose state comes back thousands of times, and in prompts of float32 tokens.  Near one, where a state
+// remembers for long, the approximate power's 2^-22 is four times a rounding.  There, |d A log2(e)| < 0.1, the series of
+// 2^v to the fourth power takes its place; it ends 1.3e-8 short of the sum.  (Decays around 1 - 1e-2, 4096 tokens, error
+// of the last state: 1.4e-6 with the approximate power, 2.1e-7 with the series, 2.9e-7 in SAFE; fed back step by step
+// 2.8e-6, 2.6e-7, 4.3e-7.  It takes a float32 prompt of 4 x 2048 x 2048 x 16 from 194 to 223 us, one of 32 x 512 x 4096
+// x 16, which fills the GPU, from 680 to 911; 2-byte tokens, whose inputs are 2^-9 off, keep the approximate power: the
+// series would take the first from 186 to 221 us.)
+constexpr float kPower1 = 0.6931471805599453f, kPower2 = 0.2402265069591007f, kPower3 = 0.0555041086648216f,
+                kPower4 = 0.0096181291076285f;
 __device__ __forceinline__ pair_t decay2_fine(pair_t d, pair_t rate) {
 #if PD_MODE == 2
     const pair_t v = mul2(d, rate);
-    const float c1 = 0.6931471805599453f, c2 = 0.2402265069591007f, c3 = 0.0555041086648216f, c4 = 0.0096181291076285f;
-    pair_t p = mad2(pack(c4, c4), v, pack(c3, c3));
-    p = mad2(p, v, pack(c2, c2));
-    p = mad2(p, v, pack(c1, c1));
+    pair_t p = mad2(pack(kPower4, kPower4), v, pack(kPower3, kPower3));
+    p = mad2(p, v, pack(kPower2, kPower2));
+    p = mad2(p, v, pack(kPower1, kPower1));
     p = mad2(p, v, pack(1.0f, 1.0f));
     float x, y, px, py;
     unpack(v, x, y);
@@ -728,6 +726,24 @@ __device__ __forceinline__ pair_t decay2_fine(pair_t d, pair_t rate) {
 #else
     return decay2(d, rate);
 #endif
+}
+__device__ __forceinline__ float decay_fine(float d, float rate) {
+#if PD_MODE == 2
+    const float v = d * rate;
+    const float p = fmaf(fmaf(fmaf(fmaf(kPower4, v, kPower3), v, kPower2), v, kPower1), v, 1.0f);
+    return fabsf(v) < 0.1f ? p : exp2_approx(v);
+#else
+    return decay(d, rate);
+#endif
+}
+
+// exp(total A) v over many tokens at once.  The factor may leave float32's range where the product does not (a state
+// of zero, or a small one, that grows): it is then taken as two halves, and a state of zero stays zero.
+__device__ __forceinline__ float carried(float v, float total, float rate) {
+    const float whole = decay_fine(total, rate);
+    if (whole >= 1.1754944e-38f && whole <= 3.4028234e38f) return whole * v;
+    const float half = decay(0.5f * total, rate);
+    return v == 0.0f ? 0.0f : half * (half * v);
 }
 
 // One token per sequence; state in and out may be the same memory.  Bound: the states, read and written once, 8
@@ -795,7 +811,7 @@ __global__ void __launch_bounds__(256) pd_selective_scan_step_kernel(PdScanArgs 
 #pragma unroll
         for (int i = 0; i < kStates; ++i) {
             const bool in = VEC || first + i < a.state;
-            h[i] = decay(d, A[i]) * now.h[i] + (in ? u * now.B[i] : 0.0f);
+            h[i] = decay_fine(d, A[i]) * now.h[i] + (in ? u * now.B[i] : 0.0f);
             y += in ? now.C[i] * h[i] : 0.0f;
         }
         y = sum_lanes<LN>(y);
@@ -1144,8 +1160,8 @@ __global__ void __launch_bounds__(kScanThreads, PdScanShape(LN, NCH, sizeof(T)).
 #pragma unroll
                 for (int j = 0; j < NCH; ++j) {
                     const pair_t step = pack(q.d[i][j], q.d[i][j]), in = pack(q.u[i][j], q.u[i][j]);
-                    w[i][j][0] = decay2(step, rate[j][0]);
-                    w[i][j][1] = decay2(step, rate[j][1]);
+                    w[i][j][0] = sizeof(T) == 4 ? decay2_fine(step, rate[j][0]) : decay2(step, rate[j][0]);
+                    w[i][j][1] = sizeof(T) == 4 ? decay2_fine(step, rate[j][1]) : decay2(step, rate[j][1]);
                     b[i][j][0] = mul2(in, q.B[i].x);
                     b[i][j][1] = mul2(in, q.B[i].y);
                     if (!FULL) {     // states beyond the last one stay zero whatever the input is

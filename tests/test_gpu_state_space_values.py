@@ -64,6 +64,40 @@ def test_gradient_through_tokens_whose_decays_grow(math_mode, state, rate):
     compare(case, math_mode)
 
 
+# ------------------------------------------------------------------ states that remember for long
+def test_fast_decays_near_one_are_as_exact_as_safe_ones():
+    """4096 tokens of float32 with decays around 1 - 1e-2: FAST's series is off by half a rounding of a value below one
+    (2^-25) and a hundredth of what its argument is, SAFE's exponential by up to two, so the errors of what thousands of
+    them make, against float64, may not be larger.  (Factor 1.5: both are sums of signed errors.)"""
+    torch.manual_seed(2)
+    s, n, d, k = 2, 4096, 32, 16
+    step = 0.02 * torch.rand(s, n, d, device="cuda")
+    A = -(0.5 + torch.rand(d, k, device="cuda"))
+    x = torch.randn(s, n, d, device="cuda").abs()
+    B, C = (torch.randn(s, n, 1, k, device="cuda").abs() for _ in range(2))
+    h = torch.randn(s, d, k, device="cuda")
+    plain = dict(softplus=False, bias=False, skip=False)
+    want, ys = h.double(), []
+    for t in range(n):
+        at = step[:, t].double()
+        want = torch.exp(at[..., None] * A.double()) * want + (at * x[:, t].double())[..., None] * B[:, t].double()
+        ys.append((want * C[:, t].double()).sum(-1))
+    want = {"y": torch.stack(ys, 1), "final": want, "stepped": want}
+
+    def errors(math_mode):
+        make = lambda f: pd.cuda_call_jit(f, grid=(s, d), out_shape=families.out_shapes(f, (s, d)), math_mode=math_mode)  # noqa: E731
+        y, final = make(families.selective_scan(n, k, initial=True, final=True, **plain))(x, step, A, B, C, h)
+        one, state = make(families.selective_scan_step(k, **plain)), h
+        for t in range(n):
+            _, state = one(state, *[v[:, t].contiguous() for v in (x, step)], A, *[v[:, t].contiguous() for v in (B, C)])
+        got = {"y": y, "final": final, "stepped": state}
+        return {name: float((got[name].double() - want[name]).norm() / want[name].norm()) for name in want}
+
+    fast, safe = errors("fast"), errors("safe")
+    for name in want:
+        assert fast[name] <= 1.5 * safe[name], (name, fast, safe)
+
+
 # ------------------------------------------------------------------ gradients of several channels per warp
 # (sequences, channels) that are given one to six channels a warp; 128 staging threads divide into neither three, five nor six
 SIZES = [(30, 63, 2), (50, 66, 3), (80, 63, 4), (50, 130, 5), (120, 63, 6)]
