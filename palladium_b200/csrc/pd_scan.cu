@@ -1643,9 +1643,12 @@ __global__ void __launch_bounds__(128) pd_selective_scan_sum_params_kernel(PdSca
 // ---------------------------------------------------------------------------
 int64_t blocks_for(int64_t threads, int block) { return (threads + block - 1) / block; }
 
+// Up to 48 KB of shared memory need no leave; beyond, a kernel is given all that a block may have, always the same: calls
+// of other sizes on other threads share its limit, and one that lowered it would have the next launch refused.
 template <class K>
-cudaError_t allow_smem(K kernel, int bytes) {     // up to 48 KB need no leave
-    return bytes <= 48 * 1024 ? cudaSuccess : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+cudaError_t allow_smem(K kernel, int bytes) {
+    return bytes <= 48 * 1024 ? cudaSuccess
+                              : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
 }
 
 template <class F>

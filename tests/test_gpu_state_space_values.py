@@ -9,7 +9,7 @@ import palladium_b200 as pd
 from palladium_b200 import families
 from palladium_b200.pl import ShapeDtypeStruct
 from tests.state_space import Case, check
-from tests.test_gpu_state_space import compare, run
+from tests.test_gpu_state_space import back, compare, device, run
 
 pytestmark = pytest.mark.gpu
 
@@ -179,3 +179,40 @@ def test_a_packed_call_takes_no_longer_for_rows_of_no_sequence_than_writing_them
 
     small, large = best(256), best(8192)
     assert large[0] < 12 * small[0] and large[1] < 8 * small[1], (small, large)
+
+
+# ------------------------------------------------------------------ calls at once
+def test_gradients_of_different_block_sizes_from_several_threads():
+    """One kernel with two to six channels a warp, so with different amounts of shared memory, launched by six threads at
+    once: no call takes another one's leave for shared memory away, and each gives its own result."""
+    import threading
+
+    made = []
+    for seqs, channels in ((30, 63), (50, 66), (80, 63), (50, 130), (120, 63), (2, 8)):
+        case = Case("scan", [40] * seqs, channels, dtype="bfloat16", state=16, gate=True)
+        *_, carries = case.call(pd.cuda_call_jit, carries=True)(*[device(a) for a in case.operands()])
+        operands = [device(a) for a in case.operands(grad=True, carries=back(carries))]
+        call = case.call(pd.cuda_call_jit, "_grad")
+        made.append((call, operands, call(*operands)))
+    torch.cuda.synchronize()
+    wrong, start = [], threading.Barrier(len(made))
+
+    def work(i):
+        call, operands, want = made[i]
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                start.wait()
+                for _ in range(200):
+                    got = call(*operands)
+                torch.cuda.current_stream().synchronize()
+            if not all(torch.equal(a, b) for a, b in zip(got, want)):
+                wrong.append((i, "other bits"))
+        except Exception as e:
+            wrong.append((i, e))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(made))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
