@@ -1821,6 +1821,12 @@ int pd_explain(int family, const void* params, size_t params_bytes, int math_mod
         info->static_smem_bytes = plan.rtc.static_smem;
         info->blocks_per_sm = plan.rtc.blocks_per_sm;
     }
+    if (dev.present && pd_is_scan_family(family)) {
+        const PdScanReport said = pd_scan_describe(family, params, math_mode, grid, plan.scan);
+        info->regs_per_thread = said.registers;
+        info->static_smem_bytes = said.static_smem;
+        info->blocks_per_sm = said.blocks_per_sm;
+    }
     if (dev.present && plan.kernel) {
         cudaFuncAttributes attr;
         if (cudaFuncGetAttributes(&attr, plan.kernel) == cudaSuccess) {

@@ -1651,6 +1651,23 @@ cudaError_t allow_smem(K kernel, int bytes) {
                               : cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
 }
 
+template <class K>
+cudaError_t describe(K kernel, int threads, int bytes, PdScanReport* to) {
+    cudaFuncAttributes attr;
+    cudaError_t err = allow_smem(kernel, bytes);
+    if (err == cudaSuccess) err = cudaFuncGetAttributes(&attr, kernel);
+    int blocks = 0;
+    if (err == cudaSuccess) err = cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kernel, threads, bytes);
+    if (err != cudaSuccess) {
+        cudaGetLastError();
+        return err;
+    }
+    to->registers = attr.numRegs;
+    to->static_smem = (int)attr.sharedSizeBytes;
+    to->blocks_per_sm = blocks;
+    return cudaSuccess;
+}
+
 template <class F>
 cudaError_t by_type(int type, F f) {
     if (type == PD_TYPE_F32) return f(float());
@@ -1687,9 +1704,10 @@ cudaError_t launch_conv(const PdConvArgs& a, cudaStream_t st) {
         using T = decltype(e);
         const int64_t lanes = (a.channels + v.value - 1) / v.value;
         const int64_t jobs = (a.tok.rows + a.run - 1) / a.run + (a.final_state ? a.tok.seqs : 0);
-        if (lanes * jobs == 0) return cudaSuccess;
         constexpr int W = decltype(w)::value, V = decltype(v)::value;
         auto kernel = a.silu ? pd_causal_conv_kernel<T, W, V, true> : pd_causal_conv_kernel<T, W, V, false>;
+        if (a.report) return describe(kernel, 256, 0, a.report);
+        if (lanes * jobs == 0) return cudaSuccess;
         kernel<<<(unsigned)blocks_for(lanes * jobs, 256), 256, 0, st>>>(a);
         return cudaGetLastError();
     });
@@ -1698,9 +1716,11 @@ cudaError_t launch_conv_step(const PdConvArgs& a, cudaStream_t st) {
     return by_conv(a, [&](auto e, auto w, auto v) {
         using T = decltype(e);
         const int64_t lanes = (a.channels + v.value - 1) / v.value;
+        auto kernel = pd_causal_conv_step_kernel<T, decltype(w)::value, decltype(v)::value>;
+        if (a.report) return describe(kernel, 128, 0, a.report);
         if (a.tok.seqs == 0) return cudaSuccess;
         const dim3 grid((unsigned)blocks_for(lanes, 128), (unsigned)(a.tok.seqs < 65535 ? a.tok.seqs : 65535));
-        pd_causal_conv_step_kernel<T, decltype(w)::value, decltype(v)::value><<<grid, 128, 0, st>>>(a);
+        kernel<<<grid, 128, 0, st>>>(a);
         return cudaGetLastError();
     });
 }
@@ -1711,6 +1731,7 @@ cudaError_t launch_conv_grad(const PdConvArgs& a, cudaStream_t st) {
         const int64_t lanes = (a.channels + V - 1) / V;
         const dim3 block(32, 8), grid((unsigned)blocks_for(lanes, 32), (unsigned)a.row_blocks);
         auto kernel = a.silu ? pd_causal_conv_grad_kernel<T, W, V, true> : pd_causal_conv_grad_kernel<T, W, V, false>;
+        if (a.report) return describe(kernel, 256, 256 * V * sizeof(float), a.report);
         kernel<<<grid, block, 256 * V * sizeof(float), st>>>(a);
         cudaError_t err = cudaGetLastError();
         if (err != cudaSuccess) return err;
@@ -1729,6 +1750,8 @@ cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
                 constexpr int NCH = decltype(nch)::value;
                 constexpr PdScanShape G(LN, NCH, sizeof(T));
                 const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels * a.groups;
+                auto kernel = full ? pd_selective_scan_kernel<T, LN, NCH, true, false> : pd_selective_scan_kernel<T, LN, NCH, false, false>;
+                if (a.report) return describe(kernel, kScanThreads, G.bytes, a.report);
                 if (a.ends && a.segments > 0) {
                     auto first = full ? pd_selective_scan_kernel<T, LN, NCH, true, true> : pd_selective_scan_kernel<T, LN, NCH, false, true>;
                     cudaError_t err = allow_smem(first, G.bytes);
@@ -1739,7 +1762,6 @@ cudaError_t launch_scan(const PdScanArgs& a, cudaStream_t st) {
                 }
                 const int64_t blocks = tiles * (a.segments + a.free_blocks);
                 if (blocks == 0) return cudaSuccess;
-                auto kernel = full ? pd_selective_scan_kernel<T, LN, NCH, true, false> : pd_selective_scan_kernel<T, LN, NCH, false, false>;
                 cudaError_t err = allow_smem(kernel, G.bytes);
                 if (err != cudaSuccess) return err;
                 kernel<<<(unsigned)blocks, kScanThreads, G.bytes, st>>>(a);
@@ -1761,12 +1783,14 @@ cudaError_t launch_scan_step(const PdScanArgs& a, cudaStream_t st) {
         using T = decltype(e);
         return by_lanes(a.state, [&](auto ln) {
             constexpr int LN = decltype(ln)::value;
+            const bool vec = a.state == 4 * LN && a.vec_states && a.vec_params;
+            auto kernel = vec ? pd_selective_scan_step_kernel<T, LN, true> : pd_selective_scan_step_kernel<T, LN, false>;
+            const int threads = 32 * pd_step_warps(a.channels, a.groups, a.state, a.tok.seqs);
+            if (a.report) return describe(kernel, threads, 0, a.report);
             if (a.tok.seqs == 0) return cudaSuccess;
             const dim3 grid((unsigned)pd_step_blocks(a.channels, a.groups, a.state, a.tok.seqs),
                             (unsigned)((a.tok.seqs + a.run - 1) / a.run));
-            const bool vec = a.state == 4 * LN && a.vec_states && a.vec_params;
-            auto kernel = vec ? pd_selective_scan_step_kernel<T, LN, true> : pd_selective_scan_step_kernel<T, LN, false>;
-            kernel<<<grid, 32 * pd_step_warps(a.channels, a.groups, a.state, a.tok.seqs), 0, st>>>(a);
+            kernel<<<grid, threads, 0, st>>>(a);
             return cudaGetLastError();
         });
     });
@@ -1780,10 +1804,11 @@ cudaError_t launch_scan_grad(const PdScanArgs& a, cudaStream_t st) {
             const PdGradShape<LN, false> G(a.state, a.per_warp, sizeof(T));
             const int64_t per = a.channels / a.groups, tiles = (per + G.channels - 1) / G.channels;
             const int64_t blocks = tiles * a.groups * a.tok.seqs;
-            if (blocks > 0) {
+            if (blocks > 0 || a.report) {
                 auto kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true, true> : pd_selective_scan_grad_kernel<T, LN, false, true>;
                 if constexpr (LN == 4)
                     if (!one) kernel = a.z ? pd_selective_scan_grad_kernel<T, LN, true, false> : pd_selective_scan_grad_kernel<T, LN, false, false>;
+                if (a.report) return describe(kernel, kGradThreads, G.bytes, a.report);
                 cudaError_t err = allow_smem(kernel, G.bytes);
                 if (err != cudaSuccess) return err;
                 kernel<<<(unsigned)blocks, kGradThreads, G.bytes, st>>>(a);

@@ -23,7 +23,13 @@ struct PdTokens {
     int64_t seqs;
 };
 
+// What a launcher says of its kernel instead of launching it.
+struct PdScanReport {
+    int registers = -1, static_smem = -1, blocks_per_sm = -1;
+};
+
 struct PdConvArgs {
+    PdScanReport* report;     // non-null: describe, do not launch (no pointer is read)
     PdTokens tok;
     int type, width, silu;
     int64_t channels;
@@ -38,6 +44,7 @@ struct PdConvArgs {
 };
 
 struct PdScanArgs {
+    PdScanReport* report;     // as above
     PdTokens tok;
     int type, state, groups, softplus;
     int vec;                  // tokens can be read four channels at a time
@@ -182,5 +189,7 @@ int pd_scan_overlap(int family, int n_in, const void* const* in, const size_t* i
                     const size_t* out_bytes, char* err, size_t err_cap);
 int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
                    const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap);
+// The kernel that a call on aligned operands gets, on the current device; what cannot be had stays -1.
+PdScanReport pd_scan_describe(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan);
 
 #endif  // PD_SCAN_H_

@@ -194,6 +194,7 @@ int plan_conv(int family, const pd_causal_conv_params* p, const int64_t grid[3],
     plan->grid_y = plan->row_blocks;
     plan->launches = 2;
     plan->scratch_bytes = conv_partial(d, p->width, plan->row_blocks);
+    plan->dynamic_smem = 256 * conv_vector(d.channels) * 4;
     return PD_OK;
 }
 
@@ -238,11 +239,13 @@ int plan_scan(int family, const pd_selective_scan_params* p, const int64_t grid[
         const int64_t per = d.channels / p->groups;
         plan->items = grad_per_warp(p, d, sms);
         const int64_t tiles = (per + 4 * plan->items - 1) / (4 * plan->items) * p->groups;
+        plan->dynamic_smem = pd_scan_grad_bytes((int)p->state, (int)plan->items, (int)e);
         plan->free_blocks = scan_free_blocks(p, d, 1, sms);      // (in the launch that adds up the parameters' sums)
         plan->grid = tiles * d.seqs;
     } else {
         scan_cut(p, d, sms, plan);
         const int64_t tiles = scan_tiles(p, d, (int)plan->items);
+        plan->dynamic_smem = PdScanShape(pd_scan_lanes((int)p->state), (int)plan->items, (int)e).bytes;
         plan->free_blocks = scan_free_blocks(p, d, tiles, sms);
         plan->grid = tiles * (plan->segments + plan->free_blocks);
         plan->block = 128;
@@ -314,8 +317,11 @@ int pd_scan_overlap(int family, int n_in, const void* const* in, const size_t* i
     return PD_OK;
 }
 
-int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
-                   const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap) {
+namespace {
+// (report: the kernel is described instead, and no pointer is read)
+int scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
+                const void* const* in, void* const* out, void* scratch, cudaStream_t st, PdScanReport* report, char* err,
+                size_t err_cap) {
     const PdScanTable* table = math_mode == PD_MATH_SAFE ? pd_scan_table_safe()
                                : math_mode == PD_MATH_RELAXED ? pd_scan_table_relaxed() : pd_scan_table_fast();
     cudaError_t e;
@@ -324,6 +330,7 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         const pd_causal_conv_params* p = static_cast<const pd_causal_conv_params*>(params);
         PdConvArgs a;
         memset(&a, 0, sizeof(a));
+        a.report = report;
         const bool step = family == PD_FAMILY_CAUSAL_CONV_STEP, grad = family == PD_FAMILY_CAUSAL_CONV_GRAD;
         a.type = (int)p->type;
         a.width = (int)p->width;
@@ -361,6 +368,7 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         const pd_selective_scan_params* p = static_cast<const pd_selective_scan_params*>(params);
         PdScanArgs a;
         memset(&a, 0, sizeof(a));
+        a.report = report;
         const bool step = family == PD_FAMILY_SELECTIVE_SCAN_STEP, grad = family == PD_FAMILY_SELECTIVE_SCAN_GRAD;
         a.type = (int)p->type;
         a.state = (int)p->state;
@@ -423,4 +431,19 @@ int pd_scan_launch(int family, const void* params, int math_mode, const int64_t 
         return PD_ERR_CUDA;
     }
     return PD_OK;
+}
+}  // namespace
+
+int pd_scan_launch(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan,
+                   const void* const* in, void* const* out, void* scratch, cudaStream_t st, char* err, size_t err_cap) {
+    return scan_launch(family, params, math_mode, grid, plan, in, out, scratch, st, nullptr, err, err_cap);
+}
+
+PdScanReport pd_scan_describe(int family, const void* params, int math_mode, const int64_t grid[3], const PdScanPlan& plan) {
+    PdScanReport report;
+    void* operands[16];       // as many as a call can have; aligned, never read
+    for (void*& p : operands) p = reinterpret_cast<void*>((uintptr_t)256);
+    char err[64];
+    scan_launch(family, params, math_mode, grid, plan, operands, operands, operands[0], nullptr, &report, err, sizeof(err));
+    return report;
 }

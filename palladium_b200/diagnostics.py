@@ -30,7 +30,7 @@ class KernelDiagnostics:
     name, grid, threadgroup, msl_lines: as in the reference
     (src/palladium/diagnostics.py:21-39).  cuda_kernel .. blocks_per_sm: the
     CUDA launch the native library will perform for that grid; register,
-    shared-memory and occupancy figures are -1 where no GPU is present."""
+    static shared-memory and occupancy figures are -1 where no GPU is present."""
 
     name: str
     grid: tuple[int, ...]
@@ -45,6 +45,7 @@ class KernelDiagnostics:
     regs: int = -1
     smem_bytes: int = -1
     blocks_per_sm: int = -1
+    dynamic_smem_bytes: int = 0
 
     def __str__(self) -> str:
         parts = [f"palladium kernel {self.name}: grid={self.grid}"]
@@ -56,7 +57,9 @@ class KernelDiagnostics:
             parts.append(f"items_per_thread={self.items_per_thread}")
             parts.append(f"launches={self.launches}")
             if self.regs >= 0:
-                parts.append(f"regs={self.regs} smem={self.smem_bytes} blocks_per_sm={self.blocks_per_sm}")
+                parts.append(f"regs={self.regs} smem={self.smem_bytes}"
+                             + (f"+{self.dynamic_smem_bytes}" if self.dynamic_smem_bytes else "")
+                             + f" blocks_per_sm={self.blocks_per_sm}")
         return " ".join(parts)
 
 
@@ -108,6 +111,7 @@ def explain_spec(spec: KernelSpec, threadgroup=None, math_mode="fast") -> Kernel
         regs=int(info.regs_per_thread),
         smem_bytes=int(info.static_smem_bytes),
         blocks_per_sm=int(info.blocks_per_sm),
+        dynamic_smem_bytes=int(info.dynamic_smem_bytes),
     )
 
 

@@ -45,3 +45,50 @@ def test_element_types_are_still_told_apart():
     assert pl.as_dtype(record) == record and pl.dtype_name(record) != "bfloat16"
     for kind in (np.float32, np.uint32, np.int32, np.float64, np.float16, np.uint8, np.dtype(">f4")):
         assert pl.dtype_name(pl.as_dtype(kind)) == np.dtype(kind).name
+
+
+# ------------------------------------------------------------------ what explain says of a call's resources
+SCANS = [("bfloat16", 4, 2), ("bfloat16", 8, 4), ("bfloat16", 16, 5), ("bfloat16", 32, 5), ("bfloat16", 64, 3),
+         ("float32", 4, 1), ("float32", 8, 2), ("float32", 16, 4), ("float32", 32, 4), ("float32", 64, 2)]
+
+
+@pytest.mark.parametrize("dtype, state, blocks", SCANS)
+def test_shared_memory_of_the_prompt_kernel(dtype, state, blocks):
+    """An SM's 228 KB hold that many blocks, each with 1 KB of its own, or five where it would hold more."""
+    diag = explain(families.selective_scan(512, state, gate=True, dtype=dtype), (2, 96))
+    fit = 228 * 1024 // (diag.dynamic_smem_bytes + 1024)
+    assert min(fit, 5) == blocks and diag.dynamic_smem_bytes <= 227 * 1024
+
+
+def test_shared_memory_of_the_gradients_and_steps():
+    for state in (1, 4, 5, 8, 16, 17, 33, 64):
+        for dtype in ("float32", "bfloat16"):
+            for grid in ((1, 8), (40, 250), (120, 63)):
+                diag = explain(families.selective_scan_grad(9, state, gate=True, dtype=dtype), grid)
+                assert 0 < diag.dynamic_smem_bytes <= 227 * 1024
+    assert explain(families.causal_conv_grad(9), (2, 8)).dynamic_smem_bytes == 4096
+    assert explain(families.causal_conv_grad(9), (2, 7)).dynamic_smem_bytes == 1024
+    for family in (families.causal_conv(9), families.causal_conv_step(), families.selective_scan_step(16)):
+        assert explain(family, (2, 8)).dynamic_smem_bytes == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("math_mode", ["safe", "relaxed", "fast"])
+@pytest.mark.parametrize("dtype, state, blocks", SCANS)
+def test_blocks_of_the_prompt_kernel_on_a_multiprocessor(dtype, state, blocks, math_mode):
+    """Its registers leave room for as many blocks as its shared memory does."""
+    diag = explain(families.selective_scan(512, state, gate=True, dtype=dtype), (2, 96), math_mode)
+    assert diag.blocks_per_sm == blocks and 0 < diag.regs <= 255 and diag.smem_bytes == 0
+    assert f"smem=0+{diag.dynamic_smem_bytes} blocks_per_sm={blocks}" in str(diag)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("packed", [False, True])
+def test_registers_and_blocks_of_every_form(packed):
+    for family in (families.causal_conv(40, packed=packed), families.causal_conv_grad(40, silu=False, packed=packed),
+                   families.causal_conv_step(3, dtype="float16"), families.selective_scan_step(5, dtype="bfloat16"),
+                   families.selective_scan(40, 24, packed=packed, initial=True, final=True, carries=True),
+                   families.selective_scan_grad(40, 24, packed=packed, initial=True, final=True, gate=True)):
+        for grid in ((3, 20), (0, 20)):
+            diag = explain(family, grid)
+            assert 0 < diag.regs <= 255 and diag.blocks_per_sm >= 1 and diag.smem_bytes == 0, (family.name, grid)
