@@ -414,23 +414,23 @@ __global__ void __launch_bounds__(128) pd_causal_conv_step_kernel(PdConvArgs a) 
     if (lane >= lanes) return;
     const int64_t c = (int64_t)lane * V;
     for (int64_t s = blockIdx.y; s < a.tok.seqs; s += gridDim.y) {
-    pair_t win[W - 1][P], now[P], pre[P], w[W][P], b[P];
-    const int64_t at = s * (W - 1) * a.channels + c;
+        pair_t win[W - 1][P], now[P], pre[P], w[W][P], b[P];
+        const int64_t at = s * (W - 1) * a.channels + c;
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) load<V>((const T*)a.initial + at + i * a.channels, win[i]);
-    load<V>((const T*)a.x + s * a.channels + c, now);
-    conv_parameters<W, V>(a, c, w, b);
-    convolve<W, P>(w, b, win, now, pre);
-    if (a.silu) {
-        float out[V];
-        silu<V>(pre, out);
-        store<V>((T*)a.y + s * a.channels + c, out);
-    } else {
-        store<V>((T*)a.y + s * a.channels + c, pre);
-    }
-    slide<W - 1, P>(win, now);
+        for (int i = 0; i < W - 1; ++i) load<V>((const T*)a.initial + at + i * a.channels, win[i]);
+        load<V>((const T*)a.x + s * a.channels + c, now);
+        conv_parameters<W, V>(a, c, w, b);
+        convolve<W, P>(w, b, win, now, pre);
+        if (a.silu) {
+            float out[V];
+            silu<V>(pre, out);
+            store<V>((T*)a.y + s * a.channels + c, out);
+        } else {
+            store<V>((T*)a.y + s * a.channels + c, pre);
+        }
+        slide<W - 1, P>(win, now);
 #pragma unroll
-    for (int i = 0; i < W - 1; ++i) store<V>((T*)a.final_state + at + i * a.channels, win[i]);
+        for (int i = 0; i < W - 1; ++i) store<V>((T*)a.final_state + at + i * a.channels, win[i]);
     }
 }
 

@@ -8,7 +8,7 @@ import torch
 import palladium_b200 as pd
 from palladium_b200 import families
 from palladium_b200.pl import ShapeDtypeStruct
-from tests.state_space import Case, check
+from tests.state_space import TYPES, Case, check
 from tests.test_gpu_state_space import back, compare, device, run
 
 pytestmark = pytest.mark.gpu
@@ -216,3 +216,64 @@ def test_gradients_of_different_block_sizes_from_several_threads():
     for t in threads:
         t.join()
     assert not wrong
+
+
+# ------------------------------------------------------------------ memory of gradients and steps
+def shifted(tensor):
+    """The same values four bytes off a 16-byte boundary."""
+    step = 4 // tensor.element_size()
+    room = torch.empty(tensor.numel() + step, dtype=tensor.dtype, device="cuda")
+    room[step:] = tensor.reshape(-1)
+    return room[step:].view(tensor.shape)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+def test_gradients_off_a_16_byte_boundary(kind, dtype):
+    more = {} if kind == "conv" else dict(state=16, gate=True)
+    case = Case(kind, [9] * 50, 68, dtype=dtype, initial=True, final=True, **more)
+    carries = None
+    if kind == "scan":
+        carries = back(case.call(pd.cuda_call_jit, carries=True)(*[device(a) for a in case.operands()])[-1])
+        assert _reached(case, 3)
+    operands = [device(a) for a in case.operands(grad=True, carries=carries)]
+    call, want = case.call(pd.cuda_call_jit, "_grad"), case.oracle()
+    outs = call(*operands)
+    for move in range(len(operands)):
+        moved = [shifted(t) if i == move else t for i, t in enumerate(operands)]
+        check(case, case.grad_names(), [back(t) for t in call(*moved)], want)
+    got = call.on_device(*operands, out=[shifted(o) for o in outs])
+    check(case, case.grad_names(), [back(t) for t in got], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+def test_steps_off_a_16_byte_boundary(kind, dtype):
+    if kind == "conv":
+        family, order = families.causal_conv_step(dtype=dtype), ["x", "initial", "weight", "bias"]
+        case = Case("conv", [1] * 20, 16, dtype=dtype, initial=True, final=True)
+    else:
+        family = families.selective_scan_step(16, groups=2, gate=True, dtype=dtype)
+        order = ["initial", "x", "delta", "A", "B", "C", "bias", "skip", "z"]
+        case = Case("scan", [1] * 20, 16, dtype=dtype, state=16, groups=2, gate=True, initial=True, final=True)
+    call = pd.cuda_call_jit(family, grid=case.grid, out_shape=families.out_shapes(family, case.grid))
+    operands = [device(case.typed(n)) for n in order]
+    operands = [t.reshape(t.shape[:1] + t.shape[2:]) if n in ("x", "delta", "B", "C", "z") else t for n, t in zip(order, operands)]
+    want = case.oracle(grad=False)
+    outs = call(*operands)
+    for move in range(len(operands)):
+        moved = [shifted(t) if i == move else t for i, t in enumerate(operands)]
+        check(case, ["y", "final"], [back(t) for t in call(*moved)], want)
+    check(case, ["y", "final"], [back(t) for t in call.on_device(*operands, out=[shifted(o) for o in outs])], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("maker", [pd.cuda_call, pd.cuda_call_jit])
+@pytest.mark.parametrize("packed", [False, True])
+def test_scan_gradients_on_host_arrays(maker, dtype, packed):
+    lengths = [40, 40] if not packed else [40, 0, 33]
+    case = Case("scan", lengths, 20, dtype=dtype, packed=packed, gate=True, initial=True, final=True)
+    *forward, carries = case.call(maker, carries=True)(*case.operands())
+    want = case.oracle()
+    check(case, case.forward_names(), forward, want)
+    check(case, case.grad_names(), case.call(maker, "_grad")(*case.operands(grad=True, carries=carries)), want)
