@@ -396,7 +396,9 @@ def causal_conv_grad(length: int, width: int = 4, *, silu: bool = True, bias: bo
     """Gradients of `causal_conv` with the same constants.  Inputs: dy like y, then x,
     weight, bias, initial as there, dfinal (the gradient of final) with `final`, offsets
     with `packed`.  Outputs: dx, dweight float32, dbias float32 with `bias`, dinitial with
-    `initial`.  Sums run in a fixed order: equal calls on one device give equal bits."""
+    `initial`.  Sums run in a fixed order: equal calls on one device give equal bits.
+    (Results of `causal_conv` carry no autograd history: a `torch.autograd.Function` of the
+    caller's connects the two calls.)"""
     return _conv_family("causal_conv_grad", length, width, silu, bias, initial, final, packed, dtype)
 
 
@@ -455,7 +457,9 @@ def selective_scan_grad(length: int, state: int = 16, *, groups: int = 1, softpl
     dinitial float32 where the constants have them.  B and C are shared by the channels of
     a group and the parameters by all tokens: their sums are float32 in a fixed order, so
     equal calls on one device give equal bits.  Scratch: about 8 bytes per token, state and
-    block of up to 24 channels (`call.explain(...).scratch_bytes` says how much)."""
+    block of up to 24 channels (`call.explain(...).scratch_bytes` says how much).
+    (Results of `selective_scan` carry no autograd history: a `torch.autograd.Function` of the
+    caller's connects the two calls.)"""
     return _scan_family("selective_scan_grad", length, state, groups, softplus, bias, skip, gate, initial, final, False,
                         packed, dtype)
 

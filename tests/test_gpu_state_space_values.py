@@ -1,6 +1,9 @@
 """Values of the state-space families where float32's range or a rounding decides, on a GPU against the float64
 operators inside the bounds of their running error analysis."""
 
+import re
+from pathlib import Path
+
 import numpy as np
 import pytest
 import torch
@@ -277,3 +280,29 @@ def test_scan_gradients_on_host_arrays(maker, dtype, packed):
     want = case.oracle()
     check(case, case.forward_names(), forward, want)
     check(case, case.grad_names(), case.call(maker, "_grad")(*case.operands(grad=True, carries=carries)), want)
+
+
+# ------------------------------------------------------------------ through torch.autograd
+def test_the_readme_connects_the_scan_to_autograd():
+    """The README's lines as they stand, in bfloat16: gradients of every operand against differentiating the formula in
+    float64, a layer's input used once more beside the scan; and a backward pass whose incoming gradient is expanded."""
+    text = (Path(__file__).resolve().parent.parent / "README.md").read_text()
+    code = next(b for b in re.findall(r"```python\n(.*?)```", text, re.S) if "class SelectiveScan" in b)
+    case = Case("scan", [50, 50], 24, dtype="bfloat16", state=16, gate=True, seed=4)
+    names = ["u", "delta", "A", "B", "C", "delta_bias", "skip", "z"]
+    operands = [device(a).requires_grad_() for a in case.operands()]
+    space = dict(torch=torch, pd=pd, families=families, batch=2, channels=24, length=50, **dict(zip(names, operands)))
+    exec(code, space)
+    y = space["y"]
+    check(case, ["y"], [back(y.detach())])
+    dy = device(case.typed("dy"))
+    grads = torch.autograd.grad(y, operands, dy, retain_graph=True)
+    check(case, case.grad_names(), [back(g) for g in grads])
+    both = torch.autograd.grad(y + operands[0], operands[0], dy, retain_graph=True)[0]       # the sum of two paths, rounded once more
+    assert torch.equal(both, (grads[0].float() + dy.float()).bfloat16())
+    ones = torch.autograd.grad(y.sum(), operands)
+    case.v["dy"][:] = 1.0
+    check(case, case.grad_names(), [back(g) for g in ones])
+    with torch.no_grad():
+        assert not space["SelectiveScan"].apply(*operands).requires_grad
+    assert not space["forward"](*operands)[0].requires_grad
