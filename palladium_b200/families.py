@@ -349,9 +349,13 @@ def _element_type(what: str, dtype) -> str:
 
 
 def _whole(what: str, name: str, value, low: int, high: int) -> int:
-    if isinstance(value, bool) or int(value) != value or not low <= value <= high:
+    try:
+        whole = int(value) if not isinstance(value, bool) and int(value) == value else None
+    except (TypeError, ValueError, OverflowError):      # None, text, NaN, infinities
+        whole = None
+    if whole is None or not low <= whole <= high:
         raise TraceError(f"{what}: {name} must be a whole number in [{low}, {high}], got {value!r}")
-    return int(value)
+    return whole
 
 
 def _conv_family(name: str, length, width, silu, bias, initial, final, packed, dtype) -> Family:

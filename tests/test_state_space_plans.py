@@ -27,6 +27,15 @@ def test_channels_per_warp_of_the_gradient_fit_the_multiprocessor(dtype, state, 
     assert 2 <= diag.items_per_thread <= most
 
 
+# ------------------------------------------------------------------ constants
+@pytest.mark.parametrize("length", [float("nan"), float("inf"), -float("inf"), None, "eight", "8", [8], True, 8.5, 2 ** 31])
+def test_lengths_that_are_no_whole_numbers_are_refused(length):
+    for make in (families.causal_conv, families.selective_scan_grad):
+        with pytest.raises(pd.TraceError, match="length must be a whole number"):
+            make(length)
+    assert families.causal_conv(np.int64(8)).constants["length"] == families.causal_conv(8.0).constants["length"] == 8
+
+
 # ------------------------------------------------------------------ what every call pays
 def test_reading_an_element_type_costs_little():
     """Every call on host arrays, of any family, reads each operand's type: spelling the type out for it once cost
