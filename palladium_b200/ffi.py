@@ -32,7 +32,7 @@ from . import _native
 from .diagnostics import KernelDiagnostics, explain_spec, log_compile
 from .dispatch import BoundKernel, bind
 from .errors import DispatchError, UnsupportedPrimitiveError
-from .families import Family, KernelSpec, trace
+from .families import STATE_SPACE, Family, KernelSpec, trace
 from .interpret import interpret_callable
 from .math_mode import MathMode, math_mode_ordinal
 from .pl import ShapeDtypeStruct, as_dtype, dtype_name
@@ -245,6 +245,11 @@ class FfiCallable:
         device = args[0].device if args else torch.device("cuda", torch.cuda.current_device())
         if out is not None:
             outs = list(out) if isinstance(out, (list, tuple)) else [out]
+            if spec.family.name in STATE_SPACE:     # (whose element types include two of the same size)
+                for i, (t, info) in enumerate(zip(outs, spec.outputs)):
+                    if getattr(t, "dtype", None) != torch_dtype[dtype_name(info.dtype)]:
+                        raise DispatchError(f"output {i}: dtype {getattr(t, 'dtype', type(t).__name__)} does not match the "
+                                            f"{dtype_name(info.dtype)} that the call writes")
         else:
             outs = [torch.empty(info.array_shape, dtype=torch_dtype[dtype_name(info.dtype)], device=device)
                     for info in spec.outputs]

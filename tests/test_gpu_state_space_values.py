@@ -11,7 +11,7 @@ import torch
 import palladium_b200 as pd
 from palladium_b200 import families
 from palladium_b200.pl import ShapeDtypeStruct
-from tests.state_space import TYPES, Case, check
+from tests.state_space import TYPES, Case, check, wide
 from tests.test_gpu_state_space import back, compare, device, run
 
 pytestmark = pytest.mark.gpu
@@ -306,3 +306,27 @@ def test_the_readme_connects_the_scan_to_autograd():
     with torch.no_grad():
         assert not space["SelectiveScan"].apply(*operands).requires_grad
     assert not space["forward"](*operands)[0].requires_grad
+
+
+# ------------------------------------------------------------------ results' memory
+def test_results_of_another_type_are_refused():
+    """float16 and bfloat16 are of one size: bits of one in a tensor of the other would be other numbers."""
+    case = Case("scan", [9, 9], 16, dtype="bfloat16", final=True)
+    call = case.call(pd.cuda_call_jit)
+    operands = [device(a) for a in case.operands()]
+    y, final = call(*operands)
+    for wrong in ((y.view(torch.float16), final), (y.view(torch.int16), final), (y, final.view(torch.int32))):
+        with pytest.raises(pd.DispatchError, match="does not match the .* that the call writes"):
+            call.on_device(*operands, out=wrong)
+    got = call.on_device(*operands, out=(torch.empty_like(y), torch.empty_like(final)))
+    assert torch.equal(got[0], y) and torch.equal(got[1], final)
+
+
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+def test_packed_calls_without_any_sequence(kind):
+    """A buffer of free rows alone: zeros, and sums of nothing."""
+    for lead, spare in ((0, 300), (7, 0), (100, 50)):
+        case = Case(kind, [], 20, dtype="float16", packed=True, lead=lead, spare=spare, initial=True, final=True)
+        forward, grads = run(case)
+        assert (wide(forward[0]) == 0).all() and forward[0].shape == (lead + spare, 20) and forward[1].size == 0
+        assert all((wide(g) == 0).all() for g in grads)
