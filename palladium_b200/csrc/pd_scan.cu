@@ -1401,74 +1401,70 @@ __global__ void __launch_bounds__(kGradThreads, 3) pd_selective_scan_grad_kernel
 #pragma unroll
                     for (int p = 0; p < 2; ++p)
                         e[p] = mul2(w[i][p], i == K - 1 ? mul2(C[i][p], gg[i]) : mad2(C[i][p], gg[i], e[p]));
+                // scans over the token groups.  The first group takes in the state kept for the chunk, the last the
+                // gradient that follows it; their decay then counts as zero, so that a group that has seen
+                // everything before it adds nothing more (a shuffle from beyond the edge returns the lane's own value).
+                const bool scans = within_range<TL>(up);
                 pair_t in[2];
-                if (within_range<TL>(up)) {
-                    // scans over the token groups.  The first group takes in the state kept for the chunk, the last the
-                    // gradient that follows it; their decay then counts as zero, so that a group that has seen
-                    // everything before it adds nothing more (a shuffle from beyond the edge returns the lane's own value).
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    in[p] = h[K][p];
+                    down[p] = up[p];
+                    in[p] = mad2(up[p], tl == 0 ? entry[p] : 0, in[p]);
+                    e[p] = mad2(down[p], tl == TL - 1 ? leave[p] : 0, e[p]);
+                    up[p] = tl == 0 ? 0 : up[p];
+                    down[p] = tl == TL - 1 ? 0 : down[p];
+                }
+#pragma unroll
+                for (int off = 1; off < TL; off *= 2)
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
-                        in[p] = h[K][p];
-                        down[p] = up[p];
-                        in[p] = mad2(up[p], tl == 0 ? entry[p] : 0, in[p]);
-                        e[p] = mad2(down[p], tl == TL - 1 ? leave[p] : 0, e[p]);
-                        up[p] = tl == 0 ? 0 : up[p];
-                        down[p] = tl == TL - 1 ? 0 : down[p];
-                    }
-#pragma unroll
-                    for (int off = 1; off < TL; off *= 2)
-#pragma unroll
-                        for (int p = 0; p < 2; ++p) {
-                            in[p] = mad2(up[p], shift_up(in[p], off * LN), in[p]);
-                            e[p] = mad2(down[p], shift_down(e[p], off * LN), e[p]);
-                            if (2 * off < TL) {
-                                up[p] = mul2(up[p], shift_up(up[p], off * LN));
-                                down[p] = mul2(down[p], shift_down(down[p], off * LN));
-                            }
-                        }
-                    __syncwarp();
-                    if (tl == 0) {
-                        *reinterpret_cast<pair_t*>(kept) = e[0];
-                        *reinterpret_cast<pair_t*>(kept + 2) = e[1];
-                    }
-                    // the true states
-#pragma unroll
-                    for (int p = 0; p < 2; ++p) {
-                        in[p] = shift_up(in[p], LN);
-                        e[p] = shift_down(e[p], LN);
-                        in[p] = tl == 0 ? entry[p] : in[p];
-                        e[p] = tl == TL - 1 ? leave[p] : e[p];
-                        h[0][p] = in[p];
-#pragma unroll
-                        for (int i = 0; i < K; ++i) {
-                            in[p] = mul2(in[p], w[i][p]);
-                            h[i + 1][p] = add2(h[i + 1][p], in[p]);
+                        in[p] = mad2(up[p], shift_up(in[p], off * LN), in[p]);
+                        e[p] = mad2(down[p], shift_down(e[p], off * LN), e[p]);
+                        if (2 * off < TL) {
+                            up[p] = mul2(up[p], shift_up(up[p], off * LN));
+                            down[p] = mul2(down[p], shift_down(down[p], off * LN));
                         }
                     }
-                } else {
+                if (!scans) {
                     // growing rates: group after group, token after token, no product of decays
 #pragma unroll
                     for (int p = 0; p < 2; ++p) {
                         pair_t now = entry[p];
 #pragma unroll 1
                         for (int t = 0; t < TL; ++t) {
-                            if (tl == t) h[0][p] = now;
 #pragma unroll
                             for (int i = 0; i < K; ++i) now = mad2(w[i][p], now, mul2(u[i], B[i][p]));
+                            if (tl == t) in[p] = now;
                             now = from_lane(now, t * LN + sub);
                         }
-#pragma unroll
-                        for (int i = 0; i < K; ++i) h[i + 1][p] = mad2(w[i][p], h[i][p], mul2(u[i], B[i][p]));
                         now = leave[p];
 #pragma unroll 1
                         for (int t = TL - 1; t >= 0; --t) {
-                            if (tl == t) e[p] = now;
 #pragma unroll
                             for (int i = K - 1; i >= 0; --i) now = mul2(w[i][p], mad2(C[i][p], gg[i], now));
+                            if (tl == t) e[p] = now;
                             now = from_lane(now, t * LN + sub);
                         }
-                        __syncwarp();
-                        if (tl == 0) *reinterpret_cast<pair_t*>(kept + 2 * p) = now;
+                    }
+                }
+                __syncwarp();
+                if (tl == 0) {
+                    *reinterpret_cast<pair_t*>(kept) = e[0];
+                    *reinterpret_cast<pair_t*>(kept + 2) = e[1];
+                }
+                // the true states
+#pragma unroll
+                for (int p = 0; p < 2; ++p) {
+                    in[p] = shift_up(in[p], LN);
+                    e[p] = shift_down(e[p], LN);
+                    in[p] = tl == 0 ? entry[p] : in[p];
+                    e[p] = tl == TL - 1 ? leave[p] : e[p];
+                    h[0][p] = in[p];
+#pragma unroll
+                    for (int i = 0; i < K; ++i) {
+                        in[p] = mul2(in[p], w[i][p]);
+                        h[i + 1][p] = add2(h[i + 1][p], in[p]);
                     }
                 }
                 if (GATE)
