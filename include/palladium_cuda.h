@@ -213,7 +213,8 @@ typedef struct pd_source_kernel_params {
  * (length, D), `length` rows in all, sequence s in rows [offsets[s],
  * offsets[s + 1]) with int32 offsets (S + 1).  Offsets are clamped to
  * [0, length] and a decreasing pair is an empty sequence; output rows of no
- * sequence are zero.  Parameters and recurrent states are float32.  Arithmetic
+ * sequence, before the first and behind the last one, are zero.  Beside a
+ * decreasing pair other sequences' results are undefined (no array is left).  Parameters and recurrent states are float32.  Arithmetic
  * is float32, rounded once at the store.  Zero values in a flag leave the
  * operands and results in [ ] out.  Scratch (the gradients' partial sums, the
  * states between the segments of a long prompt) comes from `workspace`, or from the library's pool, which a stream that is

@@ -237,12 +237,13 @@ __device__ __forceinline__ int64_t first_chunk(const PdTokens& t, int64_t s, int
 // causal convolution:  y_t = act(bias + sum_j w[W-1-j] x_{t-j})
 // One thread owns V channels and a run of consecutive rows; the last W - 1
 // inputs stay in registers, so a row is read once apart from the run's halo.
-// Bound: memory, 2 bytes in and 2 out per bf16 element; next to them stand two
-// special-function operations (30 us of the 41 that 2 x 134 MB take) and two
-// packed multiply-adds, so what matters is to keep rows in flight: four of them
-// per thread, with four blocks of 256 threads on an SM (8 x 2048 x 4096 bf16 took
-// 82 us with two blocks and the next four rows fetched ahead, 76 with eight
-// channels per thread).
+// Bound: the latency of its rows.  8 x 2048 x 4096 in bf16 take 58 us, where memory,
+// 2 bytes in and 2 out per element, asks for 41 and two special-function
+// operations for 30; a warp waits on loads 8 of every 13 cycles.  So what matters
+// is to keep rows in flight: four of them per thread, with four blocks of 256
+// threads on an SM (82 us with two blocks and the next four rows fetched ahead, 76
+// with eight channels per thread).  At their 64 registers width 4 spills 44 bytes in
+// bf16 and 72 in float32.
 // ===========================================================================
 // the taps and the bias of V channels, as 16-byte vectors where the channels are
 template <int W, int V>
@@ -1232,9 +1233,8 @@ __global__ void __launch_bounds__(kScanThreads, PdScanShape(LN, NCH, sizeof(T)).
 // while a warp goes through its channels; only their sum over the four warps passes through shared memory.
 // LN == K, and after the sums over a token's LN lanes each lane finishes one token.
 //
-// Bound: instruction issue.  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 620 us: 38 instructions per
-// state, 9.4 of them the packed arithmetic, 3.6 shuffles, at 0.51 a clock and scheduler with three blocks of 168
-// registers on an SM (eight warps of 128 registers a block spilled, 1120 us; operands read where they are used
+// Bound: instruction issue.  4 x 2048 tokens x 2048 channels x 16 states in bf16 take 640 us: 41 instructions per
+// state at 0.53 a clock and scheduler with three blocks of 168 registers on an SM (eight warps of 128 registers a block spilled, 1120 us; operands read where they are used
 // instead of a chunk ahead, 1030 us).
 // ---------------------------------------------------------------------------
 constexpr int kGradThreads = 32 * PD_SCAN_GRAD_WARPS;

@@ -380,8 +380,8 @@ def causal_conv(length: int, width: int = 4, *, silu: bool = True, bias: bool = 
     are (length, D) with `length` rows in all; the last operand, offsets (S + 1,)
     int32, gives sequence s the rows offsets[s] .. offsets[s + 1] - 1.  It is read on
     the device: values are clamped to [0, length], a decreasing pair is an empty
-    sequence, rows of no sequence come out as zeros.  Sequences that overlap
-    (offsets out of order) have undefined results.
+    sequence, rows before the first and behind the last sequence come out as zeros.
+    Beside a decreasing pair other sequences' results are undefined.
 
     `dtype`: float32, float16 or bfloat16 (`pl.bfloat16`, torch.bfloat16), the type
     of x, y, initial and final.  Sums are float32, rounded once."""
