@@ -5,6 +5,8 @@ here computed by oracle/ for each kernel family."""
 import numpy as np
 
 import oracle
+from palladium_b200 import families
+from tests import state_space
 
 
 def interpret(family, pallas_kwargs, *args, pow_flavour="pd"):
@@ -63,4 +65,6 @@ def interpret(family, pallas_kwargs, *args, pow_flavour="pd"):
         if c["op"] == "fold_in":
             return oracle.fold_in(args[0], args[1])
         return oracle.fold_uniform(args[0], n, c["count"])
+    if name in families.STATE_SPACE:
+        return state_space.interpret(family, pallas_kwargs["grid"], *args)
     raise NotImplementedError(name)

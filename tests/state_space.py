@@ -170,3 +170,60 @@ def check(case, names, results, want=None):
         bad = ~(off <= most)
         assert not bad.any(), (f"{name}: {bad.sum()} of {bad.size} values outside; worst {np.nanmax(off / most):.3g} times "
                                f"the tolerance at {np.unravel_index(np.nanargmax(off / most), off.shape)}")
+
+
+# -- the operators as `.interpret` gives them: from a call's arrays to its results, float64 rounded once ------------
+def interpret(family, grid, *args):
+    """What a call of `family` on host arrays returns, from the oracle."""
+    c, form = family.constants, family.name
+    seqs, channels = grid
+    scan, step, grad = form.startswith("selective_scan"), form.endswith("_step"), form.endswith("_grad")
+    names = ["x", "delta", "A", "B", "C"] if scan else ["x", "weight"]
+    names += [n for n in ("bias", "skip", "z") if c.get("gate" if n == "z" else n)]
+    if step:
+        names = ["initial"] + names if scan else ["x", "initial"] + names[1:]
+    elif grad:
+        names = ["dy"] + names + (["carries"] if scan else ["initial"] * c["initial"]) + ["dfinal"] * c["final"]
+    else:
+        names += ["initial"] * c["initial"]
+    names += ["offsets"] * c["packed"]
+    assert len(names) == len(args)
+    v = {n: (np.asarray(a) if n == "offsets" else wide(np.asarray(a))) for n, a in zip(names, args)}
+    length = 1 if step else c["length"]
+    rows = length if c["packed"] else seqs * length
+    starts = [int(o) for o in np.clip(v["offsets"], 0, rows)] if c["packed"] else [s * length for s in range(seqs + 1)]
+    flat = {n: v[n].reshape((rows,) + v[n].shape[-1 if n in ("x", "dy", "delta", "z") else -2:]) for n in
+            ("x", "dy", "delta", "z", "B", "C") if n in v}
+    initial = v.get("initial")
+    if scan and grad:
+        initial = np.zeros((seqs, channels, c["state"]))
+        for s in range(seqs):
+            if starts[s + 1] > starts[s]:
+                initial[s] = v["carries"][starts[s] // families.SCAN_CHUNK + s] if c["packed"] else v["carries"][s, 0]
+    given = dict(dy=flat.get("dy"), dfinal=v.get("dfinal"))
+
+    def run(starts, initial, **more):
+        if scan:
+            return S.selective_scan(flat["x"], flat["delta"], v["A"], flat["B"], flat["C"], starts, v.get("bias"),
+                                    v.get("skip"), flat.get("z"), initial, softplus_=c["softplus"], **more)
+        return S.causal_conv(flat["x"], v["weight"], v.get("bias"), starts, initial, silu=c["silu"], **more)
+
+    found = {n: r.value for n, r in run(starts, initial, **given).items()}
+    if c.get("carries"):
+        kept = found["carries"] = np.zeros(families.out_shapes(family, grid)[-1].shape)
+        for s in range(seqs):
+            for k in range(-(-(starts[s + 1] - starts[s]) // families.SCAN_CHUNK)):
+                before = run([starts[s], starts[s] + k * families.SCAN_CHUNK], None if initial is None else initial[s:s + 1])
+                kept[(starts[s] // families.SCAN_CHUNK + s + k,) if c["packed"] else (s, k)] = before["final"].value[0]
+    if not grad:
+        order = ["y"] + ["final"] * (step or c["final"]) + ["carries"] * bool(c.get("carries"))
+    elif scan:
+        order = ["dx", "ddelta", "dA", "dB", "dC"] + [n for n, f in (("dbias", "bias"), ("dskip", "skip"), ("dz", "gate"),
+                                                                     ("dinitial", "initial")) if c[f]]
+    else:
+        order = ["dx", "dweight"] + [n for n, f in (("dbias", "bias"), ("dinitial", "initial")) if c[f]]
+    shapes = families.out_shapes(family, grid)
+    shapes = shapes if isinstance(shapes, tuple) else (shapes,)
+    results = tuple(host(rounded(found[n], pl.dtype_name(o.dtype)), pl.dtype_name(o.dtype)).reshape(o.shape)
+                    for n, o in zip(order, shapes, strict=True))
+    return results[0] if len(results) == 1 else results

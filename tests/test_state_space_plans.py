@@ -7,6 +7,8 @@ import pytest
 
 import palladium_b200 as pd
 from palladium_b200 import families, pl
+from tests.oracle_provider import interpret
+from tests.state_space import Case, check
 
 
 def explain(family, grid, math_mode="fast"):
@@ -101,3 +103,40 @@ def test_registers_and_blocks_of_every_form(packed):
         for grid in ((3, 20), (0, 20)):
             diag = explain(family, grid)
             assert 0 < diag.regs <= 255 and diag.blocks_per_sm >= 1 and diag.smem_bytes == 0, (family.name, grid)
+
+
+# ------------------------------------------------------------------ interpret
+@pytest.fixture
+def provider():
+    previous = pd.register_interpret_provider(interpret)
+    yield
+    pd.register_interpret_provider(previous)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+@pytest.mark.parametrize("packed", [False, True])
+def test_interpret_reaches_prompts_and_gradients(provider, packed, kind, dtype):
+    more = dict(state=3, groups=2, gate=True) if kind == "scan" else {}
+    case = Case(kind, [70, 0, 33] if packed else [40, 40], 4, dtype=dtype, packed=packed, lead=2 * packed, spare=packed,
+                initial=True, final=True, **more)
+    call = case.call(pd.cuda_call, **({"carries": True} if kind == "scan" else {}))
+    forward = list(call.interpret(*case.operands()))
+    carries = forward.pop() if kind == "scan" else None
+    check(case, case.forward_names(), forward)
+    # (the gradient starts from the carries, float32, so from the initial state itself)
+    check(case, case.grad_names(), case.call(pd.cuda_call_jit, "_grad").interpret(*case.operands(grad=True, carries=carries)))
+
+
+@pytest.mark.parametrize("kind", ["conv", "scan"])
+def test_interpret_reaches_single_tokens(provider, kind):
+    case = Case(kind, [1] * 5, 4, initial=True, final=True, **(dict(state=3, gate=True) if kind == "scan" else {}))
+    if kind == "conv":
+        family, order = families.causal_conv_step(), ["x", "initial", "weight", "bias"]
+    else:
+        family = families.selective_scan_step(3, gate=True)
+        order = ["initial", "x", "delta", "A", "B", "C", "bias", "skip", "z"]
+    operands = [case.typed(n) for n in order]
+    operands = [a.reshape(a.shape[:1] + a.shape[2:]) if n in ("x", "delta", "B", "C", "z") else a for n, a in zip(order, operands)]
+    call = pd.cuda_call(family, grid=case.grid, out_shape=families.out_shapes(family, case.grid))
+    check(case, ["y", "final"], call.interpret(*operands), case.oracle(grad=False))
