@@ -89,7 +89,7 @@ int64_t scan_chunks(const pd_selective_scan_params* p, const Dims& d) {
 // 744, 767, 687, 763 us, of which it takes 687; float32 x 16 states 1031, 765, 716, 751, 810, 908, of which 716).
 int grad_per_warp(const pd_selective_scan_params* p, const Dims& d, int sms) {
     const int64_t per = d.channels / p->groups;
-    const int most = p->state > 16 ? 4 : 6;    // (the sums' staging has room for six, the wide states' for four)
+    const int most = p->state > 16 ? 4 : 6;    // (more were not measured)
     int best = 1;
     int64_t least = INT64_MAX;
     for (int n = most; n >= 1; --n) {
