@@ -4,6 +4,7 @@
 #include "../../include/palladium_cuda.h"
 #include "pd_scan.h"
 
+#include <math.h>
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>
@@ -117,17 +118,26 @@ int64_t scan_tiles(const pd_selective_scan_params* p, const Dims& d, int per_lan
 // channels x 16 states: 571 against 604 us; 4 x 2048 x 2048: 211 against 182).  Cutting a sequence into segments
 // costs a first pass over all but its last, which takes two thirds of the second's time: it pays where a call has
 // fewer than two blocks per SM (1 x 8192 x 2048: 16 segments 252 us; 4 x 2048 x 2048: uncut 182 us,
-// two segments 236).  A packed call is cut at three times an even share, so that one long sequence does not
+// two segments 236).  A block composes the states of all segments before its own, one after another, so a sequence is
+// cut into half the root of its length at most (1 x 131072 x 16 bf16 in 2048, 512, 181, 128, 64 segments: 1106, 188, 136,
+// 120, 173 us; 1 x 2^20 x 16 in 2072, 512, 128: 1384, 419, 622).  A packed call is cut at three times an even share, so that one long sequence does not
 // outlast all others (17 of them, 8200 x 2560: 249 us, cut at 1024 tokens 298).
 void scan_cut(const pd_selective_scan_params* p, const Dims& d, int sms, PdScanPlan* plan) {
     const int64_t seqs = d.seqs > 0 ? d.seqs : 1, rows = d.rows > 0 ? d.rows : 1, mean = (rows + seqs - 1) / seqs;
-    const int64_t most = mean / 64 > 0 ? mean / 64 : 1;
+    const int64_t root = (int64_t)(sqrt((double)mean) / 2), least = mean / 64;
+    const int64_t most = least < 1 ? 1 : least < root ? least : root;
     const int per_lane = p->state > 32 || (p->state > 8 && scan_tiles(p, d, 2) * seqs >= (int64_t)sms * 12) ? 2 : 1;
     const int64_t tiles = scan_tiles(p, d, per_lane);
     int64_t cuts = tiles * seqs < sms * 2 ? (int64_t)sms * 14 / (tiles * seqs) : 1, segment = INT32_MAX;
     if (cuts > most) cuts = most;
-    if (cuts > 1) segment = (mean + cuts - 1) / cuts;
-    else if (p->packed) segment = rows * tiles / ((int64_t)sms * 4) * 3;
+    if (cuts > 1) {
+        segment = (mean + cuts - 1) / cuts;
+        const int64_t floor = (int64_t)sqrt((double)rows);
+        // (one sequence may have nearly all the rows: 131072 tokens and 63 x 16 beside them, 16 channels, took 601 us
+        // without this floor and take 151; 64 x 2048 tokens 62 either way)
+        if (p->packed && segment < floor) segment = floor;
+    }
+    if (cuts <= 1 && p->packed) segment = rows * tiles / ((int64_t)sms * 4) * 3;
     if (segment < 64) segment = 64;
     segment = (segment + PD_SCAN_CHUNK - 1) / PD_SCAN_CHUNK * PD_SCAN_CHUNK;     // (carries are kept at whole chunks)
     plan->items = per_lane;

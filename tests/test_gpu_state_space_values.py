@@ -330,3 +330,14 @@ def test_packed_calls_without_any_sequence(kind):
         forward, grads = run(case)
         assert (wide(forward[0]) == 0).all() and forward[0].shape == (lead + spare, 20) and forward[1].size == 0
         assert all((wide(g) == 0).all() for g in grads)
+
+
+# ------------------------------------------------------------------ many segments
+@pytest.mark.parametrize("lengths", [[9000], [8000, 3, 0, 200, 1]])
+def test_sequences_of_many_segments(lengths):
+    """Some forty segments, or a sequence that has nearly all the rows of a packed call: every state between them right."""
+    packed = len(lengths) > 1
+    case = Case("scan", lengths, 5, packed=packed, state=4, gate=True, initial=True, final=True)
+    diag = case.call(pd.cuda_call).explain(*case.operands())
+    assert diag.launches == 2 and diag.cuda_grid[0] > 40
+    compare(case)

@@ -29,6 +29,14 @@ def test_channels_per_warp_of_the_gradient_fit_the_multiprocessor(dtype, state, 
     assert 2 <= diag.items_per_thread <= most
 
 
+@pytest.mark.parametrize("length, channels, most", [(131072, 16, 181), (32768, 64, 90), (2 ** 20, 16, 512), (8192, 2048, 16)])
+def test_segments_of_a_long_prompt_over_few_channels(length, channels, most):
+    """A block composes the states of all segments before its own: half the root of the length is what pays."""
+    diag = explain(families.selective_scan(length, 16, dtype="bfloat16"), (1, channels))
+    tiles = -(-channels // 16)
+    assert diag.launches == 2 and most // 2 <= diag.cuda_grid[0] // tiles <= most
+
+
 # ------------------------------------------------------------------ constants
 @pytest.mark.parametrize("length", [float("nan"), float("inf"), -float("inf"), None, "eight", "8", [8], True, 8.5, 2 ** 31])
 def test_lengths_that_are_no_whole_numbers_are_refused(length):
